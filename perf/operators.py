@@ -9,7 +9,7 @@ A block of 32 values is a byte e and 16 bytes of codes (value j in the low nibbl
   experts  MUL_MAT_ID by the matrices of MXFP4 experts, and ADD_ID of the experts' bias rows: a decode step, a few tokens, a prompt
 
 A product takes its activations as whole numbers q of -255 .. 255 times a power of two, a block of 32 each (q = rint(x 2^-s), s the exponent of the block's largest magnitude rounded to 8
-significant bits, less 7): the counterpart of the 8-bit activation blocks that the products by the other block formats use.
+significant bits, less 7, within -120 .. 120): the counterpart of the 8-bit activation blocks that the products by the other block formats use.
 """
 import ctypes as C
 import math
@@ -20,7 +20,7 @@ import torch
 own = False  # True: the framework's operators; False: the plain form of the same
 
 VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
-MIN_STEP = -120  # exponent of the smallest step of an activation block
+STEPS = 120  # exponents of an activation block's step: -STEPS .. STEPS
 
 
 def _rows(name, kind, width, rows, taken):
@@ -111,8 +111,8 @@ def _activations(x):
     top = b.abs().amax(-1, keepdim=True)
     good = torch.isfinite(top)
     frac, e = torch.frexp(torch.where(good, top, torch.ones_like(top)))
-    step = (e + (frac >= 255.5 / 256) - 8).clamp(min=MIN_STEP)
-    q = torch.round(torch.ldexp(b, -step))
+    step = (e + (frac >= 255.5 / 256) - 8).clamp(-STEPS, STEPS)
+    q = torch.round(torch.ldexp(b, -step)).clamp(-255, 255)
     return torch.where(good, torch.ldexp(q, step), torch.full_like(q, math.nan)).flatten(-2)
 
 
@@ -308,9 +308,9 @@ def _exact_activations(x):
     b = x.double().reshape(*x.shape[:-1], -1, 32)
     top = b.abs().max(-1, keepdim=True)[0]
     s = torch.floor(torch.log2(torch.where(top > 0, top, 2.0**-200))) - 7
-    s = torch.where(torch.round(top / torch.pow(2.0, s)) > 255, s + 1, s).clamp(min=MIN_STEP)
+    s = torch.where(torch.round(top / torch.pow(2.0, s)) > 255, s + 1, s).clamp(-STEPS, STEPS)
     unit = torch.pow(2.0, s)
-    return torch.where(torch.isfinite(top), torch.round(b / unit) * unit, torch.nan).reshape(x.shape)
+    return torch.where(torch.isfinite(top), torch.round(b / unit).clamp(-255, 255) * unit, torch.nan).reshape(x.shape)
 
 
 def exact(case, seed):
