@@ -152,15 +152,30 @@ def _plain(s):
 
 
 # ------------------------------------------------------------------------------------------ the framework's operators
-class _Memory:
-    """f32 memory of the backend as an array that torch reads in place"""
+class _Kept:
+    """What the backend's memory of one case hangs on: given back when neither the graph nor an output of it is left."""
 
-    def __init__(self, address, shape):
+    def __init__(self, L):
+        self.H, self.bufs = L.host(), []
+        self.ctxs = [self.H.ggml_init(L.InitParams(0, None, True)) for _ in range(2)]
+
+    def __del__(self):
+        for b in self.bufs:
+            self.H.ggml_backend_buffer_free(b)
+        for k in self.ctxs:
+            self.H.ggml_free(k)
+
+
+class _Memory:
+    """f32 memory of the backend as an array that torch reads in place; the tensor made of it keeps it, and it keeps the memory"""
+
+    def __init__(self, kept, address, shape):
+        self.kept = kept
         self.__cuda_array_interface__ = {"shape": shape, "typestr": "<f4", "data": (address, False), "strides": None, "version": 2}
 
 
 class _Graph:
-    """The graph of one case with its tensors in the backend's memory, as an engine keeps them; given back with the last reference."""
+    """The graph of one case with its tensors in the backend's memory, as an engine keeps them."""
 
     backend = None  # one for the process, as an engine has
 
@@ -171,8 +186,8 @@ class _Graph:
         if _Graph.backend is None:
             _Graph.backend = L.Backend(0)
         H, c = self.H, s["case"]
-        self.kept, self.bufs = [H.ggml_init(L.InitParams(0, None, True)) for _ in range(2)], []  # weights; everything else
-        weights, work = self.kept
+        self.kept = _Kept(L)
+        weights, work = self.kept.ctxs  # weights; everything else
         data = []
 
         def put(ctx, kind, ne, t):
@@ -205,22 +220,16 @@ class _Graph:
             buf = H.ggml_backend_alloc_ctx_tensors_from_buft(ctx, _Graph.backend.buft)
             if buf:  # (none for a context without tensors)
                 H.ggml_backend_buffer_set_usage(buf, usage)
-                self.bufs.append(buf)
+                self.kept.bufs.append(buf)
         for r, t in data:
             a = t.contiguous().cpu().numpy()
             H.ggml_backend_tensor_set(r, a.ctypes.data_as(C.c_void_p), 0, a.nbytes)
-        self.out = torch.as_tensor(_Memory(out.contents.data, shape), device="cuda")
+        self.out = torch.as_tensor(_Memory(self.kept, out.contents.data, shape), device="cuda")
 
     def __call__(self):
         if self.H.ggml_backend_graph_compute_async(_Graph.backend.backend, self.graph) != 0:
             raise RuntimeError("graph_compute failed")
         return self.out
-
-    def __del__(self):
-        for b in self.bufs:
-            self.H.ggml_backend_buffer_free(b)
-        for k in self.kept:
-            self.H.ggml_free(k)
 
 
 def prepare(case, seed):
