@@ -57,6 +57,7 @@ ggml_backend_reg_t ggml_backend_mi355x_reg(void);
  *   "ggml_backend_mi355x_graph_key_probe" ggml_backend_mi355x_graph_key_probe_t   (tests: is graph b the graph a captured hipGraph of a stands for?)
  *   "ggml_backend_mi355x_scratch_probe"   ggml_backend_mi355x_scratch_probe_t   (tests: the scratch that a graph's partial products and records may take)
  *   "ggml_backend_mi355x_k_slices"        ggml_backend_mi355x_k_slices_t        (tests: K slices of a K-quant product)
+ *   "ggml_backend_mi355x_supports_probe"  ggml_backend_mi355x_supports_probe_t  (tests: what a device's supports_op answers)
  *   "ggml_backend_mi355x_prepare_columns" ggml_backend_mi355x_prepare_columns_t
  *   "ggml_backend_mi355x_result_to"       ggml_backend_mi355x_result_to_t
  *   "ggml_backend_mi355x_decode_copy_read" ggml_backend_mi355x_decode_copy_read_t (tests: the plane-layout decode copy of a weight matrix, csrc/repack.hip)
@@ -98,6 +99,9 @@ typedef int (*ggml_backend_mi355x_graph_key_probe_t)(const struct ggml_cgraph * 
  * n_cols columns.  Host arithmetic: both work without a device. */
 typedef int64_t (*ggml_backend_mi355x_scratch_probe_t)(const struct ggml_cgraph * g);
 typedef int (*ggml_backend_mi355x_k_slices_t)(int type, int64_t K, int64_t n_rows, int64_t n_cols);
+
+/* 1 where a device of this registration would take operator `op`, else 0.  Host arithmetic: works without a device. */
+typedef int (*ggml_backend_mi355x_supports_probe_t)(const struct ggml_tensor * op);
 
 /* Makes the panel copies (csrc/mmq_panel.hip) that batches of from .. to (2 .. 32) columns would read of n weight matrices over the same activations (gate and up, say), in the backend's
  * stream.  A host that has loaded its weights may call it once per group of matrices, so that the first such batch does not have to make them; copies that exist are kept.  Returns the

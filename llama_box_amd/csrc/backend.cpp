@@ -1011,6 +1011,7 @@ static int api_graph_key_probe(const ggml_cgraph * a, const ggml_cgraph * b, int
 }
 // ... and what decides whether K slices fit the scratch: the bytes set aside for a graph, the slices that a product of n_rows rows (of all matrices of its launch) and M columns takes
 static int64_t api_scratch_probe(const ggml_cgraph * g) { return partials_reserved(g); }
+static int api_supports_probe(const ggml_tensor * op) { return supports_op(op) ? 1 : 0; }
 static int api_k_slices(int type, int64_t K, int64_t n_rows, int64_t M) { return mmq_pick_ksplit(K, n_rows, M, options().mmq_skinny, type); }
 static int api_prepare_columns(ggml_backend_t be, const ggml_tensor * const * w, int n, int64_t from, int64_t to) {
     if (!be_is_ours(be) || w == nullptr || n < 1 || std::find(w, w + n, nullptr) != w + n) return -1;
@@ -1183,6 +1184,7 @@ static void * reg_get_proc_address(ggml_backend_reg_t, const char * name) {
     if (n == "ggml_backend_mi355x_split_rows") return (void *) api_split_rows;
     if (n == "ggml_backend_mi355x_graph_key_probe") return (void *) api_graph_key_probe;
     if (n == "ggml_backend_mi355x_scratch_probe") return (void *) api_scratch_probe;
+    if (n == "ggml_backend_mi355x_supports_probe") return (void *) api_supports_probe;
     if (n == "ggml_backend_mi355x_k_slices") return (void *) api_k_slices;
     return nullptr;
 }

@@ -249,6 +249,7 @@ bool supports_op(const ggml_tensor * op) {
             if (buffer_is_split(a->buffer)) return split_mul_mat_supported(op);  // -sm row weights: every device computes its rows (split.cpp)
             if (mm_cache_image_ok(op)) return true;
             if (a->type == GGML_TYPE_BF16) return a->nb[0] == 2 && b->nb[0] == 4;  // a model's bf16 matrices: src1 rounded to bf16, f32 accumulation (mmf.hip)
+            if (a->type == GGML_TYPE_MXFP4) return a->ne[2] == 1 && a->ne[3] == 1 && mx_product_ok(TD(a), TD(b));
             if (is_quant(a->type)) {
                 return a->ne[2] == 1 && a->ne[3] == 1 && rows_contig(a) && b->nb[0] == 4 && a->ne[0] % ggml_abi_blck_size(a->type) == 0;
             }
@@ -281,8 +282,16 @@ bool supports_op(const ggml_tensor * op) {
         case GGML_OP_MUL_MAT_ID: {
             const ggml_tensor * ids = op->src[2];
             if (!a || !b || !ids || b->type != GGML_TYPE_F32 || op->type != GGML_TYPE_F32 || ids->type != GGML_TYPE_I32 || !ggml_abi_is_contiguous(op)) return false;
-            if (a->type != GGML_TYPE_F32 && a->type != GGML_TYPE_F16 && a->type != GGML_TYPE_BF16) return false;
+            if (a->type == GGML_TYPE_MXFP4) {
+                if (!mx_product_ok(TD(a), TD(b)) || !mx_id_ok(TD(a), TD(ids))) return false;
+            } else if (a->type != GGML_TYPE_F32 && a->type != GGML_TYPE_F16 && a->type != GGML_TYPE_BF16) return false;
             return a->nb[0] == ggml_abi_type_size(a->type) && b->nb[0] == 4 && a->ne[3] == 1 && b->ne[3] == 1 && (b->ne[1] == 1 || b->ne[1] == ids->ne[0]) && ids->ne[1] == b->ne[2];
+        }
+        case GGML_OP_ADD_ID: {  // a [N, n_used, T] + the rows of b [N, n_expert] that ids [n_used, T] names
+            const ggml_tensor * ids = op->src[2];
+            if (!a || !b || !ids || a->type != GGML_TYPE_F32 || b->type != GGML_TYPE_F32 || ids->type != GGML_TYPE_I32 || op->type != GGML_TYPE_F32) return false;
+            return a->nb[0] == 4 && b->nb[0] == 4 && op->nb[0] == 4 && same_shape(a, op) && a->ne[3] == 1 && a->ne[0] == b->ne[0] && b->ne[2] == 1 && b->ne[3] == 1 && a->ne[1] == ids->ne[0] &&
+                   a->ne[2] == ids->ne[1] && ids->ne[2] == 1 && ids->ne[3] == 1 && a->ne[1] <= 65535 && a->ne[2] <= 65535;
         }
         case GGML_OP_CUSTOM:
             return stream_op_ok(op);
@@ -294,6 +303,8 @@ bool supports_op(const ggml_tensor * op) {
         case GGML_OP_CPY: case GGML_OP_DUP: case GGML_OP_CONT: {
             const int st = a->type, dt = op->type;
             if (st == GGML_TYPE_I32 && dt == GGML_TYPE_I32) return true;
+            if ((st == GGML_TYPE_MXFP4 && dt == GGML_TYPE_F32) || (st == GGML_TYPE_F32 && dt == GGML_TYPE_MXFP4))
+                return ggml_abi_is_contiguous(a) && ggml_abi_is_contiguous(op) && (a->ne[0] % 32) == 0 && same_shape(a, op);
             if ((st == GGML_TYPE_Q8_0 && dt == GGML_TYPE_F32) || (st == GGML_TYPE_F32 && dt == GGML_TYPE_Q8_0))  // K-shift of a quantised cache
                 return ggml_abi_is_contiguous(a) && ggml_abi_is_contiguous(op) && (a->ne[0] % 32) == 0;
             if ((kv_store_type(st) && dt == GGML_TYPE_F32) || (st == GGML_TYPE_F32 && kv_store_type(dt)))  // ... of a cache in one of the other types (kv_types.hip)
@@ -302,13 +313,14 @@ bool supports_op(const ggml_tensor * op) {
         }
         case GGML_OP_GET_ROWS:
             return b->type == GGML_TYPE_I32 && op->type == GGML_TYPE_F32 && rows_contig(a) && op->nb[0] == 4 &&
-                   (is_quant(a->type) || a->type == GGML_TYPE_F16 || a->type == GGML_TYPE_F32 || a->type == GGML_TYPE_BF16);
+                   (a->type == GGML_TYPE_MXFP4 || is_quant(a->type) || a->type == GGML_TYPE_F16 || a->type == GGML_TYPE_F32 || a->type == GGML_TYPE_BF16);
         case GGML_OP_SET_ROWS:
             if (op->type == GGML_TYPE_BF16 && !bf16_rows_in_blocks(a))  // bf16 rows that are not whole, aligned groups of 32 values: the element-wise form (ops.hip)
                 return a->type == GGML_TYPE_F32 && b->type == GGML_TYPE_I64 && a->nb[0] == 4 && op->nb[0] == 2;
             if (kv_store_type(op->type))  // a cache row in q4_0 / q4_1 / q5_0 / q5_1 / iq4_nl / bf16: the type's from_float per block of 32 (kv_types.hip)
                 return a->type == GGML_TYPE_F32 && b->type == GGML_TYPE_I64 && a->nb[0] == 4 && (a->ne[0] % 32) == 0 && (a->nb[1] % 16) == 0 && (a->nb[2] % 16) == 0 && (a->nb[3] % 16) == 0 &&
                        op->nb[0] == ggml_abi_type_size(op->type);
+            if (op->type == GGML_TYPE_MXFP4) return a->type == GGML_TYPE_F32 && b->type == GGML_TYPE_I64 && a->nb[0] == 4 && (a->ne[0] % 32) == 0 && op->nb[0] == ggml_abi_type_size(op->type);
             if (op->type == GGML_TYPE_Q8_0) return a->type == GGML_TYPE_F32 && b->type == GGML_TYPE_I64 && a->nb[0] == 4 && (a->ne[0] % 32) == 0 && (a->nb[1] % 16) == 0 && (a->nb[2] % 16) == 0 && (a->nb[3] % 16) == 0;
             return a->type == GGML_TYPE_F32 && b->type == GGML_TYPE_I64 && a->nb[0] == 4 && (op->type == GGML_TYPE_F16 || op->type == GGML_TYPE_F32) &&
                    op->nb[0] == ggml_abi_type_size(op->type);
@@ -404,7 +416,10 @@ static ws_plan plan_ws(backend_ctx * c, const ggml_cgraph * g) {
         const ggml_tensor * n = g->nodes[i];
         // (besides what follows: K.q of one head on one key head has this form, and the attention chain that may start at it has its own scratch)
         if (n->op == GGML_OP_MUL_MAT && mm_tile_form(n)) p.act16_bytes = std::max(p.act16_bytes, (size_t) (n->src[1]->ne[0] * n->src[1]->ne[1]) * 2);
-        if (n->op == GGML_OP_MUL_MAT && is_quant(n->src[0]->type)) {
+        if (n->src[0] && n->src[0]->type == GGML_TYPE_MXFP4 && (n->op == GGML_OP_MUL_MAT || (n->op == GGML_OP_MUL_MAT_ID && n->src[2]))) {
+            const ggml_tensor * w = n->src[0], * b = n->src[1], * ids = n->src[2];
+            p.act_bytes = std::max(p.act_bytes, n->op == GGML_OP_MUL_MAT ? mx_act_bytes(w->ne[0], b->ne[1] * b->ne[2] * b->ne[3]) : mx_id_act_bytes(w->ne[0], w->ne[2], ids->ne[0] * ids->ne[1]));
+        } else if (n->op == GGML_OP_MUL_MAT && is_quant(n->src[0]->type)) {
             const ggml_tensor * b = n->src[1];
             const int64_t Mc = b->ne[1] * b->ne[2] * b->ne[3];
             // (2..32 columns: the skinny matrix-core kernel fetches 32 columns' worth of activation bytes whatever M is)
@@ -568,6 +583,10 @@ struct exec_state {
     // the MUL_MAT_ID that last left per-expert column lists in the scratch area: node index and the ids tensor they were made from
     int moe_node = -1;
     const ggml_tensor * moe_ids = nullptr;
+    // the MUL_MAT_ID by MXFP4 experts that last left its lists and its columns in the activation scratch (MI_ACT_MX_ID): node index, ids and experts they were made for, where the lists are
+    int mx_node = -1;
+    const ggml_tensor * mx_ids = nullptr;
+    int64_t mx_experts = 0;
 };
 
 // Number of readers of t.  A backend is handed ONE split of the host's graph (ggml_backend_sched: ggml_graph_view of the full
@@ -2904,6 +2923,65 @@ static int attn_gate_behind(exec_state & st, int i, attn_f32_extra & x) {
     return k - i;
 }
 
+// MUL_MAT by an MXFP4 matrix: src1 as 6-bit digits (kept for the next product that reads it), then the product
+static int run_mul_mat_mx(exec_state & st, int i) {
+    backend_ctx * c = st.c;
+    ggml_tensor * n = st.g->nodes[i];
+    const ggml_tensor * a = n->src[0], * b = n->src[1];
+    void * act = (char *) c->ws + st.act_off;
+    if (!c->act.holds(b, MI_ACT_MX)) {
+        timed_scope ts(c, "quantize_act", (double) ggml_abi_nbytes(b));
+        launch_mx_act(c->stream, TD(b), act);
+        c->st.kernel_launches++;
+        c->act.set(b, MI_ACT_MX);
+    }
+    {
+        timed_scope ts(c, "mul_mat_mxfp4", (double) ggml_abi_nbytes(a));
+        launch_mx_mul_mat(c->stream, TD(a), TD(b), TD(n), act);
+        c->st.kernel_launches++;
+    }
+    if (tp_active(c) && buffer_is_rowpar(a->view_src ? a->view_src->buffer : a->buffer)) {
+        timed_scope ts(c, "tp_all_reduce", (double) ggml_abi_nbytes(n));
+        if (!tp_all_reduce(c, (float *) n->data, (size_t) ggml_abi_nelements(n))) return -1;
+        c->st.allreduces++;
+    }
+    return 1;
+}
+// MUL_MAT_ID by MXFP4 experts [-> ADD_ID: the experts' bias rows, added where the sums are stored].  The lists serve the products behind it that read the same ids (up beside gate, then down), the
+// columns those that read the same src1 too
+static int run_mul_mat_id_mx(exec_state & st, int i) {
+    backend_ctx * c = st.c;
+    ggml_cgraph * g = st.g;
+    ggml_tensor * n = g->nodes[i];
+    const ggml_tensor * a = n->src[0], * b = n->src[1], * ids = n->src[2];
+    void * ws = (char *) c->ws + st.act_off;
+    bool lists = st.mx_node >= 0 && st.mx_ids == ids && st.mx_experts == a->ne[2] && c->act.kind == MI_ACT_MX_ID;
+    for (int k = st.mx_node + 1; lists && k < i; ++k) lists = is_view_op(g->nodes[k]) || !ranges_overlap(g->nodes[k], ids);
+    const bool cols = lists && c->act.holds(b, MI_ACT_MX_ID);
+    if (!lists) {
+        timed_scope ts(c, "moe_group", (double) ggml_abi_nbytes(ids));
+        launch_mx_group(c->stream, TD(ids), a->ne[2], ws);
+        c->st.kernel_launches++;
+    }
+    if (!cols) {
+        timed_scope ts(c, "quantize_act", (double) ggml_abi_nbytes(b));
+        launch_mx_id_act(c->stream, TD(b), TD(ids), a->ne[2], ws);
+        c->st.kernel_launches++;
+        c->act.set(b, MI_ACT_MX_ID);
+    }
+    st.mx_node = i;
+    st.mx_ids = ids;
+    st.mx_experts = a->ne[2];
+    // (the bias: the result alone reads the product, of the same ids, and is not stored over what the launch still reads)
+    ggml_tensor * ad = i + 1 < g->n_nodes && !st.done[i + 1] ? g->nodes[i + 1] : nullptr;
+    const bool bias = c->opt.fusion && ad && ad->op == GGML_OP_ADD_ID && ad->src[0] == n && ad->src[2] == ids && single_use(st, n) && is_f32_contig(ad) && supports_op(ad) && !ranges_overlap(ad, ad->src[1]) && !ranges_overlap(ad, ids);
+    timed_scope ts(c, "mul_mat_id_mxfp4", (double) ggml_abi_nbytes(a) / (double) std::max<int64_t>(1, a->ne[2]) * (double) std::min<int64_t>(a->ne[2], ggml_abi_nelements(ids)));
+    launch_mx_mul_mat_id(c->stream, TD(a), TD(ids), TD(bias ? ad : n), ws, bias ? (const float *) ad->src[1]->data : nullptr, bias ? (int64_t) ad->src[1]->nb[1] : 0);
+    c->st.kernel_launches++;
+    c->st.fused_nodes += bias;
+    return bias ? 2 : 1;
+}
+
 static int run_node(exec_state & st, int i) {
     backend_ctx * c = st.c;
     ggml_cgraph * g = st.g;
@@ -3006,6 +3084,7 @@ static int run_node(exec_state & st, int i) {
                 c->st.kv_image_nodes++;
                 return 1;
             }
+            if (a->type == GGML_TYPE_MXFP4) return run_mul_mat_mx(st, i);
             if (!is_quant(a->type) && fuse && c->opt.attn_nf && try_fuse_attn_nf(st, i)) return 1;
             if (!is_quant(a->type) && fuse && c->opt.attn_nf && try_fuse_attn_nf_mma(st, i)) return 1;
             if ((a->type == GGML_TYPE_BF16 || a->type == GGML_TYPE_F16) && fuse && try_merge_mm_16(st, i)) return 1;
@@ -3442,6 +3521,7 @@ static int run_node(exec_state & st, int i) {
         }
         case GGML_OP_MUL_MAT_ID: {
             const ggml_tensor * ids = n->src[2];
+            if (a->type == GGML_TYPE_MXFP4) return run_mul_mat_id_mx(st, i);
             // the down projection of a mixture-of-experts block reads the same ids as its up projection: the per-expert column lists are made once
             // (valid only while nothing but element-wise nodes ran in between: they do not touch the scratch area)
             bool valid = st.moe_ids == ids && st.moe_node >= 0 && i - st.moe_node <= 6 && g->nodes[st.moe_node]->src[0]->ne[2] == a->ne[2];
@@ -3458,6 +3538,12 @@ static int run_node(exec_state & st, int i) {
             c->st.kernel_launches++;
             c->st.fused_nodes += behind;
             return 1 + behind;
+        }
+        case GGML_OP_ADD_ID: {
+            timed_scope ts(c, "add_id", (double) ggml_abi_nbytes(n) * 2);
+            launch_add_id(s, TD(a), TD(b), TD(n->src[2]), TD(n));
+            c->st.kernel_launches++;
+            return 1;
         }
         case GGML_OP_GLU: {
             const tdesc bd = b ? TD(b) : TD(a);
@@ -3497,6 +3583,10 @@ static int run_node(exec_state & st, int i) {
         case GGML_OP_CPY: case GGML_OP_DUP: case GGML_OP_CONT: {
             if (a->type == n->type && ggml_abi_is_contiguous(a) && ggml_abi_is_contiguous(n)) {
                 if (hipMemcpyAsync(n->data, a->data, ggml_abi_nbytes(a), hipMemcpyDeviceToDevice, s) != hipSuccess) return -1;
+            } else if (a->type == GGML_TYPE_MXFP4 || n->type == GGML_TYPE_MXFP4) {
+                timed_scope ts(c, "cpy_mxfp4", (double) ggml_abi_nbytes(n) + (double) ggml_abi_nbytes(a));
+                if (n->type == GGML_TYPE_MXFP4) launch_mx_store(s, TD(a), nullptr, TD(n));
+                else launch_mx_read(s, TD(a), nullptr, TD(n));
             } else if (a->type == GGML_TYPE_Q8_0 || n->type == GGML_TYPE_Q8_0) {
                 timed_scope ts(c, "cpy_q8_0", (double) ggml_abi_nbytes(n) + (double) ggml_abi_nbytes(a));
                 launch_cpy_q8_0(s, a->data, n->data, ggml_abi_nelements(a), n->type == GGML_TYPE_Q8_0);
@@ -3530,6 +3620,13 @@ static int run_node(exec_state & st, int i) {
             // first fused Q/K/V launch (same positions, parameters, token count: it then finds it valid), and is simply rebuilt there if the guess was wrong
             static const bool head_on = !getenv("GGML_MI355X_STEP_HEAD") || atoi(getenv("GGML_MI355X_STEP_HEAD")) != 0;
             const int64_t n_rows = b->ne[0] * b->ne[1] * b->ne[2];
+            if (a->type == GGML_TYPE_MXFP4) {
+                timed_scope ts(c, "get_rows", (double) ggml_abi_nbytes(n));
+                const tdesc rows = TD(b);
+                launch_mx_read(s, TD(a), &rows, TD(n));
+                c->st.kernel_launches++;
+                return 1;
+            }
             if (head_on && fuse && !c->opt.timing && n_rows <= 64) {
                 const ggml_tensor * cast = nullptr;
                 int cast_at = -1;
@@ -3594,7 +3691,9 @@ static int run_node(exec_state & st, int i) {
         }
         case GGML_OP_SET_ROWS: {
             timed_scope ts(c, "set_rows", (double) ggml_abi_nbytes(a));
-            if (n->type == GGML_TYPE_Q8_0) launch_set_rows_q8_0(s, TD(a), TD(b), TD(n));
+            const tdesc places = TD(b);
+            if (n->type == GGML_TYPE_MXFP4) launch_mx_store(s, TD(a), &places, TD(n));
+            else if (n->type == GGML_TYPE_Q8_0) launch_set_rows_q8_0(s, TD(a), TD(b), TD(n));
             else if (kv_store_type(n->type) && !(n->type == GGML_TYPE_BF16 && !bf16_rows_in_blocks(a))) {
                 // K and V rows of a step go into their caches through the same indices: SET_ROWS(k), [views], SET_ROWS(v) as ONE launch
                 int j = i + 1;

@@ -29,6 +29,8 @@ size_t quantized_act_bytes(int kind, int64_t K, int64_t rows);
 void launch_quantize_act(hipStream_t s, int kind, const tdesc & src, void * dst);
 // Q8_0 activations in PANEL order, columns in groups of 32 (mmq_q80.hip): per block of 32 values [K half][column 0 .. 31][16 quants] + [column] f32 scales, 1152 B
 #define MI_ACT_Q80_PANEL 1008
+#define MI_ACT_MX 1009     // the 6-bit digits that a product by an MXFP4 matrix takes (mx.hip) ...
+#define MI_ACT_MX_ID 1010  // ... of MUL_MAT_ID's columns, sorted by expert, behind their lists
 #define MI_ACT_16 2000  // + the 16-bit type: f32 rows rounded to it (mmf_tile.hip)
 void launch_quantize_q80_panel(hipStream_t s, const tdesc & src, void * dst);
 // producers fused with that quantisation (ops.hip; same arithmetic as the unfused kernels): RMS_NORM(x) * w, SwiGLU
@@ -532,6 +534,25 @@ void launch_head_norm_gate(hipStream_t s, const tdesc & o, const float * w, int 
 void launch_add_rms_norm_mul(hipStream_t s, const float * x, const float * y, float * sum, float * d, const float * w, int64_t n, int64_t rows, float eps);
 void launch_argsort_grouped(hipStream_t s, const tdesc & src, const tdesc & dst, int groups, int keep);  // descending; entries outside the `keep` groups with the largest maxima sort last
 
+// ---- microscaled 4-bit (mx.hip)
+// f32 rows -> MXFP4 and back; idx: the places of SET_ROWS (I64) / the rows of GET_ROWS (I32), null: row by row (CPY)
+void launch_mx_store(hipStream_t s, const tdesc & a, const tdesc * idx, const tdesc & d);
+void launch_mx_read(hipStream_t s, const tdesc & a, const tdesc * idx, const tdesc & d);
+// MUL_MAT: w [K, N], b f32 rows of K, d dense.  act: mx_act_bytes(K, columns) that launch_mx_act has filled from b
+bool mx_product_ok(const tdesc & w, const tdesc & b);
+size_t mx_act_bytes(int64_t K, int64_t cols);
+void launch_mx_act(hipStream_t s, const tdesc & b, void * act);
+void launch_mx_mul_mat(hipStream_t s, const tdesc & w, const tdesc & b, const tdesc & d, const void * act);
+// MUL_MAT_ID: w [K, N, n_expert], b [K, 1 or n_used, T], ids [n_used, T], d dense; bias: rows [N] of the experts, added where they are stored, or null.
+// ws: mx_id_act_bytes(K, n_expert, n_used T), first the lists (launch_mx_group), then the columns (launch_mx_id_act)
+bool mx_id_ok(const tdesc & w, const tdesc & ids);
+size_t mx_id_act_bytes(int64_t K, int64_t n_expert, int64_t cols);
+void launch_mx_group(hipStream_t s, const tdesc & ids, int64_t n_expert, void * ws);
+void launch_mx_id_act(hipStream_t s, const tdesc & b, const tdesc & ids, int64_t n_expert, void * ws);
+void launch_mx_mul_mat_id(hipStream_t s, const tdesc & w, const tdesc & ids, const tdesc & d, const void * ws, const float * bias, int64_t nb_bias);
+// ADD_ID: a [N, n_used, T] + the rows of b [N, n_expert] that ids names
+void launch_add_id(hipStream_t s, const tdesc & a, const tdesc & b, const tdesc & ids, const tdesc & d);
+
 // ---- code-object preload (round 4).  The HIP runtime loads a translation unit's device code on the FIRST launch of one of its kernels
 // (0.3 - 2 ms each, measured as idle gaps in front of the first prompt's kernels: 5.5 ms of a 64 ms prefill).  Every kernel file ends with
 // MI_TU_TOUCH(name): an empty kernel + a launcher; init_backend launches them all once per device, so the cost moves to start-up.
@@ -558,6 +579,7 @@ void tu_touch_kv_types(hipStream_t s);
 void tu_touch_repack(hipStream_t s);
 void tu_touch_seq(hipStream_t s);
 void tu_touch_streams(hipStream_t s);
+void tu_touch_mx(hipStream_t s);
 inline void preload_kernel_files(hipStream_t s) {
     tu_touch_kv_types(s);
     tu_touch_repack(s);
@@ -579,6 +601,7 @@ inline void preload_kernel_files(hipStream_t s) {
     tu_touch_tp_p2p(s);
     tu_touch_seq(s);
     tu_touch_streams(s);
+    tu_touch_mx(s);
 }
 
 }  // namespace mi355x

@@ -1,0 +1,382 @@
+// mx.hip — microscaled 4-bit (MXFP4): rows to and from f32, MUL_MAT, MUL_MAT_ID, and the experts' bias rows (ADD_ID).
+//
+// A block is 32 values: a byte e and 16 bytes of codes, value j in the low nibble of byte j, value 16 + j in the high nibble.  A value is E2M1(code) 2^(e - 127), E2M1 = 0, 1/2, 1, 3/2, 2, 3, 4,
+// 6 with the sign in bit 3; e = 255 makes the whole block NaN.
+//
+// Products.  The matrix cores take two operands of 4 .. 8 bits per value and a power of two per 32 of them, and multiply by both powers themselves (v_mfma_scale_f32_*_f8f6f4): a weight block goes
+// in as it lies in memory.  The activations are quantised to the same form, a block of 32 as whole numbers q of -255 .. 255 times 2^s (the counterpart of the Q8_0 / Q8_K activations of the other
+// block formats; half a step is at most 2^-8 of the block's largest value, Q8_0's 1 / 254).  |q| = 16 h + l, and each of h, l <= 15 is one E2M3 value (6 bits: the codes 0 .. 15 stand for code / 8):
+// two instructions a tile, at twice the rate of 8-bit operands, and their products are exact.  Only the f32 sums round.
+#include "common.h"
+#include "dev_util.h"
+#include "kernels.h"
+
+namespace mi355x {
+
+typedef int mx_i4 __attribute__((ext_vector_type(4)));
+typedef int mx_i2 __attribute__((ext_vector_type(2)));
+typedef int mx_i8 __attribute__((ext_vector_type(8)));
+typedef float mx_f16 __attribute__((ext_vector_type(16)));
+typedef mx_i4 __attribute__((aligned(1))) mx_i4_a1;  // (a block's codes start anywhere)
+typedef uint16_t __attribute__((aligned(1))) mx_u16_a1;
+typedef float mx_f2 __attribute__((ext_vector_type(2)));
+typedef mx_f2 __attribute__((aligned(4))) mx_f2_a4;
+
+static constexpr int MX_BLOCK = 17;  // bytes
+static constexpr int MX_FP4 = 4, MX_FP6 = 2;  // operand formats of the matrix instructions: E2M1, E2M3
+
+// ------------------------------------------------------------------------------------------------ rows
+// Eight lanes share a block: lane i of them has the values 2i, 2i + 1, 16 + 2i, 16 + 2i + 1, whose codes are the bytes 2i and 2i + 1.
+__device__ __forceinline__ void mx_load4(const float * blk, const int i, float (&v)[4]) {
+    const mx_f2 a = *(const mx_f2_a4 *) (blk + 2 * i), b = *(const mx_f2_a4 *) (blk + 16 + 2 * i);
+    v[0] = a.x;
+    v[1] = a.y;
+    v[2] = b.x;
+    v[3] = b.y;
+}
+// the bits of the block's largest magnitude (an infinity's or NaN's bits are larger than any number's)
+__device__ __forceinline__ uint32_t mx_top(const float (&v)[4]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m = max(m, __float_as_uint(v[k]) & 0x7FFFFFFFu);
+    m = max(m, (uint32_t) dpp_i32<MI_DPP_QUAD_XOR1>((int) m));
+    m = max(m, (uint32_t) dpp_i32<MI_DPP_QUAD_XOR2>((int) m));
+    return max(m, (uint32_t) dpp_i32<MI_DPP_HALF_MIRROR>((int) m));
+}
+// the nearest code, a tie to the lower one (of two magnitudes the smaller, of two zeros +0); m2: 2^(127 - e) in two factors that f32 holds
+__device__ __forceinline__ uint32_t mx_code(const float v, const float f0, const float f1) {
+    const float m = fabsf(v) * f0 * f1;
+    const uint32_t c = (uint32_t) (m > 0.25f) + (uint32_t) (m > 0.75f) + (uint32_t) (m > 1.25f) + (uint32_t) (m > 1.75f) + (uint32_t) (m > 2.5f) + (uint32_t) (m > 3.5f) + (uint32_t) (m > 5.0f);
+    return c ? c | ((__float_as_uint(v) >> 31) << 3) : 0u;
+}
+// -> the block's scale byte; the lane's two bytes of codes
+__device__ __forceinline__ int mx_quantise4(const float (&v)[4], uint32_t & codes) {
+    const uint32_t top = mx_top(v);
+    codes = 0;
+    if (top >= 0x7F800000u) return 255;
+    int lg = (int) (top >> 23) - 127;                          // floor(log2) of a normal number
+    if (lg == -127) lg = -118 - __clz((int) (top | 1u));       // ... of a subnormal one: bits 2^-149; below every scale's range anyway
+    const int e = top ? max(lg + 125, 0) : 0;
+    const int half = (127 - e) / 2, rest = 127 - e - half;     // (127 - e: -127 .. 127)
+    const float f0 = __uint_as_float((uint32_t) (127 + half) << 23), f1 = __uint_as_float((uint32_t) (127 + rest) << 23);
+    codes = mx_code(v[0], f0, f1) | mx_code(v[2], f0, f1) << 4 | mx_code(v[1], f0, f1) << 8 | mx_code(v[3], f0, f1) << 12;
+    return e;
+}
+// 2^(e - 127) as f32 (e = 0: subnormal), NaN for 255
+__device__ __forceinline__ float mx_scale(const int e) { return e == 255 ? __uint_as_float(0x7FC00000u) : e == 0 ? __uint_as_float(0x00400000u) : __uint_as_float((uint32_t) e << 23); }
+__device__ __forceinline__ float mx_value(const uint32_t code, const float scale) {
+    // magnitudes 0 .. 7 doubled: 0 1 2 3 4 6 8 12, a nibble each
+    const float m = 0.5f * (float) ((0xC8643210u >> (4 * (code & 7))) & 15u);
+    return ((code & 8) ? -m : m) * scale;
+}
+struct mx_row_at { int64_t i1, i2, i3, blk; };
+__device__ __forceinline__ mx_row_at mx_row(const int64_t block, const int64_t per_row, const int64_t n1, const int64_t n2) {
+    mx_row_at r;
+    const int64_t row = block / per_row;
+    r.blk = block - row * per_row;
+    r.i1 = row % n1;
+    r.i2 = (row / n1) % n2;
+    r.i3 = row / (n1 * n2);
+    return r;
+}
+// f32 rows -> blocks.  idx: SET_ROWS, the rows' places (one outside the destination is skipped); without: row i to row i
+template <bool IDX> __global__ void __launch_bounds__(256) k_mx_store(const tdesc a, const tdesc idx, const tdesc d) {
+    const int64_t per_row = a.ne[0] / 32, block = ((int64_t) blockIdx.x * 256 + threadIdx.x) >> 3;
+    const int i = threadIdx.x & 7;
+    if (block >= per_row * a.ne[1] * a.ne[2] * a.ne[3]) return;  // (eight lanes leave together)
+    const mx_row_at r = mx_row(block, per_row, a.ne[1], a.ne[2]);
+    int64_t to = r.i1;
+    if (IDX) {
+        to = *(const int64_t *) (idx.data + r.i1 * idx.nb[0] + (r.i2 % idx.ne[1]) * idx.nb[1] + (r.i3 % idx.ne[2]) * idx.nb[2]);
+        if (to < 0 || to >= d.ne[1]) return;
+    }
+    float v[4];
+    mx_load4((const float *) (a.data + r.i1 * a.nb[1] + r.i2 * a.nb[2] + r.i3 * a.nb[3]) + r.blk * 32, i, v);
+    uint32_t codes;
+    const int e = mx_quantise4(v, codes);
+    uint8_t * out = (uint8_t *) d.data + to * d.nb[1] + r.i2 * d.nb[2] + r.i3 * d.nb[3] + r.blk * MX_BLOCK;
+    if (i == 0) out[0] = (uint8_t) e;
+    *(mx_u16_a1 *) (out + 1 + 2 * i) = (uint16_t) codes;
+}
+// blocks -> f32 rows.  idx: GET_ROWS, the rows taken (one outside the source is skipped)
+template <bool IDX> __global__ void __launch_bounds__(256) k_mx_read(const tdesc a, const tdesc idx, const tdesc d) {
+    const int64_t per_row = a.ne[0] / 32, block = ((int64_t) blockIdx.x * 256 + threadIdx.x) >> 3;
+    const int i = threadIdx.x & 7;
+    if (block >= per_row * d.ne[1] * d.ne[2] * d.ne[3]) return;
+    const mx_row_at r = mx_row(block, per_row, d.ne[1], d.ne[2]);
+    int64_t from = r.i1;
+    if (IDX) {
+        from = *(const int32_t *) (idx.data + r.i1 * idx.nb[0] + r.i2 * idx.nb[1] + r.i3 * idx.nb[2]);
+        if (from < 0 || from >= a.ne[1]) return;
+    }
+    const uint8_t * in = (const uint8_t *) a.data + from * a.nb[1] + r.i2 * a.nb[2] + r.i3 * a.nb[3] + r.blk * MX_BLOCK;
+    const float s = mx_scale(in[0]);
+    const uint32_t c = *(const mx_u16_a1 *) (in + 1 + 2 * i);
+    float * out = (float *) (d.data + r.i1 * d.nb[1] + r.i2 * d.nb[2] + r.i3 * d.nb[3]) + r.blk * 32 + 2 * i;
+    *(mx_f2_a4 *) out = mx_f2{mx_value(c & 15, s), mx_value((c >> 8) & 15, s)};
+    *(mx_f2_a4 *) (out + 16) = mx_f2{mx_value((c >> 4) & 15, s), mx_value(c >> 12, s)};
+}
+void launch_mx_store(hipStream_t s, const tdesc & a, const tdesc * idx, const tdesc & d) {
+    const int64_t n = (a.ne[0] / 32) * a.ne[1] * a.ne[2] * a.ne[3];
+    if (n <= 0) return;
+    const dim3 grid((unsigned) ((n + 31) / 32));
+    if (idx) hipLaunchKernelGGL(k_mx_store<true>, grid, dim3(256), 0, s, a, *idx, d);
+    else hipLaunchKernelGGL(k_mx_store<false>, grid, dim3(256), 0, s, a, a, d);
+}
+void launch_mx_read(hipStream_t s, const tdesc & a, const tdesc * idx, const tdesc & d) {
+    const int64_t n = (a.ne[0] / 32) * d.ne[1] * d.ne[2] * d.ne[3];
+    if (n <= 0) return;
+    const dim3 grid((unsigned) ((n + 31) / 32));
+    if (idx) hipLaunchKernelGGL(k_mx_read<true>, grid, dim3(256), 0, s, a, *idx, d);
+    else hipLaunchKernelGGL(k_mx_read<false>, grid, dim3(256), 0, s, a, a, d);
+}
+
+// ------------------------------------------------------------------------------------------------ activations
+// The quantised columns lie in groups of 32, a group in steps of 128 values (four blocks), as the lanes of a product fetch them: for each block the 16 first bytes of h of the 32 columns, those of l, the
+// 8 last bytes of h, those of l (24 bytes are 32 codes of 6 bits), and behind the four blocks 4 scale bytes a column.  A block's codes stand in the order of the weights' nibbles: value j at place 2j,
+// value 16 + j at place 2j + 1.  The scale byte is h's exponent, s + 7 + 127; l's is 4 less.  Blocks behind the last one of a row are zeros.
+static constexpr int MX_ACT_BLK = 32 * 48, MX_ACT_STEP = 4 * MX_ACT_BLK + 32 * 4;
+static inline int64_t mx_steps(int64_t K) { return (K + 127) / 128; }
+size_t mx_act_bytes(int64_t K, int64_t cols) { return (size_t) ((cols + 31) / 32) * (size_t) (mx_steps(K) * MX_ACT_STEP); }
+
+// Columns of MUL_MAT_ID sorted by expert, every expert's first column in a group of its own: list[p] the column (u + n_used t) at place p or -1, owner[g] the expert of group g, total the groups in use
+struct mx_lists {
+    int32_t * total, * owner, * list;
+};
+// ids outside the experts are in no list: their columns are left as they are
+static int64_t mx_id_groups(int64_t n_expert, int64_t cols) { return cols / 32 + std::min(n_expert, cols); }  // (at most: an expert's last group may hold one column)
+static mx_lists mx_lists_at(void * ws, int64_t groups) {
+    mx_lists l;
+    l.total = (int32_t *) ws;
+    l.owner = l.total + 4;
+    l.list = l.owner + ((groups + 3) & ~(int64_t) 3);
+    return l;
+}
+static size_t mx_lists_bytes(int64_t groups) { return ((size_t) (4 + ((groups + 3) & ~(int64_t) 3) + groups * 32) * 4 + 255) & ~(size_t) 255; }
+size_t mx_id_act_bytes(int64_t K, int64_t n_expert, int64_t cols) {
+    const int64_t g = mx_id_groups(n_expert, cols);
+    return mx_lists_bytes(g) + mx_act_bytes(K, 32 * g);
+}
+static constexpr int MX_MAX_EXPERTS = 1024;
+// One workgroup an expert: every workgroup counts all experts' columns (whole numbers in LDS: no order to depend on), takes the groups in front of its own, and lists its columns in ascending order
+__global__ void __launch_bounds__(256) k_mx_group(const tdesc ids, const int n_expert, const mx_lists l) {
+    __shared__ int cnt[MX_MAX_EXPERTS], s_before[4], s_wave[4];
+    const int e = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n_used = (int) ids.ne[0], n = n_used * (int) ids.ne[1];
+    auto id_at = [&](const int i) { return *(const int32_t *) (ids.data + (int64_t) (i % n_used) * ids.nb[0] + (int64_t) (i / n_used) * ids.nb[1]); };
+    for (int i = threadIdx.x; i < n_expert; i += 256) cnt[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int v = id_at(i);
+        if (v >= 0 && v < n_expert) atomicAdd(&cnt[v], 1);
+    }
+    __syncthreads();
+    int before = 0;
+    for (int i = threadIdx.x; i < e; i += 256) before += (cnt[i] + 31) / 32;
+    for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o, 64);
+    if (lane == 0) s_before[wave] = before;
+    __syncthreads();
+    const int g0 = s_before[0] + s_before[1] + s_before[2] + s_before[3], mine = cnt[e], groups = (mine + 31) / 32;
+    for (int i = threadIdx.x; i < groups; i += 256) l.owner[g0 + i] = e;
+    for (int i = mine + (int) threadIdx.x; i < groups * 32; i += 256) l.list[g0 * 32 + i] = -1;
+    if (e == n_expert - 1 && threadIdx.x == 0) *l.total = g0 + groups;
+    int placed = 0;
+    for (int i0 = 0; i0 < n; i0 += 256) {
+        const int i = i0 + (int) threadIdx.x;
+        const bool hit = i < n && id_at(i) == e;
+        const uint64_t bal = __ballot(hit);
+        __syncthreads();
+        if (lane == 0) s_wave[wave] = __popcll(bal);
+        __syncthreads();
+        int off = placed + __popcll(bal & ((1ull << lane) - 1ull));
+        for (int w = 0; w < wave; ++w) off += s_wave[w];
+        if (hit) l.list[g0 * 32 + off] = i;
+        placed += s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3];
+    }
+}
+
+// the lane's four values as codes: 24 bits of h and of l in the order of places, and the block's scale byte
+__device__ __forceinline__ uint32_t mx_act4(const float (&v)[4], uint32_t & h, uint32_t & l) {
+    const uint32_t top = mx_top(v);
+    h = l = 0;
+    if (top >= 0x7F800000u) return 255u;
+    const int s = min(max((int) ((top + 0x8000u) >> 23) - 134, -120), 120);  // (exponent of the largest, rounded to 8 significant bits, - 7)
+    const float f = __uint_as_float((uint32_t) (127 - s) << 23);
+    constexpr int place[4] = {0, 2, 1, 3};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float q = rintf(v[k] * f);
+        const uint32_t m = min((uint32_t) fabsf(q), 255u), sign = (__float_as_uint(q) >> 26) & 32u;
+        h |= ((m >> 4) | sign) << (6 * place[k]);
+        l |= ((m & 15) | sign) << (6 * place[k]);
+    }
+    return (uint32_t) (s + 134);
+}
+// One workgroup a group of columns and a step of 128 values; eight lanes a block, eight columns at a time.  ID: column c of the list is row (c % n_used) % b.ne[1] of token c / n_used
+template <bool ID> __global__ void __launch_bounds__(256) k_mx_act(const tdesc b, const int64_t n_cols, const mx_lists l, const int n_used, uint8_t * __restrict__ act, const int steps) {
+    const int step = blockIdx.x, group = blockIdx.y;
+    if (ID && group >= *l.total) return;
+    const int i = threadIdx.x & 7, blk = (threadIdx.x >> 3) & 3, lane = threadIdx.x & 63;
+    const int64_t k0 = (int64_t) step * 128 + blk * 32;
+    uint8_t * out = act + ((int64_t) group * steps + step) * MX_ACT_STEP;
+    for (int c0 = 0; c0 < 32; c0 += 8) {
+        const int cg = c0 + (threadIdx.x >> 5);
+        int64_t c = (int64_t) group * 32 + cg;
+        const char * col;
+        if (ID) {
+            c = l.list[c];
+            col = b.data + ((c % n_used) % b.ne[1]) * b.nb[1] + (c / n_used) * b.nb[2];
+        } else {
+            if (c >= n_cols) c = -1;
+            col = b.data + (c % b.ne[1]) * b.nb[1] + ((c / b.ne[1]) % b.ne[2]) * b.nb[2] + (c / (b.ne[1] * b.ne[2])) * b.nb[3];
+        }
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (c >= 0 && k0 < b.ne[0]) mx_load4((const float *) col + k0, i, v);
+        uint32_t h, lo;
+        const uint32_t e = mx_act4(v, h, lo);
+        // dword i (0 .. 5) of the 24 bytes: its bits start in the 24 of lane i + i / 3, at 8 (i % 3)
+        const int src = (lane & ~7) + i + i / 3, sh = 8 * (i % 3);
+        const uint32_t h0 = (uint32_t) __shfl((int) h, src & 63, 64), h1 = (uint32_t) __shfl((int) h, (src + 1) & 63, 64);
+        const uint32_t l0 = (uint32_t) __shfl((int) lo, src & 63, 64), l1 = (uint32_t) __shfl((int) lo, (src + 1) & 63, 64);
+        const uint32_t hw = (h0 >> sh) | (h1 << (24 - sh)), lw = (l0 >> sh) | (l1 << (24 - sh));
+        uint8_t * o = out + blk * MX_ACT_BLK;
+        if (i < 4) {
+            *(uint32_t *) (o + cg * 16 + 4 * i) = hw;
+            *(uint32_t *) (o + 512 + cg * 16 + 4 * i) = lw;
+        } else if (i < 6) {
+            *(uint32_t *) (o + 1024 + cg * 8 + 4 * (i - 4)) = hw;
+            *(uint32_t *) (o + 1280 + cg * 8 + 4 * (i - 4)) = lw;
+        } else if (i == 6) {
+            out[4 * MX_ACT_BLK + cg * 4 + blk] = (uint8_t) e;
+        }
+    }
+}
+void launch_mx_act(hipStream_t s, const tdesc & b, void * act) {
+    const int64_t cols = b.ne[1] * b.ne[2] * b.ne[3], steps = mx_steps(b.ne[0]);
+    hipLaunchKernelGGL(k_mx_act<false>, dim3((unsigned) steps, (unsigned) ((cols + 31) / 32)), dim3(256), 0, s, b, cols, mx_lists{}, 1, (uint8_t *) act, (int) steps);
+}
+void launch_mx_group(hipStream_t s, const tdesc & ids, int64_t n_expert, void * ws) {
+    hipLaunchKernelGGL(k_mx_group, dim3((unsigned) n_expert), dim3(256), 0, s, ids, (int) n_expert, mx_lists_at(ws, mx_id_groups(n_expert, ids.ne[0] * ids.ne[1])));
+}
+void launch_mx_id_act(hipStream_t s, const tdesc & b, const tdesc & ids, int64_t n_expert, void * ws) {
+    const int64_t cols = ids.ne[0] * ids.ne[1], steps = mx_steps(b.ne[0]), g = mx_id_groups(n_expert, cols);
+    hipLaunchKernelGGL(k_mx_act<true>, dim3((unsigned) steps, (unsigned) g), dim3(256), 0, s, b, cols, mx_lists_at(ws, g), (int) ids.ne[0], (uint8_t *) ws + mx_lists_bytes(g), (int) steps);
+}
+
+// ------------------------------------------------------------------------------------------------ products
+struct mx_mm {
+    const uint8_t * w;
+    int64_t nb1, nb2;     // bytes between rows, between experts
+    int n_rows, blocks;   // rows of the (an expert's) matrix; blocks of a row
+    const uint8_t * act;
+    int steps;
+    int64_t cols;         // columns of the product (without lists)
+    float * dst;          // column c at dst + c ldd
+    int64_t ldd;
+    const float * bias;   // + bias[expert] (nb_bias bytes apart), or null
+    int64_t nb_bias;
+    mx_lists l;
+};
+__device__ __forceinline__ mx_i8 mx_op4(const mx_i4 a) { return mx_i8{a.x, a.y, a.z, a.w, 0, 0, 0, 0}; }
+__device__ __forceinline__ mx_i8 mx_op6(const mx_i4 a, const mx_i2 b) { return mx_i8{a.x, a.y, a.z, a.w, b.x, b.y, 0, 0}; }
+
+// A wave: 32 rows by a group of 32 columns, straight from memory; four waves of a workgroup one under the other
+template <bool ID> __global__ void __launch_bounds__(256) k_mx_mm(const mx_mm p) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, half = lane >> 5;
+    const int group = blockIdx.y, row0 = ((int) blockIdx.x * 4 + wave) * 32;
+    if (row0 >= p.n_rows) return;
+    int e = 0;
+    if (ID) {
+        if (group >= *p.l.total) return;
+        e = p.l.owner[group];
+    }
+    const uint8_t * w = p.w + (int64_t) e * p.nb2 + (int64_t) min(row0 + r32, p.n_rows - 1) * p.nb1;
+    const uint8_t * x = p.act + (int64_t) group * p.steps * MX_ACT_STEP;
+    mx_f16 acc = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    for (int step = 0; step < p.steps; ++step, x += MX_ACT_STEP) {
+        const uint32_t sx = *(const uint32_t *) (x + 4 * MX_ACT_BLK + r32 * 4);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int blk = 2 * j + half;
+            const bool in = step * 4 + blk < p.blocks;
+            const uint8_t * wb = w + (int64_t) (step * 4 + blk) * MX_BLOCK;
+            mx_i4 a = {0, 0, 0, 0};
+            int sa = 127;
+            if (in) {
+                a = *(const mx_i4_a1 *) (wb + 1);
+                sa = wb[0];
+            }
+            const uint8_t * xb = x + blk * MX_ACT_BLK;
+            const mx_i4 h = *(const mx_i4 *) (xb + r32 * 16), l = *(const mx_i4 *) (xb + 512 + r32 * 16);
+            const mx_i2 h2 = *(const mx_i2 *) (xb + 1024 + r32 * 8), l2 = *(const mx_i2 *) (xb + 1280 + r32 * 8);
+            const int sh = (int) ((sx >> (8 * blk)) & 255u);
+            acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_op4(a), mx_op6(h, h2), acc, MX_FP4, MX_FP6, 0, sa, 0, sh);
+            acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_op4(a), mx_op6(l, l2), acc, MX_FP4, MX_FP6, 0, sa, 0, sh - 4);
+        }
+    }
+    int64_t c = (int64_t) group * 32 + r32;
+    if (ID) c = p.l.list[c];
+    if (c < 0 || (!ID && c >= p.cols)) return;
+    float * d = p.dst + c * p.ldd;
+    const float * bias = p.bias ? (const float *) ((const char *) p.bias + (int64_t) e * p.nb_bias) : nullptr;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int row = row0 + 8 * (i / 4) + 4 * half + i % 4;
+        if (row < p.n_rows) d[row] = bias ? acc[i] + bias[row] : acc[i];
+    }
+}
+static mx_mm mx_args(const tdesc & w, const tdesc & d, const void * act) {
+    mx_mm p{};
+    p.w = (const uint8_t *) w.data;
+    p.nb1 = w.nb[1];
+    p.nb2 = w.nb[2];
+    p.n_rows = (int) w.ne[1];
+    p.blocks = (int) (w.ne[0] / 32);
+    p.act = (const uint8_t *) act;
+    p.steps = (int) mx_steps(w.ne[0]);
+    p.dst = (float *) d.data;
+    p.ldd = w.ne[1];
+    return p;
+}
+void launch_mx_mul_mat(hipStream_t s, const tdesc & w, const tdesc & b, const tdesc & d, const void * act) {
+    mx_mm p = mx_args(w, d, act);
+    p.cols = b.ne[1] * b.ne[2] * b.ne[3];
+    if (p.n_rows == 0 || p.cols == 0) return;
+    hipLaunchKernelGGL(k_mx_mm<false>, dim3((unsigned) ((p.n_rows + 127) / 128), (unsigned) ((p.cols + 31) / 32)), dim3(256), 0, s, p);
+}
+void launch_mx_mul_mat_id(hipStream_t s, const tdesc & w, const tdesc & ids, const tdesc & d, const void * ws, const float * bias, int64_t nb_bias) {
+    const int64_t g = mx_id_groups(w.ne[2], ids.ne[0] * ids.ne[1]);
+    mx_mm p = mx_args(w, d, (const uint8_t *) ws + mx_lists_bytes(g));
+    p.l = mx_lists_at((void *) ws, g);
+    p.bias = bias;
+    p.nb_bias = nb_bias;
+    if (p.n_rows == 0 || g == 0) return;
+    hipLaunchKernelGGL(k_mx_mm<true>, dim3((unsigned) ((p.n_rows + 127) / 128), (unsigned) g), dim3(256), 0, s, p);
+}
+// which operands the products take (type and shape; the rows of both are dense, whole blocks)
+bool mx_product_ok(const tdesc & w, const tdesc & b) {
+    return w.ne[0] % 32 == 0 && w.ne[0] > 0 && w.ne[1] < ((int64_t) 1 << 31) - 256 && w.ne[0] < ((int64_t) 1 << 31) - 256 && w.nb[0] == MX_BLOCK && b.nb[0] == 4 && b.nb[1] % 4 == 0 && b.nb[2] % 4 == 0 && b.nb[3] % 4 == 0 &&
+           (b.ne[1] * b.ne[2] * b.ne[3] + 31) / 32 <= 65535;
+}
+bool mx_id_ok(const tdesc & w, const tdesc & ids) {
+    return w.ne[2] <= MX_MAX_EXPERTS && ids.nb[0] % 4 == 0 && ids.nb[1] % 4 == 0 && ids.ne[0] * ids.ne[1] < ((int64_t) 1 << 30) && mx_id_groups(w.ne[2], ids.ne[0] * ids.ne[1]) <= 65535;
+}
+
+// ------------------------------------------------------------------------------------------------ ADD_ID
+// a [N, n_used, T] + the row of b [N, n_expert] that ids [n_used, T] names (an id outside them: a's row alone)
+__global__ void __launch_bounds__(256) k_add_id(const tdesc a, const tdesc b, const tdesc ids, const tdesc d) {
+    const int64_t u = blockIdx.y, t = blockIdx.z, n = (int64_t) blockIdx.x * 256 + threadIdx.x;
+    if (n >= a.ne[0]) return;
+    const int32_t e = *(const int32_t *) (ids.data + u * ids.nb[0] + t * ids.nb[1]);
+    float v = *(const float *) (a.data + n * 4 + u * a.nb[1] + t * a.nb[2]);
+    if (e >= 0 && e < b.ne[1]) v += *(const float *) (b.data + n * 4 + (int64_t) e * b.nb[1]);
+    *(float *) (d.data + n * 4 + u * d.nb[1] + t * d.nb[2]) = v;
+}
+void launch_add_id(hipStream_t s, const tdesc & a, const tdesc & b, const tdesc & ids, const tdesc & d) {
+    if (a.ne[0] * a.ne[1] * a.ne[2] == 0) return;
+    hipLaunchKernelGGL(k_add_id, dim3((unsigned) ((a.ne[0] + 255) / 256), (unsigned) a.ne[1], (unsigned) a.ne[2]), dim3(256), 0, s, a, b, ids, d);
+}
+
+MI_TU_TOUCH(mx)
+
+}  // namespace mi355x

@@ -80,6 +80,7 @@ const char * ggml_type_name(enum ggml_type type) {
         case GGML_TYPE_Q5_K: return "q5_K";
         case GGML_TYPE_Q6_K: return "q6_K";
         case GGML_TYPE_Q8_K: return "q8_K";
+        case GGML_TYPE_MXFP4: return "mxfp4";
         case GGML_TYPE_I32: return "i32";
         case GGML_TYPE_I64: return "i64";
         default: return "?";
@@ -328,6 +329,16 @@ struct ggml_tensor * ggml_add(struct ggml_context * ctx, struct ggml_tensor * a,
 struct ggml_tensor * ggml_sub(struct ggml_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b) { return binary(ctx, GGML_OP_SUB, a, b); }
 struct ggml_tensor * ggml_mul(struct ggml_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b) { return binary(ctx, GGML_OP_MUL, a, b); }
 struct ggml_tensor * ggml_div(struct ggml_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b) { return binary(ctx, GGML_OP_DIV, a, b); }
+
+struct ggml_tensor * ggml_add_id(struct ggml_context * ctx, struct ggml_tensor * a, struct ggml_tensor * b, struct ggml_tensor * ids) {
+    LITE_ASSERT(a->ne[0] == b->ne[0] && a->ne[1] == ids->ne[0] && a->ne[2] == ids->ne[1] && a->ne[3] == 1 && ids->type == GGML_TYPE_I32);
+    ggml_tensor * r = dup_tensor(ctx, a);
+    r->op = GGML_OP_ADD_ID;
+    r->src[0] = a;
+    r->src[1] = b;
+    r->src[2] = ids;
+    return r;
+}
 
 struct ggml_tensor * ggml_scale_bias(struct ggml_context * ctx, struct ggml_tensor * a, float s, float b) {
     ggml_tensor * r = dup_tensor(ctx, a);
