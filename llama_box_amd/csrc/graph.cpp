@@ -2928,8 +2928,8 @@ static int run_mul_mat_mx(exec_state & st, int i) {
     backend_ctx * c = st.c;
     ggml_tensor * n = st.g->nodes[i];
     const ggml_tensor * a = n->src[0], * b = n->src[1];
-    void * act = (char *) c->ws + st.act_off;
-    if (!c->act.holds(b, MI_ACT_MX)) {
+    void * act = mx_vec_takes(b->ne[0], b->ne[1] * b->ne[2] * b->ne[3]) ? nullptr : (char *) c->ws + st.act_off;
+    if (act && !c->act.holds(b, MI_ACT_MX)) {
         timed_scope ts(c, "quantize_act", (double) ggml_abi_nbytes(b));
         launch_mx_act(c->stream, TD(b), act);
         c->st.kernel_launches++;
@@ -2954,29 +2954,31 @@ static int run_mul_mat_id_mx(exec_state & st, int i) {
     ggml_cgraph * g = st.g;
     ggml_tensor * n = g->nodes[i];
     const ggml_tensor * a = n->src[0], * b = n->src[1], * ids = n->src[2];
-    void * ws = (char *) c->ws + st.act_off;
+    void * ws = mx_id_vec_takes(b->ne[0], ids->ne[0] * ids->ne[1]) ? nullptr : (char *) c->ws + st.act_off;
     bool lists = st.mx_node >= 0 && st.mx_ids == ids && st.mx_experts == a->ne[2] && c->act.kind == MI_ACT_MX_ID;
     for (int k = st.mx_node + 1; lists && k < i; ++k) lists = is_view_op(g->nodes[k]) || !ranges_overlap(g->nodes[k], ids);
     const bool cols = lists && c->act.holds(b, MI_ACT_MX_ID);
-    if (!lists) {
+    if (ws && !lists) {
         timed_scope ts(c, "moe_group", (double) ggml_abi_nbytes(ids));
         launch_mx_group(c->stream, TD(ids), a->ne[2], ws);
         c->st.kernel_launches++;
     }
-    if (!cols) {
+    if (ws && !cols) {
         timed_scope ts(c, "quantize_act", (double) ggml_abi_nbytes(b));
         launch_mx_id_act(c->stream, TD(b), TD(ids), a->ne[2], ws);
         c->st.kernel_launches++;
         c->act.set(b, MI_ACT_MX_ID);
     }
-    st.mx_node = i;
-    st.mx_ids = ids;
-    st.mx_experts = a->ne[2];
+    if (ws) {
+        st.mx_node = i;
+        st.mx_ids = ids;
+        st.mx_experts = a->ne[2];
+    }
     // (the bias: the result alone reads the product, of the same ids, and is not stored over what the launch still reads)
     ggml_tensor * ad = i + 1 < g->n_nodes && !st.done[i + 1] ? g->nodes[i + 1] : nullptr;
     const bool bias = c->opt.fusion && ad && ad->op == GGML_OP_ADD_ID && ad->src[0] == n && ad->src[2] == ids && single_use(st, n) && is_f32_contig(ad) && supports_op(ad) && !ranges_overlap(ad, ad->src[1]) && !ranges_overlap(ad, ids);
     timed_scope ts(c, "mul_mat_id_mxfp4", (double) ggml_abi_nbytes(a) / (double) std::max<int64_t>(1, a->ne[2]) * (double) std::min<int64_t>(a->ne[2], ggml_abi_nelements(ids)));
-    launch_mx_mul_mat_id(c->stream, TD(a), TD(ids), TD(bias ? ad : n), ws, bias ? (const float *) ad->src[1]->data : nullptr, bias ? (int64_t) ad->src[1]->nb[1] : 0);
+    launch_mx_mul_mat_id(c->stream, TD(a), TD(b), TD(ids), TD(bias ? ad : n), ws, bias ? (const float *) ad->src[1]->data : nullptr, bias ? (int64_t) ad->src[1]->nb[1] : 0);
     c->st.kernel_launches++;
     c->st.fused_nodes += bias;
     return bias ? 2 : 1;

@@ -538,18 +538,20 @@ void launch_argsort_grouped(hipStream_t s, const tdesc & src, const tdesc & dst,
 // f32 rows -> MXFP4 and back; idx: the places of SET_ROWS (I64) / the rows of GET_ROWS (I32), null: row by row (CPY)
 void launch_mx_store(hipStream_t s, const tdesc & a, const tdesc * idx, const tdesc & d);
 void launch_mx_read(hipStream_t s, const tdesc & a, const tdesc * idx, const tdesc & d);
-// MUL_MAT: w [K, N], b f32 rows of K, d dense.  act: mx_act_bytes(K, columns) that launch_mx_act has filled from b
+// MUL_MAT: w [K, N], b f32 rows of K, d dense.  act: mx_act_bytes(K, columns) that launch_mx_act has filled from b; null for the few columns that the product quantises itself (mx_vec_takes)
+bool mx_vec_takes(int64_t K, int64_t cols);
+bool mx_id_vec_takes(int64_t K, int64_t cols);
 bool mx_product_ok(const tdesc & w, const tdesc & b);
 size_t mx_act_bytes(int64_t K, int64_t cols);
 void launch_mx_act(hipStream_t s, const tdesc & b, void * act);
 void launch_mx_mul_mat(hipStream_t s, const tdesc & w, const tdesc & b, const tdesc & d, const void * act);
 // MUL_MAT_ID: w [K, N, n_expert], b [K, 1 or n_used, T], ids [n_used, T], d dense; bias: rows [N] of the experts, added where they are stored, or null.
-// ws: mx_id_act_bytes(K, n_expert, n_used T), first the lists (launch_mx_group), then the columns (launch_mx_id_act)
+// ws: mx_id_act_bytes(K, n_expert, n_used T), first the lists (launch_mx_group), then the columns (launch_mx_id_act); null where mx_id_vec_takes
 bool mx_id_ok(const tdesc & w, const tdesc & ids);
 size_t mx_id_act_bytes(int64_t K, int64_t n_expert, int64_t cols);
 void launch_mx_group(hipStream_t s, const tdesc & ids, int64_t n_expert, void * ws);
 void launch_mx_id_act(hipStream_t s, const tdesc & b, const tdesc & ids, int64_t n_expert, void * ws);
-void launch_mx_mul_mat_id(hipStream_t s, const tdesc & w, const tdesc & ids, const tdesc & d, const void * ws, const float * bias, int64_t nb_bias);
+void launch_mx_mul_mat_id(hipStream_t s, const tdesc & w, const tdesc & b, const tdesc & ids, const tdesc & d, const void * ws, const float * bias, int64_t nb_bias);
 // ADD_ID: a [N, n_used, T] + the rows of b [N, n_expert] that ids names
 void launch_add_id(hipStream_t s, const tdesc & a, const tdesc & b, const tdesc & ids, const tdesc & d);
 

@@ -16,6 +16,7 @@ namespace mi355x {
 typedef int mx_i4 __attribute__((ext_vector_type(4)));
 typedef int mx_i2 __attribute__((ext_vector_type(2)));
 typedef int mx_i8 __attribute__((ext_vector_type(8)));
+typedef float mx_f4 __attribute__((ext_vector_type(4)));
 typedef float mx_f16 __attribute__((ext_vector_type(16)));
 typedef mx_i4 __attribute__((aligned(1))) mx_i4_a1;  // (a block's codes start anywhere)
 typedef uint16_t __attribute__((aligned(1))) mx_u16_a1;
@@ -134,25 +135,29 @@ void launch_mx_read(hipStream_t s, const tdesc & a, const tdesc * idx, const tde
 // ------------------------------------------------------------------------------------------------ activations
 // The quantised columns lie in groups of 32, a group in steps of 128 values (four blocks), as the lanes of a product fetch them: for each block the 16 first bytes of h of the 32 columns, those of l, the
 // 8 last bytes of h, those of l (24 bytes are 32 codes of 6 bits), and behind the four blocks 4 scale bytes a column.  A block's codes stand in the order of the weights' nibbles: value j at place 2j,
-// value 16 + j at place 2j + 1.  The scale byte is h's exponent, s + 7 + 127; l's is 4 less.  Blocks behind the last one of a row are zeros.
+// value 16 + j at place 2j + 1.  The scale byte is h's exponent, s + 7 + 127; l's is 4 less.  Blocks behind the last one of a row are zeros (a product takes the row's last block once more for them: whatever it holds, its own product is in the sum already).
 static constexpr int MX_ACT_BLK = 32 * 48, MX_ACT_STEP = 4 * MX_ACT_BLK + 32 * 4;
 static inline int64_t mx_steps(int64_t K) { return (K + 127) / 128; }
 size_t mx_act_bytes(int64_t K, int64_t cols) { return (size_t) ((cols + 31) / 32) * (size_t) (mx_steps(K) * MX_ACT_STEP); }
 
-// Columns of MUL_MAT_ID sorted by expert, every expert's first column in a group of its own: list[p] the column (u + n_used t) at place p or -1, owner[g] the expert of group g, total the groups in use
+// Columns of MUL_MAT_ID sorted by expert, every expert's first column in a group of its own: list[p] the column (u + n_used t) at place p or -1, owner[g] the expert of group g, tiles[4 t]: up to
+// MX_TILE groups of one expert as (expert, first group, groups); total[0] and total[1]: groups and tiles in use
 struct mx_lists {
-    int32_t * total, * owner, * list;
+    int32_t * total, * tiles, * owner, * list;
 };
+static constexpr int MX_TILE = 4;
 // ids outside the experts are in no list: their columns are left as they are
 static int64_t mx_id_groups(int64_t n_expert, int64_t cols) { return cols / 32 + std::min(n_expert, cols); }  // (at most: an expert's last group may hold one column)
-static mx_lists mx_lists_at(void * ws, int64_t groups) {
+static int64_t mx_id_tiles(int64_t n_expert, int64_t cols) { return cols / (32 * MX_TILE) + std::min(n_expert, cols); }
+static mx_lists mx_lists_at(void * ws, int64_t groups) {  // (no more tiles than groups)
     mx_lists l;
     l.total = (int32_t *) ws;
-    l.owner = l.total + 4;
+    l.tiles = l.total + 4;
+    l.owner = l.tiles + 4 * groups;
     l.list = l.owner + ((groups + 3) & ~(int64_t) 3);
     return l;
 }
-static size_t mx_lists_bytes(int64_t groups) { return ((size_t) (4 + ((groups + 3) & ~(int64_t) 3) + groups * 32) * 4 + 255) & ~(size_t) 255; }
+static size_t mx_lists_bytes(int64_t groups) { return ((size_t) (4 + 4 * groups + ((groups + 3) & ~(int64_t) 3) + groups * 32) * 4 + 255) & ~(size_t) 255; }
 size_t mx_id_act_bytes(int64_t K, int64_t n_expert, int64_t cols) {
     const int64_t g = mx_id_groups(n_expert, cols);
     return mx_lists_bytes(g) + mx_act_bytes(K, 32 * g);
@@ -160,7 +165,7 @@ size_t mx_id_act_bytes(int64_t K, int64_t n_expert, int64_t cols) {
 static constexpr int MX_MAX_EXPERTS = 1024;
 // One workgroup an expert: every workgroup counts all experts' columns (whole numbers in LDS: no order to depend on), takes the groups in front of its own, and lists its columns in ascending order
 __global__ void __launch_bounds__(256) k_mx_group(const tdesc ids, const int n_expert, const mx_lists l) {
-    __shared__ int cnt[MX_MAX_EXPERTS], s_before[4], s_wave[4];
+    __shared__ int cnt[MX_MAX_EXPERTS], s_before[4], s_tiles[4], s_wave[4];
     const int e = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n_used = (int) ids.ne[0], n = n_used * (int) ids.ne[1];
     auto id_at = [&](const int i) { return *(const int32_t *) (ids.data + (int64_t) (i % n_used) * ids.nb[0] + (int64_t) (i / n_used) * ids.nb[1]); };
@@ -171,15 +176,35 @@ __global__ void __launch_bounds__(256) k_mx_group(const tdesc ids, const int n_e
         if (v >= 0 && v < n_expert) atomicAdd(&cnt[v], 1);
     }
     __syncthreads();
-    int before = 0;
-    for (int i = threadIdx.x; i < e; i += 256) before += (cnt[i] + 31) / 32;
-    for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o, 64);
-    if (lane == 0) s_before[wave] = before;
+    int before = 0, before_t = 0;
+    for (int i = threadIdx.x; i < e; i += 256) {
+        const int gi = (cnt[i] + 31) / 32;
+        before += gi;
+        before_t += (gi + MX_TILE - 1) / MX_TILE;
+    }
+    for (int o = 32; o > 0; o >>= 1) {
+        before += __shfl_xor(before, o, 64);
+        before_t += __shfl_xor(before_t, o, 64);
+    }
+    if (lane == 0) {
+        s_before[wave] = before;
+        s_tiles[wave] = before_t;
+    }
     __syncthreads();
-    const int g0 = s_before[0] + s_before[1] + s_before[2] + s_before[3], mine = cnt[e], groups = (mine + 31) / 32;
+    const int g0 = s_before[0] + s_before[1] + s_before[2] + s_before[3], t0 = s_tiles[0] + s_tiles[1] + s_tiles[2] + s_tiles[3];
+    const int mine = cnt[e], groups = (mine + 31) / 32, tiles = (groups + MX_TILE - 1) / MX_TILE;
+    for (int i = threadIdx.x; i < tiles; i += 256) {
+        int32_t * t = l.tiles + 4 * (t0 + i);
+        t[0] = e;
+        t[1] = g0 + MX_TILE * i;
+        t[2] = min(MX_TILE, groups - MX_TILE * i);
+    }
     for (int i = threadIdx.x; i < groups; i += 256) l.owner[g0 + i] = e;
     for (int i = mine + (int) threadIdx.x; i < groups * 32; i += 256) l.list[g0 * 32 + i] = -1;
-    if (e == n_expert - 1 && threadIdx.x == 0) *l.total = g0 + groups;
+    if (e == n_expert - 1 && threadIdx.x == 0) {
+        l.total[0] = g0 + groups;
+        l.total[1] = t0 + tiles;
+    }
     int placed = 0;
     for (int i0 = 0; i0 < n; i0 += 256) {
         const int i = i0 + (int) threadIdx.x;
@@ -215,7 +240,7 @@ __device__ __forceinline__ uint32_t mx_act4(const float (&v)[4], uint32_t & h, u
 // One workgroup a group of columns and a step of 128 values; eight lanes a block, eight columns at a time.  ID: column c of the list is row (c % n_used) % b.ne[1] of token c / n_used
 template <bool ID> __global__ void __launch_bounds__(256) k_mx_act(const tdesc b, const int64_t n_cols, const mx_lists l, const int n_used, uint8_t * __restrict__ act, const int steps) {
     const int step = blockIdx.x, group = blockIdx.y;
-    if (ID && group >= *l.total) return;
+    if (ID && group >= l.total[0]) return;
     const int i = threadIdx.x & 7, blk = (threadIdx.x >> 3) & 3, lane = threadIdx.x & 63;
     const int64_t k0 = (int64_t) step * 128 + blk * 32;
     uint8_t * out = act + ((int64_t) group * steps + step) * MX_ACT_STEP;
@@ -270,7 +295,8 @@ struct mx_mm {
     int n_rows, blocks;   // rows of the (an expert's) matrix; blocks of a row
     const uint8_t * act;
     int steps;
-    int64_t cols;         // columns of the product (without lists)
+    int64_t cols;         // columns of the product
+    int n_expert;
     float * dst;          // column c at dst + c ldd
     int64_t ldd;
     const float * bias;   // + bias[expert] (nb_bias bytes apart), or null
@@ -280,78 +306,389 @@ struct mx_mm {
 __device__ __forceinline__ mx_i8 mx_op4(const mx_i4 a) { return mx_i8{a.x, a.y, a.z, a.w, 0, 0, 0, 0}; }
 __device__ __forceinline__ mx_i8 mx_op6(const mx_i4 a, const mx_i2 b) { return mx_i8{a.x, a.y, a.z, a.w, b.x, b.y, 0, 0}; }
 
-// A wave: 32 rows by a group of 32 columns, straight from memory; four waves of a workgroup one under the other
-template <bool ID> __global__ void __launch_bounds__(256) k_mx_mm(const mx_mm p) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, half = lane >> 5;
-    const int group = blockIdx.y, row0 = ((int) blockIdx.x * 4 + wave) * 32;
-    if (row0 >= p.n_rows) return;
-    int e = 0;
+// ---- one to a few columns: 16 rows a workgroup, its waves take the steps of 128 values in turn.  The workgroup quantises its columns itself, while its first weights are on the way: a launch in front
+// costs more (see the table of times at the launcher).  A lane of v_mfma_scale_f32_16x16x128: row (column) lane % 16, block lane / 16 of the step.
+// ID: blockIdx.y is a column (u + n_used t) of at most 64; the first column of an expert takes all of its expert, the others' workgroups end at once.
+static constexpr int MX_VEC_AHEAD = 8;    // steps whose weights a wave has on the way
+static constexpr int MX_VEC_REC = 48;     // LDS bytes of a block of one column: 16 of h, 16 of l, 8 of h, 8 of l
+template <bool ID> __global__ void __launch_bounds__(1024) k_mx_vec(const mx_mm p, const tdesc b, const tdesc ids, const int chunk) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    __shared__ int s_cols[64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, r16 = lane & 15, q = lane >> 4;
+    const int row0 = (int) blockIdx.x * 16, blocks4 = p.steps * 4;
+    int e = 0, n = (int) p.cols;
     if (ID) {
-        if (group >= *p.l.total) return;
-        e = p.l.owner[group];
+        const int n_used = (int) ids.ne[0], slot = blockIdx.y;
+        const int id = lane < n ? *(const int32_t *) (ids.data + (int64_t) (lane % n_used) * ids.nb[0] + (int64_t) (lane / n_used) * ids.nb[1]) : -1;
+        e = __builtin_amdgcn_readlane(id, slot);
+        if (e < 0 || e >= p.n_expert) return;
+        const uint64_t mine = __ballot(id == e);
+        if (mine & ((1ull << slot) - 1ull)) return;
+        n = __popcll(mine);
+        if (wave == 0 && id == e) s_cols[__popcll(mine & ((1ull << lane) - 1ull))] = lane;
     }
-    const uint8_t * w = p.w + (int64_t) e * p.nb2 + (int64_t) min(row0 + r32, p.n_rows - 1) * p.nb1;
-    const uint8_t * x = p.act + (int64_t) group * p.steps * MX_ACT_STEP;
-    mx_f16 acc = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-    for (int step = 0; step < p.steps; ++step, x += MX_ACT_STEP) {
-        const uint32_t sx = *(const uint32_t *) (x + 4 * MX_ACT_BLK + r32 * 4);
+    const uint8_t * w = p.w + (int64_t) e * p.nb2 + (int64_t) min(row0 + r16, p.n_rows - 1) * p.nb1;
+    uint8_t * s_rec = lds, * s_scale = lds + (size_t) chunk * blocks4 * MX_VEC_REC;  // [block][column of the chunk]
+    float * s_part = (float *) (lds + (((size_t) chunk * blocks4 * (MX_VEC_REC + 1) + 15) & ~(size_t) 15));  // [wave][column][row]
+    const float * bias = p.bias ? (const float *) ((const char *) p.bias + (int64_t) e * p.nb_bias) : nullptr;
+    for (int c0 = 0; c0 < n; c0 += chunk) {
+        const int m = min(chunk, n - c0);
+        mx_i4 a[MX_VEC_AHEAD];
+        int sa[MX_VEC_AHEAD];
+        auto fetch = [&](const int s0) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int blk = 2 * j + half;
-            const bool in = step * 4 + blk < p.blocks;
-            const uint8_t * wb = w + (int64_t) (step * 4 + blk) * MX_BLOCK;
-            mx_i4 a = {0, 0, 0, 0};
-            int sa = 127;
-            if (in) {
-                a = *(const mx_i4_a1 *) (wb + 1);
-                sa = wb[0];
+            for (int u = 0; u < MX_VEC_AHEAD; ++u) {
+                const uint8_t * wb = w + min((s0 + u * waves) * 4 + q, p.blocks - 1) * MX_BLOCK;
+                a[u] = *(const mx_i4_a1 *) (wb + 1);
+                sa[u] = wb[0];
             }
-            const uint8_t * xb = x + blk * MX_ACT_BLK;
-            const mx_i4 h = *(const mx_i4 *) (xb + r32 * 16), l = *(const mx_i4 *) (xb + 512 + r32 * 16);
-            const mx_i2 h2 = *(const mx_i2 *) (xb + 1024 + r32 * 8), l2 = *(const mx_i2 *) (xb + 1280 + r32 * 8);
-            const int sh = (int) ((sx >> (8 * blk)) & 255u);
-            acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_op4(a), mx_op6(h, h2), acc, MX_FP4, MX_FP6, 0, sa, 0, sh);
-            acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_op4(a), mx_op6(l, l2), acc, MX_FP4, MX_FP6, 0, sa, 0, sh - 4);
+        };
+        fetch(wave);
+        if (ID || c0) __syncthreads();  // (the columns' list; the last chunk's partial sums and digits are read)
+        for (int at = threadIdx.x; at < 8 * blocks4 * m; at += blockDim.x) {  // eight lanes a block (blocks4 is a multiple of four: whole half-waves)
+            const int i = at & 7, c = (at >> 3) / blocks4, blk = (at >> 3) - c * blocks4;
+            const char * col;
+            if (ID) {
+                const int cc = s_cols[c0 + c], n_used = (int) ids.ne[0];
+                col = b.data + ((cc % n_used) % b.ne[1]) * b.nb[1] + (int64_t) (cc / n_used) * b.nb[2];
+            } else {
+                const int cc = c0 + c, n1 = (int) b.ne[1], n2 = (int) b.ne[2];
+                col = b.data + (cc % n1) * b.nb[1] + (int64_t) ((cc / n1) % n2) * b.nb[2] + (int64_t) (cc / (n1 * n2)) * b.nb[3];
+            }
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (blk < p.blocks) mx_load4((const float *) col + blk * 32, i, v);
+            uint32_t h, l;
+            const uint32_t se = mx_act4(v, h, l);
+            uint8_t * rec = s_rec + ((size_t) blk * chunk + c) * MX_VEC_REC;
+            // (24 bits a lane: three bytes of h's 24, three of l's)
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+                const int o = 3 * i + k;
+                rec[o < 16 ? o : o + 16] = (uint8_t) (h >> (8 * k));
+                rec[o < 16 ? o + 16 : o + 24] = (uint8_t) (l >> (8 * k));
+            }
+            if (i == 0) s_scale[blk * chunk + c] = (uint8_t) se;
+        }
+        __syncthreads();
+        mx_f4 acc = {0, 0, 0, 0};
+        for (int s0 = wave; s0 < p.steps; s0 += MX_VEC_AHEAD * waves) {
+            if (s0 != wave) fetch(s0);
+#pragma unroll
+            for (int u = 0; u < MX_VEC_AHEAD; ++u) {
+                const int step = s0 + u * waves;
+                if (step >= p.steps) break;
+                mx_i4 h = {0, 0, 0, 0}, l = {0, 0, 0, 0};
+                mx_i2 h2 = {0, 0}, l2 = {0, 0};
+                int sh = 127;
+                if (r16 < m) {
+                    const int at = (step * 4 + q) * chunk + r16;
+                    const uint8_t * rec = s_rec + (size_t) at * MX_VEC_REC;
+                    h = *(const mx_i4 *) rec;
+                    l = *(const mx_i4 *) (rec + 16);
+                    h2 = *(const mx_i2 *) (rec + 32);
+                    l2 = *(const mx_i2 *) (rec + 40);
+                    sh = s_scale[at];
+                }
+                acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_op4(a[u]), mx_op6(h, h2), acc, MX_FP4, MX_FP6, 0, sa[u], 0, sh);
+                acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_op4(a[u]), mx_op6(l, l2), acc, MX_FP4, MX_FP6, 0, sa[u], 0, sh - 4);
+            }
+        }
+        if (r16 < m) *(mx_f4 *) (s_part + ((wave * chunk + r16) * 16 + 4 * q)) = acc;
+        __syncthreads();
+        if ((int) threadIdx.x < 16 * m) {
+            const int row = threadIdx.x & 15, c = threadIdx.x >> 4;
+            float v = 0.0f;
+            for (int k = 0; k < waves; ++k) v += s_part[(k * chunk + c) * 16 + row];
+            if (row0 + row < p.n_rows) p.dst[(int64_t) (ID ? s_cols[c0 + c] : c0 + c) * p.ldd + row0 + row] = bias ? v + bias[row0 + row] : v;
         }
     }
+}
+
+// ---- up to a few groups of columns: 32 rows by CT groups a workgroup, its waves take the steps in turn, everything straight from memory; the waves' sums are added in LDS in their order
+template <bool ID, int CT> __global__ void __launch_bounds__(512) k_mx_few(const mx_mm p) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, r32 = lane & 31, half = lane >> 5;
+    const int group0 = blockIdx.y * CT, row0 = (int) blockIdx.x * 32;
+    int e = 0;
+    if (ID) {
+        if (group0 >= p.l.total[0]) return;
+        e = p.l.owner[group0];
+    }
+    const uint8_t * w = p.w + (int64_t) e * p.nb2 + (int64_t) min(row0 + r32, p.n_rows - 1) * p.nb1;
+    const uint8_t * x = p.act + (int64_t) group0 * p.steps * MX_ACT_STEP;
+    const int64_t group_bytes = (int64_t) p.steps * MX_ACT_STEP;
+    int64_t col[CT];  // the lane's columns, -1: none
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        col[c] = (int64_t) (group0 + c) * 32 + r32;
+        if (ID) col[c] = p.l.list[col[c]];
+        else if (col[c] >= p.cols) col[c] = -1;
+    }
+    mx_f16 acc[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
+    struct part { mx_i4 a[2]; int sa[2]; mx_i4 h[CT][2], l[CT][2]; mx_i2 h2[CT][2], l2[CT][2]; uint32_t sx[CT]; };
+    auto fetch = [&](const int step, part & f) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint8_t * wb = w + min(step * 4 + 2 * j + half, p.blocks - 1) * MX_BLOCK;
+            f.a[j] = *(const mx_i4_a1 *) (wb + 1);
+            f.sa[j] = wb[0];
+        }
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            f.sx[c] = 0x7F7F7F7Fu;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                f.h[c][j] = f.l[c][j] = mx_i4{0, 0, 0, 0};
+                f.h2[c][j] = f.l2[c][j] = mx_i2{0, 0};
+            }
+            if (col[c] >= 0) {
+                const uint8_t * xs = x + c * group_bytes + (int64_t) step * MX_ACT_STEP;
+                f.sx[c] = *(const uint32_t *) (xs + 4 * MX_ACT_BLK + r32 * 4);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint8_t * xb = xs + (2 * j + half) * MX_ACT_BLK;
+                    f.h[c][j] = *(const mx_i4 *) (xb + r32 * 16);
+                    f.l[c][j] = *(const mx_i4 *) (xb + 512 + r32 * 16);
+                    f.h2[c][j] = *(const mx_i2 *) (xb + 1024 + r32 * 8);
+                    f.l2[c][j] = *(const mx_i2 *) (xb + 1280 + r32 * 8);
+                }
+            }
+        }
+    };
+    auto add = [&](const part & f) {
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int sh = (int) ((f.sx[c] >> (16 * j + 8 * half)) & 255u);
+                acc[c] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_op4(f.a[j]), mx_op6(f.h[c][j], f.h2[c][j]), acc[c], MX_FP4, MX_FP6, 0, f.sa[j], 0, sh);
+                acc[c] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_op4(f.a[j]), mx_op6(f.l[c][j], f.l2[c][j]), acc[c], MX_FP4, MX_FP6, 0, f.sa[j], 0, sh - 4);
+            }
+    };
+    part f0, f1;
+    int step = wave;
+    if (step < p.steps) fetch(step, f0);
+    for (; step < p.steps; step += 2 * waves) {
+        if (step + waves < p.steps) fetch(step + waves, f1);
+        add(f0);
+        if (step + 2 * waves < p.steps) fetch(step + 2 * waves, f0);
+        if (step + waves < p.steps) add(f1);
+    }
+    // [wave][group][column][row], the rows of a column 36 apart (of 32: no two quarters of a wave on the same banks)
+    float * part_sums = (float *) lds;
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *(mx_f4 *) (part_sums + ((wave * CT + c) * 32 + r32) * 36 + 8 * i + 4 * half) = mx_f4{acc[c][4 * i], acc[c][4 * i + 1], acc[c][4 * i + 2], acc[c][4 * i + 3]};
+    __syncthreads();
+    const float * bias = p.bias ? (const float *) ((const char *) p.bias + (int64_t) e * p.nb_bias) : nullptr;
+    for (int at = threadIdx.x; at < CT * 32 * 32; at += blockDim.x) {
+        const int row = at & 31, cg = at >> 5;  // column cg of the CT groups
+        int64_t c = (int64_t) group0 * 32 + cg;
+        if (ID) c = p.l.list[c];
+        else if (c >= p.cols) c = -1;
+        if (c < 0 || row0 + row >= p.n_rows) continue;
+        float v = 0.0f;
+        for (int k = 0; k < waves; ++k) v += part_sums[(k * CT * 32 + cg) * 36 + row];
+        p.dst[c * p.ldd + row0 + row] = bias ? v + bias[row0 + row] : v;
+    }
+}
+
+// ---- many columns: 32 RT rows by four groups of columns a workgroup.  A wave has one group and all rows: its digits come straight from memory (no other wave reads them), the weights through LDS,
+// where their blocks are aligned ([block of the step][row] 16 bytes, and 4 scale bytes a row).  While a step is multiplied, the next one's weights and digits are on the way to registers.
+template <bool ID, int RT> __global__ void __launch_bounds__(256, 2) k_mx_tile(const mx_mm p, const int row_tiles) {
+    constexpr int ROWS = 32 * RT;
+    __shared__ __align__(16) uint8_t s_w[2][4 * ROWS * 16];
+    __shared__ __align__(16) uint8_t s_s[2][ROWS * 4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r32 = lane & 31, half = lane >> 5;
+    int rt, tile;
+    if (ID) {
+        rt = blockIdx.x % row_tiles;
+        tile = blockIdx.x / row_tiles;
+    } else {
+        // consecutive workgroups go to the eight dies in turn: each die has a run of tiles, the column tiles of a row tile one after the other, so that the weights stay in its L2
+        const int n_tiles = (int) ((p.cols + 127) / 128), at = (int) (blockIdx.x & 7) * (int) (gridDim.x >> 3) + (int) (blockIdx.x >> 3);
+        tile = at % n_tiles;
+        rt = at / n_tiles;
+        if (rt >= row_tiles) return;
+    }
+    const int row0 = rt * ROWS;
+    int e = 0, group = tile * 4 + wave, groups = (int) ((p.cols + 31) / 32);
+    if (ID) {
+        if (tile >= p.l.total[1]) return;
+        const int32_t * t = p.l.tiles + 4 * tile;
+        e = t[0];
+        group = t[1] + wave;
+        groups = t[1] + t[2];
+    }
+    const bool live = group < groups;
+    // loads: four lanes a row
+    const int lblk = tid & 3, lrow = tid >> 2;
+    const uint8_t * wl[RT / 2];
+#pragma unroll
+    for (int i = 0; i < RT / 2; ++i) wl[i] = p.w + (int64_t) e * p.nb2 + (int64_t) min(row0 + lrow + 64 * i, p.n_rows - 1) * p.nb1;
+    mx_i4 wr[RT / 2];
+    uint8_t ws[RT / 2];
+    auto fetch_w = [&](const int step) {
+        const int at = min(step * 4 + lblk, p.blocks - 1) * MX_BLOCK;
+#pragma unroll
+        for (int i = 0; i < RT / 2; ++i) {
+            wr[i] = *(const mx_i4_a1 *) (wl[i] + at + 1);
+            ws[i] = wl[i][at];
+        }
+    };
+    auto store_w = [&](const int buf) {
+#pragma unroll
+        for (int i = 0; i < RT / 2; ++i) {
+            *(mx_i4 *) (s_w[buf] + ((lblk * ROWS) + lrow + 64 * i) * 16) = wr[i];
+            s_s[buf][(lrow + 64 * i) * 4 + lblk] = ws[i];
+        }
+    };
+    const uint8_t * x = p.act + (int64_t) (live ? group : groups - 1) * p.steps * MX_ACT_STEP;
+    mx_i8 h[2], l[2], hn[2], ln[2];  // the digits of this step and of the next
+    uint32_t sx, sxn;
+    auto fetch_x = [&](const int step) {
+        const uint8_t * xs = x + (int64_t) step * MX_ACT_STEP;
+        sxn = *(const uint32_t *) (xs + 4 * MX_ACT_BLK + r32 * 4);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint8_t * xb = xs + (2 * j + half) * MX_ACT_BLK;
+            hn[j] = mx_op6(*(const mx_i4 *) (xb + r32 * 16), *(const mx_i2 *) (xb + 1024 + r32 * 8));
+            ln[j] = mx_op6(*(const mx_i4 *) (xb + 512 + r32 * 16), *(const mx_i2 *) (xb + 1280 + r32 * 8));
+        }
+    };
+    auto take_x = [&]() {
+        sx = sxn;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            h[j] = hn[j];
+            l[j] = ln[j];
+        }
+    };
+    mx_f16 acc[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
+    auto multiply = [&](const int buf) {
+        const uint32_t sh = sx >> (8 * half), sl = sh - 0x00040004u;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const int sw = (int) (*(const uint32_t *) (s_s[buf] + (32 * t + r32) * 4) >> (8 * half));
+            const mx_i8 a0 = mx_op4(*(const mx_i4 *) (s_w[buf] + (half * ROWS + 32 * t + r32) * 16)), a1 = mx_op4(*(const mx_i4 *) (s_w[buf] + ((2 + half) * ROWS + 32 * t + r32) * 16));
+            acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a0, h[0], acc[t], MX_FP4, MX_FP6, 0, sw, 0, (int) sh);
+            acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a0, l[0], acc[t], MX_FP4, MX_FP6, 0, sw, 0, (int) sl);
+            acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a1, h[1], acc[t], MX_FP4, MX_FP6, 2, sw, 2, (int) sh);
+            acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a1, l[1], acc[t], MX_FP4, MX_FP6, 2, sw, 2, (int) sl);
+        }
+    };
+    fetch_w(0);
+    fetch_x(0);
+    store_w(0);
+    take_x();
+    __syncthreads();
+    for (int step = 0, buf = 0; step < p.steps; ++step, buf ^= 1) {
+        const int next = min(step + 1, p.steps - 1);  // (behind the last step: loads that nobody uses)
+        fetch_w(next);
+        fetch_x(next);
+        __builtin_amdgcn_sched_barrier(0);  // (all of them are on their way before the first product)
+        multiply(buf);
+        __builtin_amdgcn_sched_barrier(0);
+        store_w(buf ^ 1);
+        take_x();
+        __syncthreads();
+    }
+    if (!live) return;
     int64_t c = (int64_t) group * 32 + r32;
     if (ID) c = p.l.list[c];
     if (c < 0 || (!ID && c >= p.cols)) return;
     float * d = p.dst + c * p.ldd;
     const float * bias = p.bias ? (const float *) ((const char *) p.bias + (int64_t) e * p.nb_bias) : nullptr;
+    const bool wide = ((((uintptr_t) d) | (uintptr_t) (p.ldd * 4)) & 15) == 0 && row0 + ROWS <= p.n_rows && !bias;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const int row = row0 + 8 * (i / 4) + 4 * half + i % 4;
-        if (row < p.n_rows) d[row] = bias ? acc[i] + bias[row] : acc[i];
-    }
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = row0 + 32 * t + 8 * i + 4 * half;
+            if (wide) {
+                *(mx_f4 *) (d + row) = mx_f4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]};
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (row + k < p.n_rows) d[row + k] = bias ? acc[t][4 * i + k] + bias[row + k] : acc[t][4 * i + k];
+            }
+        }
 }
-static mx_mm mx_args(const tdesc & w, const tdesc & d, const void * act) {
+static mx_mm mx_args(const tdesc & w, const tdesc & d, int64_t cols) {
     mx_mm p{};
     p.w = (const uint8_t *) w.data;
     p.nb1 = w.nb[1];
     p.nb2 = w.nb[2];
     p.n_rows = (int) w.ne[1];
+    p.n_expert = (int) w.ne[2];
     p.blocks = (int) (w.ne[0] / 32);
-    p.act = (const uint8_t *) act;
     p.steps = (int) mx_steps(w.ne[0]);
     p.dst = (float *) d.data;
     p.ldd = w.ne[1];
+    p.cols = cols;
     return p;
 }
-void launch_mx_mul_mat(hipStream_t s, const tdesc & w, const tdesc & b, const tdesc & d, const void * act) {
-    mx_mm p = mx_args(w, d, act);
-    p.cols = b.ne[1] * b.ne[2] * b.ne[3];
-    if (p.n_rows == 0 || p.cols == 0) return;
-    hipLaunchKernelGGL(k_mx_mm<false>, dim3((unsigned) ((p.n_rows + 127) / 128), (unsigned) ((p.cols + 31) / 32)), dim3(256), 0, s, p);
+// k_mx_vec: workgroups of as many waves as give each the steps it has on the way at once; columns quantised at a time (0: a column does not fit)
+static constexpr size_t MX_VEC_LDS = 64 << 10;
+static int mx_vec_waves(int64_t K) { return (int) std::min<int64_t>(16, std::max<int64_t>(4, (mx_steps(K) + MX_VEC_AHEAD - 1) / MX_VEC_AHEAD)); }
+static size_t mx_vec_lds(int64_t K, int64_t cols) { return (((size_t) cols * (size_t) (mx_steps(K) * 4 * (MX_VEC_REC + 1)) + 15) & ~(size_t) 15) + (size_t) (mx_vec_waves(K) * cols * 16 * 4); }
+static int mx_vec_chunk(int64_t K, int64_t cols) {
+    int64_t c = std::min<int64_t>(16, cols);
+    while (c > 0 && mx_vec_lds(K, c) > MX_VEC_LDS) --c;
+    return (int) c;
 }
-void launch_mx_mul_mat_id(hipStream_t s, const tdesc & w, const tdesc & ids, const tdesc & d, const void * ws, const float * bias, int64_t nb_bias) {
-    const int64_t g = mx_id_groups(w.ne[2], ids.ne[0] * ids.ne[1]);
-    mx_mm p = mx_args(w, d, (const uint8_t *) ws + mx_lists_bytes(g));
-    p.l = mx_lists_at((void *) ws, g);
+static constexpr int64_t MX_VEC_COLS = 4, MX_VEC_ID_COLS = 32, MX_FEW_COLS = 64;
+bool mx_vec_takes(int64_t K, int64_t cols) { return cols <= MX_VEC_COLS && mx_vec_chunk(K, cols) >= cols; }
+bool mx_id_vec_takes(int64_t K, int64_t cols) { return cols <= MX_VEC_ID_COLS && mx_vec_chunk(K, cols) >= 1; }
+
+static void mx_launch_vec(hipStream_t s, const mx_mm & p, const tdesc & b, const tdesc * ids) {
+    const int64_t K = b.ne[0];
+    const int chunk = mx_vec_chunk(K, p.cols);
+    const dim3 block((unsigned) (64 * mx_vec_waves(K)));
+    const unsigned rows = (unsigned) ((p.n_rows + 15) / 16);
+    if (ids) hipLaunchKernelGGL(k_mx_vec<true>, dim3(rows, (unsigned) p.cols), block, mx_vec_lds(K, chunk), s, p, b, *ids, chunk);
+    else hipLaunchKernelGGL(k_mx_vec<false>, dim3(rows), block, mx_vec_lds(K, chunk), s, p, b, b, chunk);
+}
+template <bool ID> static void mx_launch_tile(hipStream_t s, const mx_mm & p, int64_t col_tiles) {
+    auto tiles = [&](int rt) { return (p.n_rows + 32 * rt - 1) / (32 * rt); };
+    const int rt = tiles(8) * col_tiles >= 192 ? 8 : tiles(4) * col_tiles >= 192 ? 4 : 2;
+    const unsigned grid = (unsigned) ((tiles(rt) * col_tiles + 7) / 8 * 8);
+    if (rt == 8) hipLaunchKernelGGL((k_mx_tile<ID, 8>), dim3(grid), dim3(256), 0, s, p, tiles(8));
+    else if (rt == 4) hipLaunchKernelGGL((k_mx_tile<ID, 4>), dim3(grid), dim3(256), 0, s, p, tiles(4));
+    else hipLaunchKernelGGL((k_mx_tile<ID, 2>), dim3(grid), dim3(256), 0, s, p, tiles(2));
+}
+static size_t mx_few_lds(int waves, int ct) { return (size_t) waves * ct * 32 * 36 * 4; }
+// act: null where mx_vec_takes
+void launch_mx_mul_mat(hipStream_t s, const tdesc & w, const tdesc & b, const tdesc & d, const void * act) {
+    mx_mm p = mx_args(w, d, b.ne[1] * b.ne[2] * b.ne[3]);
+    p.act = (const uint8_t *) act;
+    if (p.n_rows == 0 || p.cols == 0) return;
+    const unsigned rows = (unsigned) ((p.n_rows + 31) / 32);
+    if (!act) mx_launch_vec(s, p, b, nullptr);
+    else if (p.cols <= 32) hipLaunchKernelGGL((k_mx_few<false, 1>), dim3(rows, 1), dim3(512), mx_few_lds(8, 1), s, p);
+    else if (p.cols <= MX_FEW_COLS) hipLaunchKernelGGL((k_mx_few<false, 2>), dim3(rows, 1), dim3(256), mx_few_lds(4, 2), s, p);
+    else mx_launch_tile<false>(s, p, (p.cols + 127) / 128);
+}
+void launch_mx_mul_mat_id(hipStream_t s, const tdesc & w, const tdesc & b, const tdesc & ids, const tdesc & d, const void * ws, const float * bias, int64_t nb_bias) {
+    const int64_t cols = ids.ne[0] * ids.ne[1], g = mx_id_groups(w.ne[2], cols);
+    mx_mm p = mx_args(w, d, cols);
     p.bias = bias;
     p.nb_bias = nb_bias;
     if (p.n_rows == 0 || g == 0) return;
-    hipLaunchKernelGGL(k_mx_mm<true>, dim3((unsigned) ((p.n_rows + 127) / 128), (unsigned) g), dim3(256), 0, s, p);
+    if (!ws) return mx_launch_vec(s, p, b, &ids);
+    p.act = (const uint8_t *) ws + mx_lists_bytes(g);
+    p.l = mx_lists_at((void *) ws, g);
+    if (cols <= 32 * w.ne[2]) hipLaunchKernelGGL((k_mx_few<true, 1>), dim3((unsigned) ((p.n_rows + 31) / 32), (unsigned) g), dim3(512), mx_few_lds(8, 1), s, p);
+    else mx_launch_tile<true>(s, p, mx_id_tiles(w.ne[2], cols));
 }
 // which operands the products take (type and shape; the rows of both are dense, whole blocks)
 bool mx_product_ok(const tdesc & w, const tdesc & b) {
