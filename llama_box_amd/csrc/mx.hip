@@ -18,7 +18,7 @@ typedef int mx_i2 __attribute__((ext_vector_type(2)));
 typedef int mx_i8 __attribute__((ext_vector_type(8)));
 typedef float mx_f4 __attribute__((ext_vector_type(4)));
 typedef float mx_f16 __attribute__((ext_vector_type(16)));
-typedef mx_i4 __attribute__((aligned(1))) mx_i4_a1;  // (a block's codes start anywhere)
+typedef mx_i4 __attribute__((aligned(4))) mx_i4_a4;
 typedef uint16_t __attribute__((aligned(1))) mx_u16_a1;
 typedef float mx_f2 __attribute__((ext_vector_type(2)));
 typedef mx_f2 __attribute__((aligned(4))) mx_f2_a4;
@@ -306,12 +306,71 @@ struct mx_mm {
 __device__ __forceinline__ mx_i8 mx_op4(const mx_i4 a) { return mx_i8{a.x, a.y, a.z, a.w, 0, 0, 0, 0}; }
 __device__ __forceinline__ mx_i8 mx_op6(const mx_i4 a, const mx_i2 b) { return mx_i8{a.x, a.y, a.z, a.w, b.x, b.y, 0, 0}; }
 
-// ---- one to a few columns: 16 rows a workgroup, its waves take the steps of 128 values in turn.  The workgroup quantises its columns itself, while its first weights are on the way: a launch in front
-// costs more (see the table of times at the launcher).  A lane of v_mfma_scale_f32_16x16x128: row (column) lane % 16, block lane / 16 of the step.
+// Weights.  A row is a run of 17-byte blocks; a lane takes four blocks (a step's 128 values, 68 bytes) of one row at a time.  Loads at odd addresses cost four times those at whole dwords, so the 68
+// bytes come as 17 dwords and the codes are moved into place (GB/s over rows of 2176 bytes: 16 bytes at 17 b + 1 and a byte at 17 b 2335, the dwords around a block 4750, 17 dwords a lane 6960,
+// aligned 16-byte loads of something else 7500).  A scale byte stays where it is, byte j of its dword: the instruction picks it.
+// DW: rows of whole steps at whole dwords (K a multiple of 128); otherwise block by block, the dwords around each (none of them without a byte of the block).
+struct mx_w4 { mx_i4 a[4]; int s[4]; };  // codes of four blocks; dwords whose byte j is the scale of block j
+template <bool DW> struct mx_raw;
+template <> struct mx_raw<true> {
+    mx_i4 v[4];
+    int d;
+    __device__ __forceinline__ void load(const uint8_t * row, const int step, const int) {
+        const uint8_t * p = row + (int64_t) step * (4 * MX_BLOCK);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = *(const mx_i4_a4 *) (p + 16 * i);
+        d = *(const int *) (p + 64);
+    }
+    __device__ __forceinline__ void place(mx_w4 & w) const {
+        const int q[17] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w, v[2].x, v[2].y, v[2].z, v[2].w, v[3].x, v[3].y, v[3].z, v[3].w, d};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w.a[0][i] = __builtin_amdgcn_alignbyte(q[i + 1], q[i], 1);
+            w.a[1][i] = __builtin_amdgcn_alignbyte(q[i + 5], q[i + 4], 2);
+            w.a[2][i] = __builtin_amdgcn_alignbyte(q[i + 9], q[i + 8], 3);
+            w.a[3][i] = q[i + 13];
+            w.s[i] = q[4 * i];
+        }
+    }
+};
+// a block's codes out of the five dwords around it, sh the first one's bytes in front of the block
+__device__ __forceinline__ mx_i4 mx_window(const mx_i4 v, const int d, const uint32_t sh) {
+    const uint32_t sel = 0x04030201u + 0x01010101u * sh;
+    return mx_i4{(int) __builtin_amdgcn_perm((uint32_t) v.y, (uint32_t) v.x, sel), (int) __builtin_amdgcn_perm((uint32_t) v.z, (uint32_t) v.y, sel),
+                 (int) __builtin_amdgcn_perm((uint32_t) v.w, (uint32_t) v.z, sel), (int) __builtin_amdgcn_perm((uint32_t) d, (uint32_t) v.w, sel)};
+}
+template <> struct mx_raw<false> {
+    mx_i4 v[4];
+    int d[4];
+    uint32_t sh[4];
+    __device__ __forceinline__ void load(const uint8_t * row, const int step, const int blocks) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uintptr_t p = (uintptr_t) row + (uintptr_t) (min(step * 4 + j, blocks - 1) * MX_BLOCK);
+            const uint8_t * q = (const uint8_t *) (p & ~(uintptr_t) 3);
+            sh[j] = (uint32_t) p & 3u;
+            v[j] = *(const mx_i4_a4 *) q;
+            d[j] = *(const int *) (q + 16);
+        }
+    }
+    __device__ __forceinline__ void place(mx_w4 & w) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            w.a[j] = mx_window(v[j], d[j], sh[j]);
+            w.s[j] = (int) ((((uint32_t) v[j].x >> (8 * sh[j])) & 255u) << (8 * j));
+        }
+    }
+};
+// acc += one block: w's block J by the digits h, l, whose scale bytes are byte J of sh, sl
+#define MX_MFMA(N, ACC, W, J, H, L, SH, SL)                                                                                                         \
+    ACC = __builtin_amdgcn_mfma_scale_f32_##N##_f8f6f4(mx_op4((W).a[J]), H, ACC, MX_FP4, MX_FP6, J, (W).s[J], J, (int) (SH));                     \
+    ACC = __builtin_amdgcn_mfma_scale_f32_##N##_f8f6f4(mx_op4((W).a[J]), L, ACC, MX_FP4, MX_FP6, J, (W).s[J], J, (int) (SL));
+
+// ---- one to a few columns: 16 rows a workgroup, its waves take four steps of 128 values in turn.  The workgroup quantises its columns itself, while its first weights are on the way: a launch in front
+// costs more.  A lane of v_mfma_scale_f32_16x16x128: row (column) lane % 16, step lane / 16 of the four.
 // ID: blockIdx.y is a column (u + n_used t) of at most 64; the first column of an expert takes all of its expert, the others' workgroups end at once.
-static constexpr int MX_VEC_AHEAD = 8;    // steps whose weights a wave has on the way
 static constexpr int MX_VEC_REC = 48;     // LDS bytes of a block of one column: 16 of h, 16 of l, 8 of h, 8 of l
-template <bool ID> __global__ void __launch_bounds__(1024) k_mx_vec(const mx_mm p, const tdesc b, const tdesc ids, const int chunk) {
+template <bool ID, bool DW> __global__ void __launch_bounds__(512) k_mx_vec(const mx_mm p, const tdesc b, const tdesc ids, const int chunk) {
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ int s_cols[64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, r16 = lane & 15, q = lane >> 4;
@@ -328,70 +387,81 @@ template <bool ID> __global__ void __launch_bounds__(1024) k_mx_vec(const mx_mm 
         if (wave == 0 && id == e) s_cols[__popcll(mine & ((1ull << lane) - 1ull))] = lane;
     }
     const uint8_t * w = p.w + (int64_t) e * p.nb2 + (int64_t) min(row0 + r16, p.n_rows - 1) * p.nb1;
-    uint8_t * s_rec = lds, * s_scale = lds + (size_t) chunk * blocks4 * MX_VEC_REC;  // [block][column of the chunk]
-    float * s_part = (float *) (lds + (((size_t) chunk * blocks4 * (MX_VEC_REC + 1) + 15) & ~(size_t) 15));  // [wave][column][row]
+    uint8_t * s_rec = lds, * s_scale = lds + (size_t) chunk * blocks4 * MX_VEC_REC;  // [block][column of the chunk]; [step][column][block] scale bytes
+    float * s_part = (float *) (lds + (size_t) chunk * blocks4 * (MX_VEC_REC + 1));  // [wave][column][row]
     const float * bias = p.bias ? (const float *) ((const char *) p.bias + (int64_t) e * p.nb_bias) : nullptr;
     for (int c0 = 0; c0 < n; c0 += chunk) {
         const int m = min(chunk, n - c0);
-        mx_i4 a[MX_VEC_AHEAD];
-        int sa[MX_VEC_AHEAD];
-        auto fetch = [&](const int s0) {
-#pragma unroll
-            for (int u = 0; u < MX_VEC_AHEAD; ++u) {
-                const uint8_t * wb = w + min((s0 + u * waves) * 4 + q, p.blocks - 1) * MX_BLOCK;
-                a[u] = *(const mx_i4_a1 *) (wb + 1);
-                sa[u] = wb[0];
-            }
-        };
-        fetch(wave);
+        mx_raw<DW> f0, f1;
+        const int last = p.steps - 1, stride = 4 * waves;
+        int step = wave * 4 + q;  // (behind the last step: its weights again, and digits of zero)
+        f0.load(w, min(step, last), p.blocks);
+        f1.load(w, min(step + stride, last), p.blocks);
         if (ID || c0) __syncthreads();  // (the columns' list; the last chunk's partial sums and digits are read)
-        for (int at = threadIdx.x; at < 8 * blocks4 * m; at += blockDim.x) {  // eight lanes a block (blocks4 is a multiple of four: whole half-waves)
-            const int i = at & 7, c = (at >> 3) / blocks4, blk = (at >> 3) - c * blocks4;
+        const int i = threadIdx.x & 7, per = (int) blockDim.x >> 3;  // eight lanes a block
+        for (int c = 0; c < m; ++c) {
             const char * col;
             if (ID) {
                 const int cc = s_cols[c0 + c], n_used = (int) ids.ne[0];
-                col = b.data + ((cc % n_used) % b.ne[1]) * b.nb[1] + (int64_t) (cc / n_used) * b.nb[2];
+                col = b.data + ((cc % n_used) % (int) b.ne[1]) * b.nb[1] + (int64_t) (cc / n_used) * b.nb[2];
             } else {
                 const int cc = c0 + c, n1 = (int) b.ne[1], n2 = (int) b.ne[2];
                 col = b.data + (cc % n1) * b.nb[1] + (int64_t) ((cc / n1) % n2) * b.nb[2] + (int64_t) (cc / (n1 * n2)) * b.nb[3];
             }
-            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (blk < p.blocks) mx_load4((const float *) col + blk * 32, i, v);
-            uint32_t h, l;
-            const uint32_t se = mx_act4(v, h, l);
-            uint8_t * rec = s_rec + ((size_t) blk * chunk + c) * MX_VEC_REC;
-            // (24 bits a lane: three bytes of h's 24, three of l's)
+            for (int blk0 = threadIdx.x >> 3; blk0 < blocks4; blk0 += 4 * per) {
+                float v[4][4];
 #pragma unroll
-            for (int k = 0; k < 3; ++k) {
-                const int o = 3 * i + k;
-                rec[o < 16 ? o : o + 16] = (uint8_t) (h >> (8 * k));
-                rec[o < 16 ? o + 16 : o + 24] = (uint8_t) (l >> (8 * k));
+                for (int k = 0; k < 4; ++k) mx_load4((const float *) col + min(blk0 + k * per, p.blocks - 1) * 32, i, v[k]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int blk = blk0 + k * per;
+                    if (blk >= blocks4) break;
+                    uint32_t h, l, se = mx_act4(v[k], h, l);
+                    if (blk >= p.blocks) {
+                        h = l = 0;
+                        se = 127;
+                    }
+                    uint8_t * rec = s_rec + ((size_t) blk * chunk + c) * MX_VEC_REC;
+                    // (24 bits a lane: three bytes of h's 24, three of l's)
+#pragma unroll
+                    for (int t = 0; t < 3; ++t) {
+                        const int o = 3 * i + t;
+                        rec[o < 16 ? o : o + 16] = (uint8_t) (h >> (8 * t));
+                        rec[o < 16 ? o + 16 : o + 24] = (uint8_t) (l >> (8 * t));
+                    }
+                    if (i == 0) s_scale[((blk >> 2) * chunk + c) * 4 + (blk & 3)] = (uint8_t) se;
+                }
             }
-            if (i == 0) s_scale[blk * chunk + c] = (uint8_t) se;
         }
         __syncthreads();
         mx_f4 acc = {0, 0, 0, 0};
-        for (int s0 = wave; s0 < p.steps; s0 += MX_VEC_AHEAD * waves) {
-            if (s0 != wave) fetch(s0);
+        auto add = [&](const int st, const mx_raw<DW> & f) {
+            mx_w4 wt;
+            f.place(wt);
+            mx_i8 h[4], l[4];
+            uint32_t sx = 0x7F7F7F7Fu;
 #pragma unroll
-            for (int u = 0; u < MX_VEC_AHEAD; ++u) {
-                const int step = s0 + u * waves;
-                if (step >= p.steps) break;
-                mx_i4 h = {0, 0, 0, 0}, l = {0, 0, 0, 0};
-                mx_i2 h2 = {0, 0}, l2 = {0, 0};
-                int sh = 127;
-                if (r16 < m) {
-                    const int at = (step * 4 + q) * chunk + r16;
-                    const uint8_t * rec = s_rec + (size_t) at * MX_VEC_REC;
-                    h = *(const mx_i4 *) rec;
-                    l = *(const mx_i4 *) (rec + 16);
-                    h2 = *(const mx_i2 *) (rec + 32);
-                    l2 = *(const mx_i2 *) (rec + 40);
-                    sh = s_scale[at];
+            for (int j = 0; j < 4; ++j) h[j] = l[j] = mx_i8{0, 0, 0, 0, 0, 0, 0, 0};
+            if (r16 < m && st <= last) {
+                sx = *(const uint32_t *) (s_scale + (st * chunk + r16) * 4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint8_t * rec = s_rec + ((size_t) (st * 4 + j) * chunk + r16) * MX_VEC_REC;
+                    h[j] = mx_op6(*(const mx_i4 *) rec, *(const mx_i2 *) (rec + 32));
+                    l[j] = mx_op6(*(const mx_i4 *) (rec + 16), *(const mx_i2 *) (rec + 40));
                 }
-                acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_op4(a[u]), mx_op6(h, h2), acc, MX_FP4, MX_FP6, 0, sa[u], 0, sh);
-                acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_op4(a[u]), mx_op6(l, l2), acc, MX_FP4, MX_FP6, 0, sa[u], 0, sh - 4);
             }
+            const uint32_t sl = sx - 0x04040404u;
+            MX_MFMA(16x16x128, acc, wt, 0, h[0], l[0], sx, sl)
+            MX_MFMA(16x16x128, acc, wt, 1, h[1], l[1], sx, sl)
+            MX_MFMA(16x16x128, acc, wt, 2, h[2], l[2], sx, sl)
+            MX_MFMA(16x16x128, acc, wt, 3, h[3], l[3], sx, sl)
+        };
+        for (int s0 = wave * 4; s0 < p.steps; s0 += 2 * stride, step += 2 * stride) {  // (s0: the wave's, for all its lanes)
+            add(step, f0);
+            f0.load(w, min(step + 2 * stride, last), p.blocks);
+            if (s0 + stride < p.steps) add(step + stride, f1);
+            f1.load(w, min(step + 3 * stride, last), p.blocks);
         }
         if (r16 < m) *(mx_f4 *) (s_part + ((wave * chunk + r16) * 16 + 4 * q)) = acc;
         __syncthreads();
@@ -404,8 +474,8 @@ template <bool ID> __global__ void __launch_bounds__(1024) k_mx_vec(const mx_mm 
     }
 }
 
-// ---- up to a few groups of columns: 32 rows by CT groups a workgroup, its waves take the steps in turn, everything straight from memory; the waves' sums are added in LDS in their order
-template <bool ID, int CT> __global__ void __launch_bounds__(512) k_mx_few(const mx_mm p) {
+// ---- up to a few groups of columns: 32 rows by CT groups a workgroup, its waves take two steps in turn, everything straight from memory; the waves' sums are added in LDS in their order
+template <bool ID, int CT, bool DW> __global__ void __launch_bounds__(512) k_mx_few(const mx_mm p) {
     extern __shared__ __align__(16) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, r32 = lane & 31, half = lane >> 5;
     const int group0 = blockIdx.y * CT, row0 = (int) blockIdx.x * 32;
@@ -417,66 +487,53 @@ template <bool ID, int CT> __global__ void __launch_bounds__(512) k_mx_few(const
     const uint8_t * w = p.w + (int64_t) e * p.nb2 + (int64_t) min(row0 + r32, p.n_rows - 1) * p.nb1;
     const uint8_t * x = p.act + (int64_t) group0 * p.steps * MX_ACT_STEP;
     const int64_t group_bytes = (int64_t) p.steps * MX_ACT_STEP;
-    int64_t col[CT];  // the lane's columns, -1: none
+    bool live[CT];  // the lane's columns
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
-        col[c] = (int64_t) (group0 + c) * 32 + r32;
-        if (ID) col[c] = p.l.list[col[c]];
-        else if (col[c] >= p.cols) col[c] = -1;
-    }
+    for (int c = 0; c < CT; ++c) live[c] = ID ? p.l.list[(group0 + c) * 32 + r32] >= 0 : (int64_t) (group0 + c) * 32 + r32 < p.cols;
     mx_f16 acc[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
-    struct part { mx_i4 a[2]; int sa[2]; mx_i4 h[CT][2], l[CT][2]; mx_i2 h2[CT][2], l2[CT][2]; uint32_t sx[CT]; };
-    auto fetch = [&](const int step, part & f) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const uint8_t * wb = w + min(step * 4 + 2 * j + half, p.blocks - 1) * MX_BLOCK;
-            f.a[j] = *(const mx_i4_a1 *) (wb + 1);
-            f.sa[j] = wb[0];
-        }
+    const int last = p.steps - 1;
+    mx_raw<DW> f;
+    mx_i8 h[CT][4], l[CT][4];
+    uint32_t sx[CT];
+    auto fetch_x = [&](const int step) {
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
-            f.sx[c] = 0x7F7F7F7Fu;
+            sx[c] = 0x7F7F7F7Fu;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                f.h[c][j] = f.l[c][j] = mx_i4{0, 0, 0, 0};
-                f.h2[c][j] = f.l2[c][j] = mx_i2{0, 0};
-            }
-            if (col[c] >= 0) {
+            for (int j = 0; j < 4; ++j) h[c][j] = l[c][j] = mx_i8{0, 0, 0, 0, 0, 0, 0, 0};
+            if (live[c] && step <= last) {
                 const uint8_t * xs = x + c * group_bytes + (int64_t) step * MX_ACT_STEP;
-                f.sx[c] = *(const uint32_t *) (xs + 4 * MX_ACT_BLK + r32 * 4);
+                sx[c] = *(const uint32_t *) (xs + 4 * MX_ACT_BLK + r32 * 4);
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const uint8_t * xb = xs + (2 * j + half) * MX_ACT_BLK;
-                    f.h[c][j] = *(const mx_i4 *) (xb + r32 * 16);
-                    f.l[c][j] = *(const mx_i4 *) (xb + 512 + r32 * 16);
-                    f.h2[c][j] = *(const mx_i2 *) (xb + 1024 + r32 * 8);
-                    f.l2[c][j] = *(const mx_i2 *) (xb + 1280 + r32 * 8);
+                for (int j = 0; j < 4; ++j) {
+                    const uint8_t * xb = xs + j * MX_ACT_BLK;
+                    h[c][j] = mx_op6(*(const mx_i4 *) (xb + r32 * 16), *(const mx_i2 *) (xb + 1024 + r32 * 8));
+                    l[c][j] = mx_op6(*(const mx_i4 *) (xb + 512 + r32 * 16), *(const mx_i2 *) (xb + 1280 + r32 * 8));
                 }
             }
         }
     };
-    auto add = [&](const part & f) {
+    int step = wave * 2 + half;
+    f.load(w, min(step, last), p.blocks);
+    fetch_x(step);
+    for (int s0 = wave * 2; s0 < p.steps; s0 += 2 * waves) {  // (s0: the wave's, for both halves)
+        mx_w4 wt;
+        f.place(wt);
+        step += 2 * waves;
+        f.load(w, min(step, last), p.blocks);
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int sh = (int) ((f.sx[c] >> (16 * j + 8 * half)) & 255u);
-                acc[c] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_op4(f.a[j]), mx_op6(f.h[c][j], f.h2[c][j]), acc[c], MX_FP4, MX_FP6, 0, f.sa[j], 0, sh);
-                acc[c] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_op4(f.a[j]), mx_op6(f.l[c][j], f.l2[c][j]), acc[c], MX_FP4, MX_FP6, 0, f.sa[j], 0, sh - 4);
-            }
-    };
-    part f0, f1;
-    int step = wave;
-    if (step < p.steps) fetch(step, f0);
-    for (; step < p.steps; step += 2 * waves) {
-        if (step + waves < p.steps) fetch(step + waves, f1);
-        add(f0);
-        if (step + 2 * waves < p.steps) fetch(step + 2 * waves, f0);
-        if (step + waves < p.steps) add(f1);
+        for (int c = 0; c < CT; ++c) {
+            const uint32_t sl = sx[c] - 0x04040404u;
+            MX_MFMA(32x32x64, acc[c], wt, 0, h[c][0], l[c][0], sx[c], sl)
+            MX_MFMA(32x32x64, acc[c], wt, 1, h[c][1], l[c][1], sx[c], sl)
+            MX_MFMA(32x32x64, acc[c], wt, 2, h[c][2], l[c][2], sx[c], sl)
+            MX_MFMA(32x32x64, acc[c], wt, 3, h[c][3], l[c][3], sx[c], sl)
+        }
+        fetch_x(step);
     }
     // [wave][group][column][row], the rows of a column 36 apart (of 32: no two quarters of a wave on the same banks)
     float * part_sums = (float *) lds;
@@ -500,9 +557,9 @@ template <bool ID, int CT> __global__ void __launch_bounds__(512) k_mx_few(const
 
 // ---- many columns: 32 RT rows by four groups of columns a workgroup.  A wave has one group and all rows: its digits come straight from memory (no other wave reads them), the weights through LDS,
 // where their blocks are aligned ([block of the step][row] 16 bytes, and 4 scale bytes a row).  While a step is multiplied, the next one's weights and digits are on the way to registers.
-template <bool ID, int RT> __global__ void __launch_bounds__(256, 2) k_mx_tile(const mx_mm p, const int row_tiles) {
-    constexpr int ROWS = 32 * RT;
-    __shared__ __align__(16) uint8_t s_w[2][4 * ROWS * 16];
+template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, 2) k_mx_tile(const mx_mm p, const int row_tiles) {
+    constexpr int ROWS = 32 * RT, PLANE = ROWS * 16 + 64;  // (64: the four planes that a quad of lanes writes to lie on different banks)
+    __shared__ __align__(16) uint8_t s_w[2][4 * PLANE];
     __shared__ __align__(16) uint8_t s_s[2][ROWS * 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r32 = lane & 31, half = lane >> 5;
     int rt, tile;
@@ -526,26 +583,37 @@ template <bool ID, int RT> __global__ void __launch_bounds__(256, 2) k_mx_tile(c
         groups = t[1] + t[2];
     }
     const bool live = group < groups;
-    // loads: four lanes a row
-    const int lblk = tid & 3, lrow = tid >> 2;
+    // loads: four lanes a row, its 68 bytes of a step as 64 in a row and one dword; lane q's block starts at byte q of its first dword
+    const int q = tid & 3, lrow = tid >> 2;
     const uint8_t * wl[RT / 2];
 #pragma unroll
     for (int i = 0; i < RT / 2; ++i) wl[i] = p.w + (int64_t) e * p.nb2 + (int64_t) min(row0 + lrow + 64 * i, p.n_rows - 1) * p.nb1;
     mx_i4 wr[RT / 2];
-    uint8_t ws[RT / 2];
+    int wd[RT / 2];
+    uint32_t wsh[RT / 2];
     auto fetch_w = [&](const int step) {
-        const int at = min(step * 4 + lblk, p.blocks - 1) * MX_BLOCK;
 #pragma unroll
         for (int i = 0; i < RT / 2; ++i) {
-            wr[i] = *(const mx_i4_a1 *) (wl[i] + at + 1);
-            ws[i] = wl[i][at];
+            if (DW) {
+                const uint8_t * a = wl[i] + (int64_t) step * (4 * MX_BLOCK);
+                wr[i] = *(const mx_i4_a4 *) (a + 16 * q);
+                wd[i] = *(const int *) (a + 64);
+            } else {
+                const uintptr_t a = (uintptr_t) wl[i] + (uintptr_t) (min(step * 4 + q, p.blocks - 1) * MX_BLOCK);
+                wsh[i] = (uint32_t) a & 3u;
+                wr[i] = *(const mx_i4_a4 *) (a & ~(uintptr_t) 3);
+                wd[i] = *(const int *) ((a & ~(uintptr_t) 3) + 16);
+            }
         }
     };
     auto store_w = [&](const int buf) {
 #pragma unroll
         for (int i = 0; i < RT / 2; ++i) {
-            *(mx_i4 *) (s_w[buf] + ((lblk * ROWS) + lrow + 64 * i) * 16) = wr[i];
-            s_s[buf][(lrow + 64 * i) * 4 + lblk] = ws[i];
+            const uint32_t sh = DW ? (uint32_t) q : wsh[i];
+            const int next = __builtin_amdgcn_update_dpp(0, wr[i].x, 0xF9, 0xF, 0xF, true);  // (the first dword of the quad's next lane: quad_perm 1, 2, 3, 3)
+            const int d = !DW || q == 3 ? wd[i] : next;
+            *(mx_i4 *) (s_w[buf] + q * PLANE + (lrow + 64 * i) * 16) = mx_window(wr[i], d, sh);
+            s_s[buf][(lrow + 64 * i) * 4 + q] = (uint8_t) ((uint32_t) wr[i].x >> (8 * sh));
         }
     };
     const uint8_t * x = p.act + (int64_t) (live ? group : groups - 1) * p.steps * MX_ACT_STEP;
@@ -576,14 +644,16 @@ template <bool ID, int RT> __global__ void __launch_bounds__(256, 2) k_mx_tile(c
         for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
     auto multiply = [&](const int buf) {
         const uint32_t sh = sx >> (8 * half), sl = sh - 0x00040004u;
+        int sw[RT];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) sw[t] = (int) (*(const uint32_t *) (s_s[buf] + (32 * t + r32) * 4) >> (8 * half));
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            const int sw = (int) (*(const uint32_t *) (s_s[buf] + (32 * t + r32) * 4) >> (8 * half));
-            const mx_i8 a0 = mx_op4(*(const mx_i4 *) (s_w[buf] + (half * ROWS + 32 * t + r32) * 16)), a1 = mx_op4(*(const mx_i4 *) (s_w[buf] + ((2 + half) * ROWS + 32 * t + r32) * 16));
-            acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a0, h[0], acc[t], MX_FP4, MX_FP6, 0, sw, 0, (int) sh);
-            acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a0, l[0], acc[t], MX_FP4, MX_FP6, 0, sw, 0, (int) sl);
-            acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a1, h[1], acc[t], MX_FP4, MX_FP6, 2, sw, 2, (int) sh);
-            acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a1, l[1], acc[t], MX_FP4, MX_FP6, 2, sw, 2, (int) sl);
+            const mx_i8 a0 = mx_op4(*(const mx_i4 *) (s_w[buf] + half * PLANE + (32 * t + r32) * 16)), a1 = mx_op4(*(const mx_i4 *) (s_w[buf] + (2 + half) * PLANE + (32 * t + r32) * 16));
+            acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a0, h[0], acc[t], MX_FP4, MX_FP6, 0, sw[t], 0, (int) sh);
+            acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a0, l[0], acc[t], MX_FP4, MX_FP6, 0, sw[t], 0, (int) sl);
+            acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a1, h[1], acc[t], MX_FP4, MX_FP6, 2, sw[t], 2, (int) sh);
+            acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a1, l[1], acc[t], MX_FP4, MX_FP6, 2, sw[t], 2, (int) sl);
         }
     };
     fetch_w(0);
@@ -637,10 +707,10 @@ static mx_mm mx_args(const tdesc & w, const tdesc & d, int64_t cols) {
     p.cols = cols;
     return p;
 }
-// k_mx_vec: workgroups of as many waves as give each the steps it has on the way at once; columns quantised at a time (0: a column does not fit)
+// k_mx_vec: a wave has two times four steps on the way; columns quantised at a time (0: a column does not fit)
 static constexpr size_t MX_VEC_LDS = 64 << 10;
-static int mx_vec_waves(int64_t K) { return (int) std::min<int64_t>(16, std::max<int64_t>(4, (mx_steps(K) + MX_VEC_AHEAD - 1) / MX_VEC_AHEAD)); }
-static size_t mx_vec_lds(int64_t K, int64_t cols) { return (((size_t) cols * (size_t) (mx_steps(K) * 4 * (MX_VEC_REC + 1)) + 15) & ~(size_t) 15) + (size_t) (mx_vec_waves(K) * cols * 16 * 4); }
+static int mx_vec_waves(int64_t K) { return (int) std::min<int64_t>(8, std::max<int64_t>(4, (mx_steps(K) + 7) / 8)); }
+static size_t mx_vec_lds(int64_t K, int64_t cols) { return (size_t) cols * (size_t) (mx_steps(K) * 4 * (MX_VEC_REC + 1)) + (size_t) (mx_vec_waves(K) * cols * 16 * 4); }
 static int mx_vec_chunk(int64_t K, int64_t cols) {
     int64_t c = std::min<int64_t>(16, cols);
     while (c > 0 && mx_vec_lds(K, c) > MX_VEC_LDS) --c;
@@ -649,33 +719,44 @@ static int mx_vec_chunk(int64_t K, int64_t cols) {
 static constexpr int64_t MX_VEC_COLS = 4, MX_VEC_ID_COLS = 32, MX_FEW_COLS = 64;
 bool mx_vec_takes(int64_t K, int64_t cols) { return cols <= MX_VEC_COLS && mx_vec_chunk(K, cols) >= cols; }
 bool mx_id_vec_takes(int64_t K, int64_t cols) { return cols <= MX_VEC_ID_COLS && mx_vec_chunk(K, cols) >= 1; }
-
+// rows of whole steps, every one at a whole dword
+static bool mx_dwords(const mx_mm & p) { return p.blocks % 4 == 0 && p.nb1 % 4 == 0 && p.nb2 % 4 == 0 && ((uintptr_t) p.w & 3) == 0; }
 static void mx_launch_vec(hipStream_t s, const mx_mm & p, const tdesc & b, const tdesc * ids) {
     const int64_t K = b.ne[0];
     const int chunk = mx_vec_chunk(K, p.cols);
     const dim3 block((unsigned) (64 * mx_vec_waves(K)));
     const unsigned rows = (unsigned) ((p.n_rows + 15) / 16);
-    if (ids) hipLaunchKernelGGL(k_mx_vec<true>, dim3(rows, (unsigned) p.cols), block, mx_vec_lds(K, chunk), s, p, b, *ids, chunk);
-    else hipLaunchKernelGGL(k_mx_vec<false>, dim3(rows), block, mx_vec_lds(K, chunk), s, p, b, b, chunk);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(rows, ids ? (unsigned) p.cols : 1u), block, mx_vec_lds(K, chunk), s, p, b, ids ? *ids : b, chunk); };
+    const bool dw = mx_dwords(p);
+    if (ids) dw ? go(k_mx_vec<true, true>) : go(k_mx_vec<true, false>);
+    else dw ? go(k_mx_vec<false, true>) : go(k_mx_vec<false, false>);
+}
+template <bool ID, int RT> static void mx_launch_tile_of(hipStream_t s, const mx_mm & p, int64_t col_tiles) {
+    const int row_tiles = (p.n_rows + 32 * RT - 1) / (32 * RT);
+    const dim3 grid((unsigned) ((row_tiles * col_tiles + 7) / 8 * 8));
+    if (mx_dwords(p)) hipLaunchKernelGGL((k_mx_tile<ID, RT, true>), grid, dim3(256), 0, s, p, row_tiles);
+    else hipLaunchKernelGGL((k_mx_tile<ID, RT, false>), grid, dim3(256), 0, s, p, row_tiles);
 }
 template <bool ID> static void mx_launch_tile(hipStream_t s, const mx_mm & p, int64_t col_tiles) {
-    auto tiles = [&](int rt) { return (p.n_rows + 32 * rt - 1) / (32 * rt); };
-    const int rt = tiles(8) * col_tiles >= 192 ? 8 : tiles(4) * col_tiles >= 192 ? 4 : 2;
-    const unsigned grid = (unsigned) ((tiles(rt) * col_tiles + 7) / 8 * 8);
-    if (rt == 8) hipLaunchKernelGGL((k_mx_tile<ID, 8>), dim3(grid), dim3(256), 0, s, p, tiles(8));
-    else if (rt == 4) hipLaunchKernelGGL((k_mx_tile<ID, 4>), dim3(grid), dim3(256), 0, s, p, tiles(4));
-    else hipLaunchKernelGGL((k_mx_tile<ID, 2>), dim3(grid), dim3(256), 0, s, p, tiles(2));
+    auto wide = [&](int rt) { return (p.n_rows + 32 * rt - 1) / (32 * rt) * col_tiles >= 192; };
+    if (wide(8)) mx_launch_tile_of<ID, 8>(s, p, col_tiles);
+    else if (wide(4)) mx_launch_tile_of<ID, 4>(s, p, col_tiles);
+    else mx_launch_tile_of<ID, 2>(s, p, col_tiles);
 }
-static size_t mx_few_lds(int waves, int ct) { return (size_t) waves * ct * 32 * 36 * 4; }
+template <bool ID, int CT> static void mx_launch_few(hipStream_t s, const mx_mm & p, int64_t groups, int waves) {
+    const dim3 grid((unsigned) ((p.n_rows + 31) / 32), (unsigned) groups), block((unsigned) (64 * waves));
+    const size_t lds = (size_t) waves * CT * 32 * 36 * 4;
+    if (mx_dwords(p)) hipLaunchKernelGGL((k_mx_few<ID, CT, true>), grid, block, lds, s, p);
+    else hipLaunchKernelGGL((k_mx_few<ID, CT, false>), grid, block, lds, s, p);
+}
 // act: null where mx_vec_takes
 void launch_mx_mul_mat(hipStream_t s, const tdesc & w, const tdesc & b, const tdesc & d, const void * act) {
     mx_mm p = mx_args(w, d, b.ne[1] * b.ne[2] * b.ne[3]);
     p.act = (const uint8_t *) act;
     if (p.n_rows == 0 || p.cols == 0) return;
-    const unsigned rows = (unsigned) ((p.n_rows + 31) / 32);
     if (!act) mx_launch_vec(s, p, b, nullptr);
-    else if (p.cols <= 32) hipLaunchKernelGGL((k_mx_few<false, 1>), dim3(rows, 1), dim3(512), mx_few_lds(8, 1), s, p);
-    else if (p.cols <= MX_FEW_COLS) hipLaunchKernelGGL((k_mx_few<false, 2>), dim3(rows, 1), dim3(256), mx_few_lds(4, 2), s, p);
+    else if (p.cols <= 32) mx_launch_few<false, 1>(s, p, 1, 8);
+    else if (p.cols <= MX_FEW_COLS) mx_launch_few<false, 2>(s, p, 1, 4);
     else mx_launch_tile<false>(s, p, (p.cols + 127) / 128);
 }
 void launch_mx_mul_mat_id(hipStream_t s, const tdesc & w, const tdesc & b, const tdesc & ids, const tdesc & d, const void * ws, const float * bias, int64_t nb_bias) {
@@ -687,7 +768,7 @@ void launch_mx_mul_mat_id(hipStream_t s, const tdesc & w, const tdesc & b, const
     if (!ws) return mx_launch_vec(s, p, b, &ids);
     p.act = (const uint8_t *) ws + mx_lists_bytes(g);
     p.l = mx_lists_at((void *) ws, g);
-    if (cols <= 32 * w.ne[2]) hipLaunchKernelGGL((k_mx_few<true, 1>), dim3((unsigned) ((p.n_rows + 31) / 32), (unsigned) g), dim3(512), mx_few_lds(8, 1), s, p);
+    if (cols <= 32 * w.ne[2]) mx_launch_few<true, 1>(s, p, g, 8);
     else mx_launch_tile<true>(s, p, mx_id_tiles(w.ne[2], cols));
 }
 // which operands the products take (type and shape; the rows of both are dense, whole blocks)
