@@ -294,7 +294,7 @@ struct mx_mm {
     int64_t nb1, nb2;     // bytes between rows, between experts
     int n_rows, blocks;   // rows of the (an expert's) matrix; blocks of a row
     const uint8_t * act;
-    int steps;
+    int steps;            // of 128 values
     int64_t cols;         // columns of the product
     int n_expert;
     float * dst;          // column c at dst + c ldd
@@ -555,13 +555,39 @@ template <bool ID, int CT, bool DW> __global__ void __launch_bounds__(512) k_mx_
     }
 }
 
+// a wave's 32 RT rows by 32 columns to their places
+template <bool ID, int RT> __device__ __forceinline__ void mx_store_tile(const mx_mm & p, const mx_f16 (&acc)[RT], const int group, const int row0, const int e, const int r32, const int half) {
+    constexpr int ROWS = 32 * RT;
+    int64_t c = (int64_t) group * 32 + r32;
+    if (ID) c = p.l.list[c];
+    if (c < 0 || (!ID && c >= p.cols)) return;
+    float * d = p.dst + c * p.ldd;
+    const float * bias = p.bias ? (const float *) ((const char *) p.bias + (int64_t) e * p.nb_bias) : nullptr;
+    const bool wide = ((((uintptr_t) d) | (uintptr_t) (p.ldd * 4)) & 15) == 0 && row0 + ROWS <= p.n_rows && !bias;
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = row0 + 32 * t + 8 * i + 4 * half;
+            if (wide) {
+                *(mx_f4 *) (d + row) = mx_f4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]};
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (row + k < p.n_rows) d[row + k] = bias ? acc[t][4 * i + k] + bias[row + k] : acc[t][4 * i + k];
+            }
+        }
+}
 // ---- many columns: 32 RT rows by four groups of columns a workgroup.  A wave has one group and all rows: its digits come straight from memory (no other wave reads them), the weights through LDS,
-// where their blocks are aligned ([block of the step][row] 16 bytes, and 4 scale bytes a row).  While a step is multiplied, the next one's weights and digits are on the way to registers.
-template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, 2) k_mx_tile(const mx_mm p, const int row_tiles) {
+// where their blocks are aligned ([block of the step][row] 16 bytes, and 4 scale bytes a row).  In a step of 128 values: the next step's digits are requested, the next step's weights (requested a step
+// ago) stored, the weights after those requested — one such item behind each product.  (Requested in a bunch in front of the products they hold up all four waves at once: 512 columns 62 us.)
+#define MX_MFMA1(A, B, C, BYTE, SA, SB) __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, C, MX_FP4, MX_FP6, BYTE, SA, BYTE, (int) (SB))
+template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, RT == 8 ? 1 : 2) k_mx_tile(const mx_mm p, const int row_tiles) {
+    constexpr int SET = RT < 4 ? RT : 4, SETS = RT / SET;
     constexpr int ROWS = 32 * RT, PLANE = ROWS * 16 + 64;  // (64: the four planes that a quad of lanes writes to lie on different banks)
     __shared__ __align__(16) uint8_t s_w[2][4 * PLANE];
     __shared__ __align__(16) uint8_t s_s[2][ROWS * 4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r32 = lane & 31, half = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r32 = lane & 31, half = lane >> 5;
     int rt, tile;
     if (ID) {
         rt = blockIdx.x % row_tiles;
@@ -583,58 +609,59 @@ template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, 2) k_
         groups = t[1] + t[2];
     }
     const bool live = group < groups;
-    // loads: four lanes a row, its 68 bytes of a step as 64 in a row and one dword; lane q's block starts at byte q of its first dword
+    // weights: four lanes a row, its 68 bytes of a step as 64 in a row and one dword; lane q's block starts at byte q of its first dword
     const int q = tid & 3, lrow = tid >> 2;
-    const uint8_t * wl[RT / 2];
+    const uint8_t * w0 = p.w + (int64_t) e * p.nb2 + (int64_t) row0 * p.nb1;
+    const uint32_t odd = DW ? 0u : (uint32_t) (uintptr_t) w0 & 3u;
+    w0 -= odd;
+    uint32_t wl[RT / 2];
 #pragma unroll
-    for (int i = 0; i < RT / 2; ++i) wl[i] = p.w + (int64_t) e * p.nb2 + (int64_t) min(row0 + lrow + 64 * i, p.n_rows - 1) * p.nb1;
+    for (int i = 0; i < RT / 2; ++i) wl[i] = (uint32_t) (min(row0 + lrow + 64 * i, p.n_rows - 1) - row0) * (uint32_t) p.nb1 + (DW ? 16u * q : odd);
     mx_i4 wr[RT / 2];
     int wd[RT / 2];
     uint32_t wsh[RT / 2];
-    auto fetch_w = [&](const int step) {
-#pragma unroll
-        for (int i = 0; i < RT / 2; ++i) {
-            if (DW) {
-                const uint8_t * a = wl[i] + (int64_t) step * (4 * MX_BLOCK);
-                wr[i] = *(const mx_i4_a4 *) (a + 16 * q);
-                wd[i] = *(const int *) (a + 64);
-            } else {
-                const uintptr_t a = (uintptr_t) wl[i] + (uintptr_t) (min(step * 4 + q, p.blocks - 1) * MX_BLOCK);
-                wsh[i] = (uint32_t) a & 3u;
-                wr[i] = *(const mx_i4_a4 *) (a & ~(uintptr_t) 3);
-                wd[i] = *(const int *) ((a & ~(uintptr_t) 3) + 16);
-            }
+    auto fetch_w = [&](const int i, const int step) {
+        if (DW) {
+            const uint8_t * a = w0 + (int64_t) step * (4 * MX_BLOCK);
+            wr[i] = *(const mx_i4_a4 *) (a + wl[i]);
+            wd[i] = *(const int *) (a + 64 - 16 * q + wl[i]);
+        } else {
+            const uint32_t a = wl[i] + (uint32_t) (min(step * 4 + q, p.blocks - 1) * MX_BLOCK);
+            wsh[i] = a & 3u;
+            wr[i] = *(const mx_i4_a4 *) (w0 + (a & ~3u));
+            wd[i] = *(const int *) (w0 + (a & ~3u) + 16);
         }
     };
-    auto store_w = [&](const int buf) {
-#pragma unroll
-        for (int i = 0; i < RT / 2; ++i) {
-            const uint32_t sh = DW ? (uint32_t) q : wsh[i];
-            const int next = __builtin_amdgcn_update_dpp(0, wr[i].x, 0xF9, 0xF, 0xF, true);  // (the first dword of the quad's next lane: quad_perm 1, 2, 3, 3)
-            const int d = !DW || q == 3 ? wd[i] : next;
-            *(mx_i4 *) (s_w[buf] + q * PLANE + (lrow + 64 * i) * 16) = mx_window(wr[i], d, sh);
-            s_s[buf][(lrow + 64 * i) * 4 + q] = (uint8_t) ((uint32_t) wr[i].x >> (8 * sh));
-        }
+    auto store_w = [&](const int i, const int buf) {
+        const uint32_t sh = DW ? (uint32_t) q : wsh[i];
+        const int next = __builtin_amdgcn_update_dpp(0, wr[i].x, 0xF9, 0xF, 0xF, true);  // (the first dword of the quad's next lane: quad_perm 1, 2, 3, 3)
+        const int d = !DW || q == 3 ? wd[i] : next;
+        *(mx_i4 *) (s_w[buf] + q * PLANE + (lrow + 64 * i) * 16) = mx_window(wr[i], d, sh);
+        s_s[buf][(lrow + 64 * i) * 4 + q] = (uint8_t) ((uint32_t) wr[i].x >> (8 * sh));
     };
     const uint8_t * x = p.act + (int64_t) (live ? group : groups - 1) * p.steps * MX_ACT_STEP;
-    mx_i8 h[2], l[2], hn[2], ln[2];  // the digits of this step and of the next
+    const uint32_t x16 = (uint32_t) (half * MX_ACT_BLK + r32 * 16), x8 = (uint32_t) (half * MX_ACT_BLK + r32 * 8);
+    mx_i4 h4[2], l4[2], hn4[2], ln4[2];  // the digits of this step and of the next
+    mx_i2 h2[2], l2[2], hn2[2], ln2[2];
     uint32_t sx, sxn;
-    auto fetch_x = [&](const int step) {
+    auto fetch_x = [&](const int n, const int step) {  // the n-th of nine loads
         const uint8_t * xs = x + (int64_t) step * MX_ACT_STEP;
-        sxn = *(const uint32_t *) (xs + 4 * MX_ACT_BLK + r32 * 4);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const uint8_t * xb = xs + (2 * j + half) * MX_ACT_BLK;
-            hn[j] = mx_op6(*(const mx_i4 *) (xb + r32 * 16), *(const mx_i2 *) (xb + 1024 + r32 * 8));
-            ln[j] = mx_op6(*(const mx_i4 *) (xb + 512 + r32 * 16), *(const mx_i2 *) (xb + 1280 + r32 * 8));
-        }
+        if (n == 0) sxn = *(const uint32_t *) (xs + 4 * MX_ACT_BLK + r32 * 4);
+        const int j = (n - 1) >> 2, what = (n - 1) & 3;
+        const uint8_t * xb = xs + 2 * j * MX_ACT_BLK;
+        if (n > 0 && what == 0) hn4[j] = *(const mx_i4 *) (xb + x16);
+        if (n > 0 && what == 1) hn2[j] = *(const mx_i2 *) (xb + 1024 + x8);
+        if (n > 0 && what == 2) ln4[j] = *(const mx_i4 *) (xb + 512 + x16);
+        if (n > 0 && what == 3) ln2[j] = *(const mx_i2 *) (xb + 1280 + x8);
     };
     auto take_x = [&]() {
         sx = sxn;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            h[j] = hn[j];
-            l[j] = ln[j];
+            h4[j] = hn4[j];
+            h2[j] = hn2[j];
+            l4[j] = ln4[j];
+            l2[j] = ln2[j];
         }
     };
     mx_f16 acc[RT];
@@ -642,56 +669,197 @@ template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, 2) k_
     for (int t = 0; t < RT; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
-    auto multiply = [&](const int buf) {
+    const int last = p.steps - 1;
+    // in groups of SET tiles and a half step: an accumulator's next product comes SET instructions later, and the next group's weights are read meanwhile
+    auto multiply = [&](const int buf, const int step) {
+        constexpr int GROUPS = 2 * SETS, ITEMS = 9 + 3 * (RT / 2), SLOTS = GROUPS * 2 * SET, PER = (ITEMS + SLOTS - 1) / SLOTS;
+        const int next = min(step + 1, last), after = min(step + 2, last);  // (behind the last step: loads that nobody uses)
         const uint32_t sh = sx >> (8 * half), sl = sh - 0x00040004u;
-        int sw[RT];
+        auto item = [&](const int n) {
+            if (n < 9) fetch_x(n, next);
+            else if (n < ITEMS && (n - 9) % 3 == 0) store_w((n - 9) / 3, buf ^ 1);
+            else if (n < ITEMS && (n - 9) % 3 == 1) fetch_w((n - 9) / 3, after);
+        };
+        mx_i4 a[2][SET];
+        int sw[2][SET];
+        auto read = [&](const int g) {
+            const int j = g / SETS, t0 = (g % SETS) * SET;
 #pragma unroll
-        for (int t = 0; t < RT; ++t) sw[t] = (int) (*(const uint32_t *) (s_s[buf] + (32 * t + r32) * 4) >> (8 * half));
+            for (int u = 0; u < SET; ++u) {
+                a[g & 1][u] = *(const mx_i4 *) (s_w[buf] + (2 * j + half) * PLANE + (32 * (t0 + u) + r32) * 16);
+                sw[g & 1][u] = (int) (*(const uint32_t *) (s_s[buf] + (32 * (t0 + u) + r32) * 4) >> (8 * half));
+            }
+        };
+        read(0);
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            const mx_i8 a0 = mx_op4(*(const mx_i4 *) (s_w[buf] + half * PLANE + (32 * t + r32) * 16)), a1 = mx_op4(*(const mx_i4 *) (s_w[buf] + (2 + half) * PLANE + (32 * t + r32) * 16));
-            acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a0, h[0], acc[t], MX_FP4, MX_FP6, 0, sw[t], 0, (int) sh);
-            acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a0, l[0], acc[t], MX_FP4, MX_FP6, 0, sw[t], 0, (int) sl);
-            acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a1, h[1], acc[t], MX_FP4, MX_FP6, 2, sw[t], 2, (int) sh);
-            acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a1, l[1], acc[t], MX_FP4, MX_FP6, 2, sw[t], 2, (int) sl);
+        for (int g = 0; g < GROUPS; ++g) {
+            const int j = g / SETS, t0 = (g % SETS) * SET;
+            if (g + 1 < GROUPS) read(g + 1);
+            const mx_i8 hx = mx_op6(h4[j], h2[j]), lx = mx_op6(l4[j], l2[j]);
+#pragma unroll
+            for (int u = 0; u < 2 * SET; ++u) {
+                const int t = u % SET;
+                const mx_i8 wx = mx_op4(a[g & 1][t]);
+                if (j == 0) acc[t0 + t] = u < SET ? MX_MFMA1(wx, hx, acc[t0 + t], 0, sw[g & 1][t], sh) : MX_MFMA1(wx, lx, acc[t0 + t], 0, sw[g & 1][t], sl);
+                else acc[t0 + t] = u < SET ? MX_MFMA1(wx, hx, acc[t0 + t], 2, sw[g & 1][t], sh) : MX_MFMA1(wx, lx, acc[t0 + t], 2, sw[g & 1][t], sl);
+#pragma unroll
+                for (int k = 0; k < PER; ++k) item((g * 2 * SET + u) * PER + k);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     };
-    fetch_w(0);
-    fetch_x(0);
-    store_w(0);
+#pragma unroll
+    for (int i = 0; i < RT / 2; ++i) fetch_w(i, 0);
+#pragma unroll
+    for (int n = 0; n < 9; ++n) fetch_x(n, 0);
+#pragma unroll
+    for (int i = 0; i < RT / 2; ++i) {
+        store_w(i, 0);
+        fetch_w(i, min(1, last));
+    }
     take_x();
     __syncthreads();
     for (int step = 0, buf = 0; step < p.steps; ++step, buf ^= 1) {
-        const int next = min(step + 1, p.steps - 1);  // (behind the last step: loads that nobody uses)
-        fetch_w(next);
-        fetch_x(next);
-        __builtin_amdgcn_sched_barrier(0);  // (all of them are on their way before the first product)
-        multiply(buf);
-        __builtin_amdgcn_sched_barrier(0);
-        store_w(buf ^ 1);
+        multiply(buf, step);
         take_x();
         __syncthreads();
     }
     if (!live) return;
-    int64_t c = (int64_t) group * 32 + r32;
-    if (ID) c = p.l.list[c];
-    if (c < 0 || (!ID && c >= p.cols)) return;
-    float * d = p.dst + c * p.ldd;
-    const float * bias = p.bias ? (const float *) ((const char *) p.bias + (int64_t) e * p.nb_bias) : nullptr;
-    const bool wide = ((((uintptr_t) d) | (uintptr_t) (p.ldd * 4)) & 15) == 0 && row0 + ROWS <= p.n_rows && !bias;
+    mx_store_tile<ID, RT>(p, acc, group, row0, e, r32, half);
+}
+// ---- many columns of rows that are whole 16-byte pieces (K a multiple of 512: 272 bytes): as k_mx_tile, but the weights go to LDS by DMA as they lie in memory, 512 values a stage and row by row, and a
+// lane moves its codes into place behind its LDS read: at byte 17 i of its half row (8 blocks, 136 bytes) block i starts at byte i of an 8-byte unit, and needs the two units behind it, so that a block
+// costs one 16-byte read (the unit between two blocks is kept) and up to four byte shifts.  The digits of the eight blocks are requested again right behind their last product, a stage ahead of the next.
+__device__ __forceinline__ void mx_dma16(const uint8_t * base, const uint32_t off, const uint32_t lds) {  // lane i's 16 bytes at base + off to LDS[lds + 16 i]; base and lds of the wave
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0" : "=&s"(keep) : "v"(off), "s"(base), "s"(lds));
+}
+template <int RT> constexpr int mx_wide_pieces() { return (32 * RT * 17 + 255) / 256; }  // DMA instructions a wave and stage
+template <bool ID, int RT> __global__ void __launch_bounds__(256, RT == 8 ? 1 : 2) k_mx_wide(const mx_mm p, const int row_tiles) {
+    constexpr int SET = RT < 4 ? RT : 4, SETS = RT / SET, ROWS = 32 * RT, PIECES = mx_wide_pieces<RT>(), STAGE = PIECES * 4096, PER = 8 / RT;
+    static_assert(PIECES <= 4 + 5 * 3, "a stage's pieces");
+    extern __shared__ __align__(16) uint8_t lds[];  // two stages of [row] 272 bytes
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r32 = lane & 31, half = lane >> 5;
+    int rt, tile;
+    if (ID) {
+        rt = blockIdx.x % row_tiles;
+        tile = blockIdx.x / row_tiles;
+    } else {
+        const int n_tiles = (int) ((p.cols + 127) / 128), at = (int) (blockIdx.x & 7) * (int) (gridDim.x >> 3) + (int) (blockIdx.x >> 3);
+        tile = at % n_tiles;
+        rt = at / n_tiles;
+        if (rt >= row_tiles) return;
+    }
+    const int row0 = rt * ROWS;
+    int e = 0, group = tile * 4 + wave, groups = (int) ((p.cols + 31) / 32);
+    if (ID) {
+        if (tile >= p.l.total[1]) return;
+        const int32_t * t = p.l.tiles + 4 * tile;
+        e = t[0];
+        group = t[1] + wave;
+        groups = t[1] + t[2];
+    }
+    const bool live = group < groups;
+    const uint8_t * w = p.w + (int64_t) e * p.nb2 + (int64_t) row0 * p.nb1;
+    uint32_t wo[PIECES];  // the lane's pieces: 17 a row, in the order of LDS
+#pragma unroll
+    for (int n = 0; n < PIECES; ++n) {
+        const int c = n * 256 + tid, row = min(min(c / 17, ROWS - 1), p.n_rows - 1 - row0);
+        wo[n] = (uint32_t) row * (uint32_t) p.nb1 + (uint32_t) (c % 17) * 16u;
+    }
+    const uint32_t lds0 = (uint32_t) (uintptr_t) lds;
+    auto dma = [&](const int n, const int stage, const int buf) { mx_dma16(w + (int64_t) stage * 272, wo[n], lds0 + (uint32_t) (buf * STAGE + n * 4096 + wave * 1024)); };
+    const uint8_t * x = p.act + (int64_t) (live ? group : groups - 1) * p.steps * MX_ACT_STEP;
+    const uint32_t x16 = (uint32_t) (half * 2 * MX_ACT_STEP + r32 * 16), x8 = (uint32_t) (half * 2 * MX_ACT_STEP + r32 * 8), x4 = (uint32_t) (half * 2 * MX_ACT_STEP + r32 * 4);
+    mx_i4 h4[8], l4[8];
+    mx_i2 h2[8], l2[8];
+    uint32_t sx[2];
+    auto fetch_x = [&](const int i, const int what, const int stage) {
+        const uint8_t * xs = x + (int64_t) stage * (4 * MX_ACT_STEP) + (i / 4) * MX_ACT_STEP, * xb = xs + (i % 4) * MX_ACT_BLK;
+        if (what == 0) h4[i] = *(const mx_i4 *) (xb + x16);
+        if (what == 1) h2[i] = *(const mx_i2 *) (xb + 1024 + x8);
+        if (what == 2) l4[i] = *(const mx_i4 *) (xb + 512 + x16);
+        if (what == 3) l2[i] = *(const mx_i2 *) (xb + 1280 + x8);
+        if (what == 3 && i % 4 == 3) sx[i / 4] = *(const uint32_t *) (xs + 4 * MX_ACT_BLK + x4);
+    };
+    mx_f16 acc[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = row0 + 32 * t + 8 * i + 4 * half;
-            if (wide) {
-                *(mx_f4 *) (d + row) = mx_f4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]};
-            } else {
+        for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
+    const int stages = p.steps / 4;
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (row + k < p.n_rows) d[row + k] = bias ? acc[t][4 * i + k] + bias[row + k] : acc[t][4 * i + k];
+    for (int n = 0; n < PIECES; ++n) dma(n, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 5; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) fetch_x(i, k, 0);
+    sx[0] = *(const uint32_t *) (x + 4 * MX_ACT_BLK + x4);
+    sx[1] = *(const uint32_t *) (x + MX_ACT_STEP + 4 * MX_ACT_BLK + x4);
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    for (int stage = 0, buf = 0; stage < stages; ++stage, buf ^= 1) {
+        const int next = min(stage + 1, stages - 1);  // (behind the last stage: loads that nobody uses)
+        const uint8_t * at = lds + buf * STAGE + r32 * 272 + half * 136;
+        mx_i2 kept[RT];
+        mx_i4 a[2][SET];
+        // items of block i, PER behind each of its 2 RT products while they last: digits of block i - 1 of the next stage (5 .. 7 of this stage in block 0), three pieces of the next stage's weights
+        auto item = [&](const int i, const int n) {
+            if (i == 0 && n < 12) fetch_x(5 + n / 4, n % 4, stage);
+            if (i >= 1 && i <= 5 && n < 4) fetch_x(i - 1, n, next);
+            const int d = i == 0 ? n - 12 : n - 4;
+            constexpr int first = 4, each = 3;  // (block 0 has room for four pieces beside its digits)
+            if (i == 0 && d >= 0 && d < first && d < PIECES) dma(d, next, buf ^ 1);
+            if (i >= 1 && i <= 5 && d >= 0 && d < each && first + (i - 1) * each + d < PIECES) dma(first + (i - 1) * each + d, next, buf ^ 1);
+        };
+        auto read = [&](const int g) {  // group g: block g / SETS, tiles of set g % SETS
+            const int i = g / SETS, t0 = (g % SETS) * SET;
+#pragma unroll
+            for (int u = 0; u < SET; ++u) {
+                typedef mx_i4 __attribute__((aligned(8))) mx_i4_a8;
+                a[g & 1][u] = *(const mx_i4_a8 *) (at + (t0 + u) * (32 * 272) + 16 * i + 8);
+            }
+        };
+#pragma unroll
+        for (int t = 0; t < RT; ++t) kept[t] = *(const mx_i2 *) (at + t * (32 * 272));
+        read(0);
+#pragma unroll
+        for (int g = 0; g < 8 * SETS; ++g) {
+            const int i = g / SETS, t0 = (g % SETS) * SET;
+            if (g + 1 < 8 * SETS) read(g + 1);
+            const mx_i8 hx = mx_op6(h4[i], h2[i]), lx = mx_op6(l4[i], l2[i]);
+            const uint32_t sh = sx[i / 4], sl = sh - 0x04040404u;
+            mx_i8 wx[SET];
+            int sw[SET];
+#pragma unroll
+            for (int u = 0; u < SET; ++u) {
+                const mx_i4 v = a[g & 1][u];
+                const int d[6] = {kept[t0 + u].x, kept[t0 + u].y, v.x, v.y, v.z, v.w};
+                const int k = (i + 1) / 4, sh8 = (i + 1) % 4;
+                mx_i4 c;
+#pragma unroll
+                for (int z = 0; z < 4; ++z) c[z] = sh8 ? (int) __builtin_amdgcn_alignbyte(d[k + z + (sh8 ? 1 : 0)], d[k + z], sh8) : d[k + z];
+                wx[u] = mx_op4(c);
+                sw[u] = d[i / 4];
+                kept[t0 + u] = mx_i2{v.z, v.w};
+            }
+#pragma unroll
+            for (int u = 0; u < 2 * SET; ++u) {
+                const int t = u % SET;
+                const mx_i8 dx = u < SET ? hx : lx;
+                const uint32_t sd = u < SET ? sh : sl;
+                if (i % 4 == 0) acc[t0 + t] = MX_MFMA1(wx[t], dx, acc[t0 + t], 0, sw[t], sd);
+                if (i % 4 == 1) acc[t0 + t] = MX_MFMA1(wx[t], dx, acc[t0 + t], 1, sw[t], sd);
+                if (i % 4 == 2) acc[t0 + t] = MX_MFMA1(wx[t], dx, acc[t0 + t], 2, sw[t], sd);
+                if (i % 4 == 3) acc[t0 + t] = MX_MFMA1(wx[t], dx, acc[t0 + t], 3, sw[t], sd);
+#pragma unroll
+                for (int k = 0; k < PER; ++k) item(i, ((g % SETS) * 2 * SET + u) * PER + k);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (the next stage has landed; the last requests are two blocks old)
+    }
+    if (!live) return;
+    mx_store_tile<ID, RT>(p, acc, group, row0, e, r32, half);
 }
 static mx_mm mx_args(const tdesc & w, const tdesc & d, int64_t cols) {
     mx_mm p{};
@@ -721,6 +889,9 @@ bool mx_vec_takes(int64_t K, int64_t cols) { return cols <= MX_VEC_COLS && mx_ve
 bool mx_id_vec_takes(int64_t K, int64_t cols) { return cols <= MX_VEC_ID_COLS && mx_vec_chunk(K, cols) >= 1; }
 // rows of whole steps, every one at a whole dword
 static bool mx_dwords(const mx_mm & p) { return p.blocks % 4 == 0 && p.nb1 % 4 == 0 && p.nb2 % 4 == 0 && ((uintptr_t) p.w & 3) == 0; }
+// ... of whole 16-byte pieces
+static bool mx_pieces(const mx_mm & p) { return p.blocks % 16 == 0 && p.nb1 % 16 == 0 && p.nb2 % 16 == 0 && ((uintptr_t) p.w & 15) == 0 && p.nb1 <= (1 << 24); }
+
 static void mx_launch_vec(hipStream_t s, const mx_mm & p, const tdesc & b, const tdesc * ids) {
     const int64_t K = b.ne[0];
     const int chunk = mx_vec_chunk(K, p.cols);
@@ -734,6 +905,14 @@ static void mx_launch_vec(hipStream_t s, const mx_mm & p, const tdesc & b, const
 template <bool ID, int RT> static void mx_launch_tile_of(hipStream_t s, const mx_mm & p, int64_t col_tiles) {
     const int row_tiles = (p.n_rows + 32 * RT - 1) / (32 * RT);
     const dim3 grid((unsigned) ((row_tiles * col_tiles + 7) / 8 * 8));
+    if (mx_pieces(p)) {
+        constexpr size_t lds = 2 * mx_wide_pieces<RT>() * 4096;
+        static std::atomic<uint32_t> done{0};
+        if (ensure_dyn_lds((const void *) k_mx_wide<ID, RT>, lds, done)) {
+            hipLaunchKernelGGL((k_mx_wide<ID, RT>), grid, dim3(256), lds, s, p, row_tiles);
+            return;
+        }
+    }
     if (mx_dwords(p)) hipLaunchKernelGGL((k_mx_tile<ID, RT, true>), grid, dim3(256), 0, s, p, row_tiles);
     else hipLaunchKernelGGL((k_mx_tile<ID, RT, false>), grid, dim3(256), 0, s, p, row_tiles);
 }
