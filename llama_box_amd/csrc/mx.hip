@@ -735,9 +735,9 @@ __device__ __forceinline__ void mx_dma16(const uint8_t * base, const uint32_t of
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0" : "=&s"(keep) : "v"(off), "s"(base), "s"(lds));
 }
 template <int RT> constexpr int mx_wide_pieces() { return (32 * RT * 17 + 255) / 256; }  // DMA instructions a wave and stage
-template <bool ID, int RT> __global__ void __launch_bounds__(256, RT == 8 ? 1 : 2) k_mx_wide(const mx_mm p, const int row_tiles) {
-    constexpr int SET = RT < 4 ? RT : 4, SETS = RT / SET, ROWS = 32 * RT, PIECES = mx_wide_pieces<RT>(), STAGE = PIECES * 4096, PER = 8 / RT;
-    static_assert(PIECES <= 4 + 5 * 3, "a stage's pieces");
+template <bool ID, int RT> __global__ void __launch_bounds__(256, 1) k_mx_wide(const mx_mm p, const int row_tiles) {
+    constexpr int SET = RT < 4 ? RT : 4, SETS = RT / SET, ROWS = 32 * RT, PIECES = mx_wide_pieces<RT>(), STAGE = PIECES * 4096;
+    static_assert(PIECES <= 17, "a stage's pieces");
     extern __shared__ __align__(16) uint8_t lds[];  // two stages of [row] 272 bytes
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r32 = lane & 31, half = lane >> 5;
     int rt, tile;
@@ -787,76 +787,88 @@ template <bool ID, int RT> __global__ void __launch_bounds__(256, RT == 8 ? 1 : 
     for (int t = 0; t < RT; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
+    // The stream of groups (a block of each half row, SET tiles), GROUPS a stage: group g is multiplied, the codes of g + 1 are moved into place, those of g + 2 read.  An accumulator's next product
+    // comes SET instructions later, and what a product's time leaves room for stands behind it.  The one barrier of a stage lies ahead of its last two groups, which already read the next stage: all
+    // of this stage's reads are done by then, and the DMA of the next one, first thing in a stage, has landed.
+    constexpr int GROUPS = 8 * SETS, SLOTS = 2 * SET;
     const int stages = p.steps / 4;
+    const uint8_t * own = lds + r32 * 272 + half * 136;
+    mx_i2 kept[RT];       // the unit between a tile's last block and its next
+    mx_i4 a[2][SET];      // the two units behind it
+    mx_i8 wx[2][SET];     // codes in place
+    int sw[2][SET];
+    auto read = [&](const int g, const int u, const uint8_t * at) {
+        typedef mx_i4 __attribute__((aligned(8))) mx_i4_a8;
+        a[g & 1][u] = *(const mx_i4_a8 *) (at + ((g % SETS) * SET + u) * (32 * 272) + 16 * (g / SETS) + 8);
+    };
+    auto place = [&](const int g, const int u) {
+        const int i = g / SETS, t = (g % SETS) * SET + u, k = (i + 1) / 4, sh8 = (i + 1) % 4;
+        const mx_i4 v = a[g & 1][u];
+        const int d[6] = {kept[t].x, kept[t].y, v.x, v.y, v.z, v.w};
+        mx_i4 c;
+#pragma unroll
+        for (int z = 0; z < 4; ++z) c[z] = sh8 ? (int) __builtin_amdgcn_alignbyte(d[k + z + (sh8 ? 1 : 0)], d[k + z], sh8) : d[k + z];
+        wx[g & 1][u] = mx_op4(c);
+        sw[g & 1][u] = d[i / 4];
+        kept[t] = mx_i2{v.z, v.w};
+    };
+    auto read_first = [&](const int t, const uint8_t * at) { kept[t] = *(const mx_i2 *) (at + t * (32 * 272)); };
 #pragma unroll
     for (int n = 0; n < PIECES; ++n) dma(n, 0, 0);
 #pragma unroll
-    for (int i = 0; i < 5; ++i)
+    for (int i = 0; i < 7; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) fetch_x(i, k, 0);
-    sx[0] = *(const uint32_t *) (x + 4 * MX_ACT_BLK + x4);
-    sx[1] = *(const uint32_t *) (x + MX_ACT_STEP + 4 * MX_ACT_BLK + x4);
+        for (int k = 0; k < 4; ++k) {
+            fetch_x(i, k, 0);
+            __builtin_amdgcn_sched_barrier(0);  // (in the order of the loop's: the compiler's counts of what is under way then hold for both)
+        }
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int t = 0; t < RT; ++t) read_first(t, own);
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int u = 0; u < SET; ++u) {
+            read(g, u, own);
+            if (g == 0) place(0, u);
+        }
     for (int stage = 0, buf = 0; stage < stages; ++stage, buf ^= 1) {
         const int next = min(stage + 1, stages - 1);  // (behind the last stage: loads that nobody uses)
-        const uint8_t * at = lds + buf * STAGE + r32 * 272 + half * 136;
-        mx_i2 kept[RT];
-        mx_i4 a[2][SET];
-        // items of block i, PER behind each of its 2 RT products while they last: digits of block i - 1 of the next stage (5 .. 7 of this stage in block 0), three pieces of the next stage's weights
-        auto item = [&](const int i, const int n) {
-            if (i == 0 && n < 12) fetch_x(5 + n / 4, n % 4, stage);
-            if (i >= 1 && i <= 5 && n < 4) fetch_x(i - 1, n, next);
-            const int d = i == 0 ? n - 12 : n - 4;
-            constexpr int first = 4, each = 3;  // (block 0 has room for four pieces beside its digits)
-            if (i == 0 && d >= 0 && d < first && d < PIECES) dma(d, next, buf ^ 1);
-            if (i >= 1 && i <= 5 && d >= 0 && d < each && first + (i - 1) * each + d < PIECES) dma(first + (i - 1) * each + d, next, buf ^ 1);
-        };
-        auto read = [&](const int g) {  // group g: block g / SETS, tiles of set g % SETS
+        const uint8_t * at = own + buf * STAGE, * at_next = own + (buf ^ 1) * STAGE;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
             const int i = g / SETS, t0 = (g % SETS) * SET;
-#pragma unroll
-            for (int u = 0; u < SET; ++u) {
-                typedef mx_i4 __attribute__((aligned(8))) mx_i4_a8;
-                a[g & 1][u] = *(const mx_i4_a8 *) (at + (t0 + u) * (32 * 272) + 16 * i + 8);
-            }
-        };
-#pragma unroll
-        for (int t = 0; t < RT; ++t) kept[t] = *(const mx_i2 *) (at + t * (32 * 272));
-        read(0);
-#pragma unroll
-        for (int g = 0; g < 8 * SETS; ++g) {
-            const int i = g / SETS, t0 = (g % SETS) * SET;
-            if (g + 1 < 8 * SETS) read(g + 1);
             const mx_i8 hx = mx_op6(h4[i], h2[i]), lx = mx_op6(l4[i], l2[i]);
             const uint32_t sh = sx[i / 4], sl = sh - 0x04040404u;
-            mx_i8 wx[SET];
-            int sw[SET];
+            if (g == GROUPS - 2) asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (more than 16 requests of digits lie behind the last DMA)
 #pragma unroll
-            for (int u = 0; u < SET; ++u) {
-                const mx_i4 v = a[g & 1][u];
-                const int d[6] = {kept[t0 + u].x, kept[t0 + u].y, v.x, v.y, v.z, v.w};
-                const int k = (i + 1) / 4, sh8 = (i + 1) % 4;
-                mx_i4 c;
-#pragma unroll
-                for (int z = 0; z < 4; ++z) c[z] = sh8 ? (int) __builtin_amdgcn_alignbyte(d[k + z + (sh8 ? 1 : 0)], d[k + z], sh8) : d[k + z];
-                wx[u] = mx_op4(c);
-                sw[u] = d[i / 4];
-                kept[t0 + u] = mx_i2{v.z, v.w};
-            }
-#pragma unroll
-            for (int u = 0; u < 2 * SET; ++u) {
+            for (int u = 0; u < SLOTS; ++u) {
                 const int t = u % SET;
                 const mx_i8 dx = u < SET ? hx : lx;
                 const uint32_t sd = u < SET ? sh : sl;
-                if (i % 4 == 0) acc[t0 + t] = MX_MFMA1(wx[t], dx, acc[t0 + t], 0, sw[t], sd);
-                if (i % 4 == 1) acc[t0 + t] = MX_MFMA1(wx[t], dx, acc[t0 + t], 1, sw[t], sd);
-                if (i % 4 == 2) acc[t0 + t] = MX_MFMA1(wx[t], dx, acc[t0 + t], 2, sw[t], sd);
-                if (i % 4 == 3) acc[t0 + t] = MX_MFMA1(wx[t], dx, acc[t0 + t], 3, sw[t], sd);
+                if (i % 4 == 0) acc[t0 + t] = MX_MFMA1(wx[g & 1][t], dx, acc[t0 + t], 0, sw[g & 1][t], sd);
+                if (i % 4 == 1) acc[t0 + t] = MX_MFMA1(wx[g & 1][t], dx, acc[t0 + t], 1, sw[g & 1][t], sd);
+                if (i % 4 == 2) acc[t0 + t] = MX_MFMA1(wx[g & 1][t], dx, acc[t0 + t], 2, sw[g & 1][t], sd);
+                if (i % 4 == 3) acc[t0 + t] = MX_MFMA1(wx[g & 1][t], dx, acc[t0 + t], 3, sw[g & 1][t], sd);
+                if (u < SET) place((g + 1) % GROUPS, u);
+                else if (g + 2 < GROUPS) read(g + 2, u - SET, at);
+                else {
+                    if (g + 2 - GROUPS < SETS) read_first((g + 2 - GROUPS) * SET + u - SET, at_next);
+                    read(g + 2 - GROUPS, u - SET, at_next);
+                }
+                // requests, the n-th slot of block i: the next stage's weights and the last block's digits in block 0, then the digits of block i - 1 of the next stage
+                constexpr int PER = 8 / RT;
 #pragma unroll
-                for (int k = 0; k < PER; ++k) item(i, ((g % SETS) * 2 * SET + u) * PER + k);
+                for (int k = 0; k < PER; ++k) {
+                    const int n = ((g % SETS) * SLOTS + u) * PER + k;
+                    if (i == 0 && n < 4) fetch_x(7, n, stage);
+                    if (i == 0 && n < PIECES) dma(n, next, buf ^ 1);
+                    if (i == 1 && n == 0 && PIECES == 17) dma(16, next, buf ^ 1);
+                    if (i >= 1 && n >= 4 && n < 8) fetch_x(i - 1, n - 4, next);
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (the next stage has landed; the last requests are two blocks old)
     }
     if (!live) return;
     mx_store_tile<ID, RT>(p, acc, group, row0, e, r32, half);
