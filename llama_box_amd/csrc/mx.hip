@@ -11,6 +11,9 @@
 #include "dev_util.h"
 #include "kernels.h"
 
+#ifndef MX_SET
+#define MX_SET 1
+#endif
 namespace mi355x {
 
 typedef int mx_i4 __attribute__((ext_vector_type(4)));
@@ -728,16 +731,131 @@ template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, RT ==
     mx_store_tile<ID, RT>(p, acc, group, row0, e, r32, half);
 }
 // ---- many columns of rows that are whole 16-byte pieces (K a multiple of 512: 272 bytes): as k_mx_tile, but the weights go to LDS by DMA as they lie in memory, 512 values a stage and row by row, and a
-// lane moves its codes into place behind its LDS read: at byte 17 i of its half row (8 blocks, 136 bytes) block i starts at byte i of an 8-byte unit, and needs the two units behind it, so that a block
-// costs one 16-byte read (the unit between two blocks is kept) and up to four byte shifts.  The digits of the eight blocks are requested again right behind their last product, a stage ahead of the next.
+// lane moves its codes into place behind its LDS read.  Eight waves: a group of columns has two, which take the even and the odd quarters of a row's stage (68 bytes, four blocks each) and add up at the
+// end; the second wave of a SIMD issues while the first one's product runs (one wave alone, eight blocks a stage: 512 columns 46 us).  In a quarter that starts at a unit of 8 bytes (the odd ones: at its
+// second half) block i starts at byte i of a unit, and needs the two units behind it: one 16-byte read a block (the unit between two blocks is kept) and up to four byte shifts.
 __device__ __forceinline__ void mx_dma16(const uint8_t * base, const uint32_t off, const uint32_t lds) {  // lane i's 16 bytes at base + off to LDS[lds + 16 i]; base and lds of the wave
     uint32_t keep;
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0" : "=&s"(keep) : "v"(off), "s"(base), "s"(lds));
 }
-template <int RT> constexpr int mx_wide_pieces() { return (32 * RT * 17 + 255) / 256; }  // DMA instructions a wave and stage
-template <bool ID, int RT> __global__ void __launch_bounds__(256, 1) k_mx_wide(const mx_mm p, const int row_tiles) {
-    constexpr int SET = RT < 4 ? RT : 4, SETS = RT / SET, ROWS = 32 * RT, PIECES = mx_wide_pieces<RT>(), STAGE = PIECES * 4096;
-    static_assert(PIECES <= 17, "a stage's pieces");
+template <int RT> constexpr int mx_wide_pieces() { return (32 * RT * 17 + 511) / 512; }  // DMA instructions a wave and stage
+template <int RT> struct mx_wide_args {
+    const uint8_t * w;    // the tile's first row
+    uint32_t first, last; // byte offsets of the lane's pieces of a stage (17 a row, in the order of LDS): its first and its last; the n-th between them is 30 rows and 2 pieces behind the one before,
+    int piece;            // one row and no 17 pieces where that leaves the row (piece: of the first)
+    uint32_t jump, wrap;
+    const uint8_t * x;    // the group's digits
+    int stages, wave, lane;
+};
+// one wave's share of a tile: quarter 2 half + ODD of every stage
+template <int RT, int ODD> __device__ __forceinline__ void mx_wide_sum(const mx_wide_args<RT> & p, uint8_t * lds, mx_f16 (&acc)[RT]) {
+    constexpr int SET = MX_SET, SETS = RT / SET, PIECES = mx_wide_pieces<RT>(), STAGE = PIECES * 8192, GROUPS = 4 * SETS, SLOTS = 2 * SET;
+    const int r32 = p.lane & 31, half = p.lane >> 5;
+    const uint32_t lds0 = (uint32_t) (uintptr_t) lds;
+    uint32_t first = p.first;
+    auto dma = [&](const int n, const int stage, const int buf) {
+        const uint32_t off = n == PIECES - 1 ? p.last : first + (uint32_t) n * p.jump + (p.piece >= 17 - 2 * n ? p.wrap : 0u);
+        mx_dma16(p.w + (int64_t) stage * 272, off, lds0 + (uint32_t) (buf * STAGE + n * 8192 + p.wave * 1024));
+    };
+    const uint32_t q = (uint32_t) (half * 2 + ODD) * MX_ACT_STEP, x16 = q + (uint32_t) r32 * 16, x8 = q + (uint32_t) r32 * 8, x4 = q + (uint32_t) r32 * 4;
+    const __amdgpu_buffer_rsrc_t digits = __builtin_amdgcn_make_buffer_rsrc((void *) p.x, 0, p.stages * (4 * MX_ACT_STEP), 0x00020000);
+    mx_i4 h4[4], l4[4];
+    mx_i2 h2[4], l2[4];
+    uint32_t sx, sxn;  // the scale bytes of this stage's four blocks and of the next's
+    auto fetch_x = [&](const int i, const int what, const int stage) {
+        const int at = stage * (4 * MX_ACT_STEP), blk = at + i * MX_ACT_BLK;
+        if (what == 0) h4[i] = __builtin_bit_cast(mx_i4, __builtin_amdgcn_raw_buffer_load_b128(digits, (int) x16, blk, 0));
+        if (what == 1) h2[i] = __builtin_bit_cast(mx_i2, __builtin_amdgcn_raw_buffer_load_b64(digits, (int) x8, blk + 1024, 0));
+        if (what == 2) l4[i] = __builtin_bit_cast(mx_i4, __builtin_amdgcn_raw_buffer_load_b128(digits, (int) x16, blk + 512, 0));
+        if (what == 3) l2[i] = __builtin_bit_cast(mx_i2, __builtin_amdgcn_raw_buffer_load_b64(digits, (int) x8, blk + 1280, 0));
+        if (what == 3 && i == 0) sxn = (uint32_t) __builtin_amdgcn_raw_buffer_load_b32(digits, (int) x4, at + 4 * MX_ACT_BLK, 0);
+    };
+    // The stream of groups (a block, SET tiles), GROUPS a stage: group g is multiplied, the codes of g + 1 are moved into place, those of g + 2 read, and what a product's time leaves room for stands
+    // behind it.  The one barrier of a stage lies ahead of its last two groups, which already read the next stage: all of this stage's reads are done by then, and the DMA of the next one, first thing
+    // in a stage, has landed.
+    const uint8_t * own = lds + r32 * 272 + half * 136 + ODD * 64;
+    mx_i2 kept[RT];       // the unit between a tile's last block and its next
+    mx_i4 a[2][SET];      // the two units behind it
+    mx_i8 wx[2][SET];     // codes in place
+    int sw[2][SET];
+    auto read = [&](const int g, const int u, const uint8_t * at) {
+        typedef mx_i4 __attribute__((aligned(8))) mx_i4_a8;
+        const int t = (g % SETS) * SET + u;
+        if (g < SETS) kept[t] = *(const mx_i2 *) (at + t * (32 * 272));
+        a[g & 1][u] = *(const mx_i4_a8 *) (at + t * (32 * 272) + 16 * (g / SETS) + 8);
+    };
+    auto place = [&](const int g, const int u) {
+        const int i = g / SETS, t = (g % SETS) * SET + u, k = (i + 1) / 4 + ODD, sh8 = (i + 1) % 4;
+        const mx_i4 v = a[g & 1][u];
+        const int d[6] = {kept[t].x, kept[t].y, v.x, v.y, v.z, v.w};
+        mx_i4 c;
+#pragma unroll
+        for (int z = 0; z < 4; ++z) c[z] = sh8 ? (int) __builtin_amdgcn_alignbyte(d[k + z + (sh8 ? 1 : 0)], d[k + z], sh8) : d[k + z];
+        wx[g & 1][u] = mx_op4(c);
+        sw[g & 1][u] = d[ODD];
+        kept[t] = mx_i2{v.z, v.w};
+    };
+#pragma unroll
+    for (int n = 0; n < PIECES; ++n) dma(n, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            fetch_x(i, k, 0);
+            __builtin_amdgcn_sched_barrier(0);  // (in the order of the loop's: the compiler's counts of what is under way then hold for both)
+        }
+    sx = sxn;
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int u = 0; u < SET; ++u) {
+            read(g, u, own);
+            if (g == 0) place(0, u);
+        }
+    for (int stage = 0, buf = 0; stage < p.stages; ++stage, buf ^= 1) {
+        const int next = min(stage + 1, p.stages - 1);  // (behind the last stage: loads that nobody uses)
+        const uint8_t * at = own + buf * STAGE, * at_next = own + (buf ^ 1) * STAGE;
+        asm volatile("" : "+v"(first));  // (the pieces' offsets are made where they are used: kept for the whole loop they leave no room for the digits)
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            const int i = g / SETS, t0 = (g % SETS) * SET;
+            const mx_i8 hx = mx_op6(h4[i], h2[i]), lx = mx_op6(l4[i], l2[i]);
+            const uint32_t sh = sx, sl = sh - 0x04040404u;
+            // (at least as many requests of digits lie behind the last DMA: those of block 1 and, with eight tiles, 2)
+            if (g == GROUPS - 2) {
+                if (RT == 8) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                else asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            }
+#pragma unroll
+            for (int u = 0; u < SLOTS; ++u) {
+                const int t = u % SET;
+                const mx_i8 dx = u < SET ? hx : lx;
+                const uint32_t sd = u < SET ? sh : sl;
+                if (i == 0) acc[t0 + t] = MX_MFMA1(wx[g & 1][t], dx, acc[t0 + t], 0, sw[g & 1][t], sd);
+                if (i == 1) acc[t0 + t] = MX_MFMA1(wx[g & 1][t], dx, acc[t0 + t], 1, sw[g & 1][t], sd);
+                if (i == 2) acc[t0 + t] = MX_MFMA1(wx[g & 1][t], dx, acc[t0 + t], 2, sw[g & 1][t], sd);
+                if (i == 3) acc[t0 + t] = MX_MFMA1(wx[g & 1][t], dx, acc[t0 + t], 3, sw[g & 1][t], sd);
+                if (u < SET) place((g + 1) % GROUPS, u);
+                else read((g + 2) % GROUPS, u - SET, g + 2 < GROUPS ? at : at_next);
+                // requests, the n-th slot of block i: the next stage's weights and the last block's digits in block 0, then the digits of block i - 1 of the next stage
+                constexpr int PER = 8 / RT;
+#pragma unroll
+                for (int k = 0; k < PER; ++k) {
+                    const int n = ((g % SETS) * SLOTS + u) * PER + k;
+                    if (i == 0 && n < 4) fetch_x(3, n, stage);
+                    if (i == 0 && n < PIECES) dma(n, next, buf ^ 1);
+                    if (i >= 1 && n < 4) fetch_x(i - 1, n, next);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        sx = sxn;
+    }
+}
+template <bool ID, int RT> __global__ void __launch_bounds__(512, 2) k_mx_wide(const mx_mm p, const int row_tiles) {
+    constexpr int ROWS = 32 * RT, PIECES = mx_wide_pieces<RT>();
+    static_assert(PIECES <= 9, "a lane's pieces leave their row once");
     extern __shared__ __align__(16) uint8_t lds[];  // two stages of [row] 272 bytes
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r32 = lane & 31, half = lane >> 5;
     int rt, tile;
@@ -750,128 +868,55 @@ template <bool ID, int RT> __global__ void __launch_bounds__(256, 1) k_mx_wide(c
         rt = at / n_tiles;
         if (rt >= row_tiles) return;
     }
-    const int row0 = rt * ROWS;
-    int e = 0, group = tile * 4 + wave, groups = (int) ((p.cols + 31) / 32);
+    const int row0 = min(rt * ROWS, p.n_rows - ROWS);  // (the last tile has some of the rows of the one before it, with the same result)
+    int e = 0, group = tile * 4 + (wave & 3), groups = (int) ((p.cols + 31) / 32);
     if (ID) {
         if (tile >= p.l.total[1]) return;
         const int32_t * t = p.l.tiles + 4 * tile;
         e = t[0];
-        group = t[1] + wave;
+        group = t[1] + (wave & 3);
         groups = t[1] + t[2];
     }
-    const bool live = group < groups;
-    const uint8_t * w = p.w + (int64_t) e * p.nb2 + (int64_t) row0 * p.nb1;
-    uint32_t wo[PIECES];  // the lane's pieces: 17 a row, in the order of LDS
-#pragma unroll
-    for (int n = 0; n < PIECES; ++n) {
-        const int c = n * 256 + tid, row = min(min(c / 17, ROWS - 1), p.n_rows - 1 - row0);
-        wo[n] = (uint32_t) row * (uint32_t) p.nb1 + (uint32_t) (c % 17) * 16u;
-    }
-    const uint32_t lds0 = (uint32_t) (uintptr_t) lds;
-    auto dma = [&](const int n, const int stage, const int buf) { mx_dma16(w + (int64_t) stage * 272, wo[n], lds0 + (uint32_t) (buf * STAGE + n * 4096 + wave * 1024)); };
-    const uint8_t * x = p.act + (int64_t) (live ? group : groups - 1) * p.steps * MX_ACT_STEP;
-    const uint32_t x16 = (uint32_t) (half * 2 * MX_ACT_STEP + r32 * 16), x8 = (uint32_t) (half * 2 * MX_ACT_STEP + r32 * 8), x4 = (uint32_t) (half * 2 * MX_ACT_STEP + r32 * 4);
-    mx_i4 h4[8], l4[8];
-    mx_i2 h2[8], l2[8];
-    uint32_t sx[2];
-    auto fetch_x = [&](const int i, const int what, const int stage) {
-        const uint8_t * xs = x + (int64_t) stage * (4 * MX_ACT_STEP) + (i / 4) * MX_ACT_STEP, * xb = xs + (i % 4) * MX_ACT_BLK;
-        if (what == 0) h4[i] = *(const mx_i4 *) (xb + x16);
-        if (what == 1) h2[i] = *(const mx_i2 *) (xb + 1024 + x8);
-        if (what == 2) l4[i] = *(const mx_i4 *) (xb + 512 + x16);
-        if (what == 3) l2[i] = *(const mx_i2 *) (xb + 1280 + x8);
-        if (what == 3 && i % 4 == 3) sx[i / 4] = *(const uint32_t *) (xs + 4 * MX_ACT_BLK + x4);
-    };
+    mx_wide_args<RT> q;
+    q.w = p.w + (int64_t) e * p.nb2 + (int64_t) row0 * p.nb1;
+    auto offset = [&](const int c) { return (uint32_t) (c / 17) * (uint32_t) p.nb1 + (uint32_t) (c % 17) * 16u; };
+    q.first = offset(tid);
+    q.last = offset(min((PIECES - 1) * 512 + tid, ROWS * 17 - 1));
+    q.piece = tid % 17;
+    q.jump = 30u * (uint32_t) p.nb1 + 32u;
+    q.wrap = (uint32_t) p.nb1 - 272u;
+    q.x = p.act + (int64_t) min(group, groups - 1) * p.steps * MX_ACT_STEP;
+    q.stages = p.steps / 4;
+    q.wave = wave;
+    q.lane = lane;
     mx_f16 acc[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
-    // The stream of groups (a block of each half row, SET tiles), GROUPS a stage: group g is multiplied, the codes of g + 1 are moved into place, those of g + 2 read.  An accumulator's next product
-    // comes SET instructions later, and what a product's time leaves room for stands behind it.  The one barrier of a stage lies ahead of its last two groups, which already read the next stage: all
-    // of this stage's reads are done by then, and the DMA of the next one, first thing in a stage, has landed.
-    constexpr int GROUPS = 8 * SETS, SLOTS = 2 * SET;
-    const int stages = p.steps / 4;
-    const uint8_t * own = lds + r32 * 272 + half * 136;
-    mx_i2 kept[RT];       // the unit between a tile's last block and its next
-    mx_i4 a[2][SET];      // the two units behind it
-    mx_i8 wx[2][SET];     // codes in place
-    int sw[2][SET];
-    auto read = [&](const int g, const int u, const uint8_t * at) {
-        typedef mx_i4 __attribute__((aligned(8))) mx_i4_a8;
-        a[g & 1][u] = *(const mx_i4_a8 *) (at + ((g % SETS) * SET + u) * (32 * 272) + 16 * (g / SETS) + 8);
-    };
-    auto place = [&](const int g, const int u) {
-        const int i = g / SETS, t = (g % SETS) * SET + u, k = (i + 1) / 4, sh8 = (i + 1) % 4;
-        const mx_i4 v = a[g & 1][u];
-        const int d[6] = {kept[t].x, kept[t].y, v.x, v.y, v.z, v.w};
-        mx_i4 c;
+    if (wave < 4) mx_wide_sum<RT, 0>(q, lds, acc);
+    else mx_wide_sum<RT, 1>(q, lds, acc);
+    // the two waves of a group: each passes one half of the tiles to the other and ends with the sum of the other half
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (no DMA under way, no stage read any more)
+    mx_f16 sum[RT / 2];
+    mx_f4 * give = (mx_f4 *) lds + (wave * (RT / 2) * 4) * 64 + lane, * take = (mx_f4 *) lds + ((wave ^ 4) * (RT / 2) * 4) * 64 + lane;
 #pragma unroll
-        for (int z = 0; z < 4; ++z) c[z] = sh8 ? (int) __builtin_amdgcn_alignbyte(d[k + z + (sh8 ? 1 : 0)], d[k + z], sh8) : d[k + z];
-        wx[g & 1][u] = mx_op4(c);
-        sw[g & 1][u] = d[i / 4];
-        kept[t] = mx_i2{v.z, v.w};
-    };
-    auto read_first = [&](const int t, const uint8_t * at) { kept[t] = *(const mx_i2 *) (at + t * (32 * 272)); };
+    for (int t = 0; t < RT / 2; ++t) {
+        sum[t] = wave < 4 ? acc[t] : acc[RT / 2 + t];
+        const mx_f16 other = wave < 4 ? acc[RT / 2 + t] : acc[t];
 #pragma unroll
-    for (int n = 0; n < PIECES; ++n) dma(n, 0, 0);
-#pragma unroll
-    for (int i = 0; i < 7; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            fetch_x(i, k, 0);
-            __builtin_amdgcn_sched_barrier(0);  // (in the order of the loop's: the compiler's counts of what is under way then hold for both)
-        }
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-#pragma unroll
-    for (int t = 0; t < RT; ++t) read_first(t, own);
-#pragma unroll
-    for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int u = 0; u < SET; ++u) {
-            read(g, u, own);
-            if (g == 0) place(0, u);
-        }
-    for (int stage = 0, buf = 0; stage < stages; ++stage, buf ^= 1) {
-        const int next = min(stage + 1, stages - 1);  // (behind the last stage: loads that nobody uses)
-        const uint8_t * at = own + buf * STAGE, * at_next = own + (buf ^ 1) * STAGE;
-#pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-            const int i = g / SETS, t0 = (g % SETS) * SET;
-            const mx_i8 hx = mx_op6(h4[i], h2[i]), lx = mx_op6(l4[i], l2[i]);
-            const uint32_t sh = sx[i / 4], sl = sh - 0x04040404u;
-            if (g == GROUPS - 2) asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (more than 16 requests of digits lie behind the last DMA)
-#pragma unroll
-            for (int u = 0; u < SLOTS; ++u) {
-                const int t = u % SET;
-                const mx_i8 dx = u < SET ? hx : lx;
-                const uint32_t sd = u < SET ? sh : sl;
-                if (i % 4 == 0) acc[t0 + t] = MX_MFMA1(wx[g & 1][t], dx, acc[t0 + t], 0, sw[g & 1][t], sd);
-                if (i % 4 == 1) acc[t0 + t] = MX_MFMA1(wx[g & 1][t], dx, acc[t0 + t], 1, sw[g & 1][t], sd);
-                if (i % 4 == 2) acc[t0 + t] = MX_MFMA1(wx[g & 1][t], dx, acc[t0 + t], 2, sw[g & 1][t], sd);
-                if (i % 4 == 3) acc[t0 + t] = MX_MFMA1(wx[g & 1][t], dx, acc[t0 + t], 3, sw[g & 1][t], sd);
-                if (u < SET) place((g + 1) % GROUPS, u);
-                else if (g + 2 < GROUPS) read(g + 2, u - SET, at);
-                else {
-                    if (g + 2 - GROUPS < SETS) read_first((g + 2 - GROUPS) * SET + u - SET, at_next);
-                    read(g + 2 - GROUPS, u - SET, at_next);
-                }
-                // requests, the n-th slot of block i: the next stage's weights and the last block's digits in block 0, then the digits of block i - 1 of the next stage
-                constexpr int PER = 8 / RT;
-#pragma unroll
-                for (int k = 0; k < PER; ++k) {
-                    const int n = ((g % SETS) * SLOTS + u) * PER + k;
-                    if (i == 0 && n < 4) fetch_x(7, n, stage);
-                    if (i == 0 && n < PIECES) dma(n, next, buf ^ 1);
-                    if (i == 1 && n == 0 && PIECES == 17) dma(16, next, buf ^ 1);
-                    if (i >= 1 && n >= 4 && n < 8) fetch_x(i - 1, n - 4, next);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
+        for (int i = 0; i < 4; ++i) give[(t * 4 + i) * 64] = mx_f4{other[4 * i], other[4 * i + 1], other[4 * i + 2], other[4 * i + 3]};
     }
-    if (!live) return;
-    mx_store_tile<ID, RT>(p, acc, group, row0, e, r32, half);
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < RT / 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const mx_f4 v = take[(t * 4 + i) * 64];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum[t][4 * i + k] += v[k];
+        }
+    if (group < groups) mx_store_tile<ID, RT / 2>(p, sum, group, row0 + (wave < 4 ? 0 : ROWS / 2), e, r32, half);
 }
 static mx_mm mx_args(const tdesc & w, const tdesc & d, int64_t cols) {
     mx_mm p{};
@@ -902,7 +947,7 @@ bool mx_id_vec_takes(int64_t K, int64_t cols) { return cols <= MX_VEC_ID_COLS &&
 // rows of whole steps, every one at a whole dword
 static bool mx_dwords(const mx_mm & p) { return p.blocks % 4 == 0 && p.nb1 % 4 == 0 && p.nb2 % 4 == 0 && ((uintptr_t) p.w & 3) == 0; }
 // ... of whole 16-byte pieces
-static bool mx_pieces(const mx_mm & p) { return p.blocks % 16 == 0 && p.nb1 % 16 == 0 && p.nb2 % 16 == 0 && ((uintptr_t) p.w & 15) == 0 && p.nb1 <= (1 << 24); }
+static bool mx_pieces(const mx_mm & p) { return p.blocks % 16 == 0 && p.nb1 % 16 == 0 && p.nb2 % 16 == 0 && ((uintptr_t) p.w & 15) == 0 && p.nb1 <= (1 << 22); }
 
 static void mx_launch_vec(hipStream_t s, const mx_mm & p, const tdesc & b, const tdesc * ids) {
     const int64_t K = b.ne[0];
@@ -917,11 +962,11 @@ static void mx_launch_vec(hipStream_t s, const mx_mm & p, const tdesc & b, const
 template <bool ID, int RT> static void mx_launch_tile_of(hipStream_t s, const mx_mm & p, int64_t col_tiles) {
     const int row_tiles = (p.n_rows + 32 * RT - 1) / (32 * RT);
     const dim3 grid((unsigned) ((row_tiles * col_tiles + 7) / 8 * 8));
-    if (mx_pieces(p)) {
-        constexpr size_t lds = 2 * mx_wide_pieces<RT>() * 4096;
+    if (mx_pieces(p) && p.n_rows >= 32 * RT) {
+        constexpr size_t lds = 2 * mx_wide_pieces<RT>() * 8192;
         static std::atomic<uint32_t> done{0};
         if (ensure_dyn_lds((const void *) k_mx_wide<ID, RT>, lds, done)) {
-            hipLaunchKernelGGL((k_mx_wide<ID, RT>), grid, dim3(256), lds, s, p, row_tiles);
+            hipLaunchKernelGGL((k_mx_wide<ID, RT>), grid, dim3(512), lds, s, p, row_tiles);
             return;
         }
     }

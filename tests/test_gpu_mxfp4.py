@@ -137,7 +137,7 @@ def test_read_outside_leaves_rows(backend):
 
 # ------------------------------------------------------------------------------------------ MUL_MAT
 SHAPES = [(32, 1, 1), (32, 33, 3), (64, 31, 2), (96, 129, 1), (128, 16, 16), (160, 64, 17), (224, 257, 33), (256, 100, 64), (2080, 1001, 5), (512, 300, 65), (1056, 70, 129),
-          (4096, 512, 1), (4096, 512, 4), (4096, 130, 31), (4096, 260, 32), (640, 515, 200), (14336, 96, 1), (14336, 40, 2), (1024, 1024, 300), (288, 640, 513)]
+          (4096, 512, 1), (4096, 512, 4), (4096, 130, 31), (4096, 260, 32), (640, 515, 200), (14336, 96, 1), (14336, 40, 2), (1024, 1024, 300), (288, 640, 513), (1536, 2050, 513), (2048, 6200, 1000)]
 
 
 def mul_mat(backend, w, x, K, N, M, **kw):
