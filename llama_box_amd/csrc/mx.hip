@@ -166,24 +166,35 @@ size_t mx_id_act_bytes(int64_t K, int64_t n_expert, int64_t cols) {
     return mx_lists_bytes(g) + mx_act_bytes(K, 32 * g);
 }
 static constexpr int MX_MAX_EXPERTS = 1024;
-// One workgroup an expert: every workgroup counts all experts' columns (whole numbers in LDS: no order to depend on), takes the groups in front of its own, and lists its columns in ascending order
-__global__ void __launch_bounds__(256) k_mx_group(const tdesc ids, const int n_expert, const mx_lists l) {
-    __shared__ int cnt[MX_MAX_EXPERTS], s_before[4], s_tiles[4], s_wave[4];
-    const int e = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int n_used = (int) ids.ne[0], n = n_used * (int) ids.ne[1];
-    auto id_at = [&](const int i) { return *(const int32_t *) (ids.data + (int64_t) (i % n_used) * ids.nb[0] + (int64_t) (i / n_used) * ids.nb[1]); };
-    for (int i = threadIdx.x; i < n_expert; i += 256) cnt[i] = 0;
+// One workgroup an expert: every workgroup counts all experts' columns (whole numbers in LDS: no order to depend on), takes the groups and tiles in front of its own, and lists its columns in ascending
+// order.  A round is MX_IDS ids a thread, requested at once (4000 ids of 32 experts: 15.7 us with one id a thread and round on 256 threads).
+static constexpr int MX_IDS = 4;
+__global__ void __launch_bounds__(1024) k_mx_group(const tdesc ids, const int n_expert, const mx_lists l) {
+    __shared__ int cnt[MX_MAX_EXPERTS], s_before[16], s_tiles[16], s_hits[MX_IDS * 16];
+    const int e = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t n_used = (uint32_t) ids.ne[0], n = n_used * (uint32_t) ids.ne[1];
+    int32_t id[MX_IDS];
+    auto fetch = [&](const uint32_t i0) {
+#pragma unroll
+        for (int k = 0; k < MX_IDS; ++k) {
+            const uint32_t i = i0 + (uint32_t) (k * 1024 + tid), t = i / n_used;
+            id[k] = i < n ? *(const int32_t *) (ids.data + (int64_t) (i - t * n_used) * ids.nb[0] + (int64_t) t * ids.nb[1]) : -1;
+        }
+    };
+    fetch(0);
+    if (tid < n_expert) cnt[tid] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const int v = id_at(i);
-        if (v >= 0 && v < n_expert) atomicAdd(&cnt[v], 1);
+    for (uint32_t i0 = 0; i0 < n; i0 += MX_IDS * 1024) {
+        if (i0) fetch(i0);
+#pragma unroll
+        for (int k = 0; k < MX_IDS; ++k)
+            if (id[k] >= 0 && id[k] < n_expert) atomicAdd(&cnt[id[k]], 1);
     }
     __syncthreads();
     int before = 0, before_t = 0;
-    for (int i = threadIdx.x; i < e; i += 256) {
-        const int gi = (cnt[i] + 31) / 32;
-        before += gi;
-        before_t += (gi + MX_TILE - 1) / MX_TILE;
+    if (tid < e) {
+        before = (cnt[tid] + 31) / 32;
+        before_t = (before + MX_TILE - 1) / MX_TILE;
     }
     for (int o = 32; o > 0; o >>= 1) {
         before += __shfl_xor(before, o, 64);
@@ -194,97 +205,151 @@ __global__ void __launch_bounds__(256) k_mx_group(const tdesc ids, const int n_e
         s_tiles[wave] = before_t;
     }
     __syncthreads();
-    const int g0 = s_before[0] + s_before[1] + s_before[2] + s_before[3], t0 = s_tiles[0] + s_tiles[1] + s_tiles[2] + s_tiles[3];
+    int g0 = 0, t0 = 0;
+    for (int w = 0; w < 16; ++w) {
+        g0 += s_before[w];
+        t0 += s_tiles[w];
+    }
     const int mine = cnt[e], groups = (mine + 31) / 32, tiles = (groups + MX_TILE - 1) / MX_TILE;
-    for (int i = threadIdx.x; i < tiles; i += 256) {
+    for (int i = tid; i < tiles; i += 1024) {
         int32_t * t = l.tiles + 4 * (t0 + i);
         t[0] = e;
         t[1] = g0 + MX_TILE * i;
         t[2] = min(MX_TILE, groups - MX_TILE * i);
     }
-    for (int i = threadIdx.x; i < groups; i += 256) l.owner[g0 + i] = e;
-    for (int i = mine + (int) threadIdx.x; i < groups * 32; i += 256) l.list[g0 * 32 + i] = -1;
-    if (e == n_expert - 1 && threadIdx.x == 0) {
+    for (int i = tid; i < groups; i += 1024) l.owner[g0 + i] = e;
+    for (int i = mine + tid; i < groups * 32; i += 1024) l.list[g0 * 32 + i] = -1;
+    if (e == n_expert - 1 && tid == 0) {
         l.total[0] = g0 + groups;
         l.total[1] = t0 + tiles;
     }
-    int placed = 0;
-    for (int i0 = 0; i0 < n; i0 += 256) {
-        const int i = i0 + (int) threadIdx.x;
-        const bool hit = i < n && id_at(i) == e;
-        const uint64_t bal = __ballot(hit);
+    if (mine == 0) return;
+    int placed = g0 * 32;
+    for (uint32_t i0 = 0; i0 < n; i0 += MX_IDS * 1024) {
+        if (n > MX_IDS * 1024) fetch(i0);  // (else they are still at hand)
+        uint64_t hit[MX_IDS];
+#pragma unroll
+        for (int k = 0; k < MX_IDS; ++k) hit[k] = __ballot(id[k] == e);
         __syncthreads();
-        if (lane == 0) s_wave[wave] = __popcll(bal);
+#pragma unroll
+        for (int k = 0; k < MX_IDS; ++k)
+            if (lane == 0) s_hits[k * 16 + wave] = __popcll(hit[k]);
         __syncthreads();
-        int off = placed + __popcll(bal & ((1ull << lane) - 1ull));
-        for (int w = 0; w < wave; ++w) off += s_wave[w];
-        if (hit) l.list[g0 * 32 + off] = i;
-        placed += s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3];
+        int sum = s_hits[lane];  // (64 counts in the order of the columns: an inclusive sum over them)
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(sum, o, 64);
+            if (lane >= o) sum += v;
+        }
+#pragma unroll
+        for (int k = 0; k < MX_IDS; ++k) {
+            const int at = __shfl(sum, k * 16 + wave, 64) - __popcll(hit[k]);
+            if (id[k] == e) l.list[placed + at + __popcll(hit[k] & ((1ull << lane) - 1ull))] = (int32_t) (i0 + (uint32_t) (k * 1024 + tid));
+        }
+        placed += __shfl(sum, 63, 64);
     }
 }
 
-// the lane's four values as codes: 24 bits of h and of l in the order of places, and the block's scale byte
+// whole numbers and step of a block: q = v f rounded, f = 2^-s, s the exponent of the block's largest magnitude (its bits: top), rounded to 8 significant bits, - 7; -> the scale byte of h
+__device__ __forceinline__ uint32_t mx_step(const uint32_t top, float & f) {
+    const int s = min(max((int) ((top + 0x8000u) >> 23) - 134, -120), 120);
+    f = top >= 0x7F800000u ? 0.0f : __uint_as_float((uint32_t) (127 - s) << 23);
+    return top >= 0x7F800000u ? 255u : (uint32_t) (s + 134);
+}
+// one value's digits: 6 bits of h, of l
+__device__ __forceinline__ void mx_digits(const float v, const float f, uint32_t & h, uint32_t & l) {
+    const float q = rintf(v * f);
+    const uint32_t m = min((uint32_t) fabsf(q), 255u), sign = (__float_as_uint(q) >> 26) & 32u;
+    h = (m >> 4) | sign;
+    l = (m & 15) | sign;
+}
+// the lane's four values (eight lanes a block) as codes: 24 bits of h and of l in the order of places, and the block's scale byte
 __device__ __forceinline__ uint32_t mx_act4(const float (&v)[4], uint32_t & h, uint32_t & l) {
-    const uint32_t top = mx_top(v);
+    float f;
+    const uint32_t e = mx_step(mx_top(v), f);
     h = l = 0;
-    if (top >= 0x7F800000u) return 255u;
-    const int s = min(max((int) ((top + 0x8000u) >> 23) - 134, -120), 120);  // (exponent of the largest, rounded to 8 significant bits, - 7)
-    const float f = __uint_as_float((uint32_t) (127 - s) << 23);
+    if (e == 255u) return e;  // (0 f is NaN for an infinity: the digits do not matter beside this scale, but they are numbers)
     constexpr int place[4] = {0, 2, 1, 3};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const float q = rintf(v[k] * f);
-        const uint32_t m = min((uint32_t) fabsf(q), 255u), sign = (__float_as_uint(q) >> 26) & 32u;
-        h |= ((m >> 4) | sign) << (6 * place[k]);
-        l |= ((m & 15) | sign) << (6 * place[k]);
+        uint32_t a, b;
+        mx_digits(v[k], f, a, b);
+        h |= a << (6 * place[k]);
+        l |= b << (6 * place[k]);
     }
-    return (uint32_t) (s + 134);
+    return e;
 }
-// One workgroup a group of columns and a step of 128 values; eight lanes a block, eight columns at a time.  ID: column c of the list is row (c % n_used) % b.ne[1] of token c / n_used
+// One workgroup a group of columns and a step of 128 values.  Four lanes a block: lane i has the values 4i .. 4i + 3 and 16 + 4i .. 16 + 4i + 3, places 8i .. 8i + 7, 48 bits of h and of l; a pair of lanes
+// has three dwords of each.  The 6272 bytes are put together in LDS and leave in 16-byte pieces.  ID: column c of the list is row (c % n_used) % b.ne[1] of token c / n_used
+typedef mx_f4 __attribute__((aligned(4))) mx_f4_a4;
 template <bool ID> __global__ void __launch_bounds__(256) k_mx_act(const tdesc b, const int64_t n_cols, const mx_lists l, const int n_used, uint8_t * __restrict__ act, const int steps) {
-    const int step = blockIdx.x, group = blockIdx.y;
+    __shared__ __align__(16) uint8_t s[MX_ACT_STEP];
+    const int step = blockIdx.x, group = blockIdx.y, tid = threadIdx.x;
     if (ID && group >= l.total[0]) return;
-    const int i = threadIdx.x & 7, blk = (threadIdx.x >> 3) & 3, lane = threadIdx.x & 63;
+    const int i = tid & 3, blk = (tid >> 2) & 3;
     const int64_t k0 = (int64_t) step * 128 + blk * 32;
-    uint8_t * out = act + ((int64_t) group * steps + step) * MX_ACT_STEP;
-    for (int c0 = 0; c0 < 32; c0 += 8) {
-        const int cg = c0 + (threadIdx.x >> 5);
-        int64_t c = (int64_t) group * 32 + cg;
+    mx_f4 v[2][2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        int c = group * 32 + r * 16 + (tid >> 4);
         const char * col;
         if (ID) {
             c = l.list[c];
-            col = b.data + ((c % n_used) % b.ne[1]) * b.nb[1] + (c / n_used) * b.nb[2];
+            col = b.data + ((c % n_used) % (int) b.ne[1]) * b.nb[1] + (int64_t) (c / n_used) * b.nb[2];
         } else {
+            const uint32_t n1 = (uint32_t) b.ne[1], n2 = (uint32_t) b.ne[2], c2 = (uint32_t) c / n1, c3 = c2 / n2;
+            col = b.data + (int64_t) ((uint32_t) c - c2 * n1) * b.nb[1] + (int64_t) (c2 - c3 * n2) * b.nb[2] + (int64_t) c3 * b.nb[3];
             if (c >= n_cols) c = -1;
-            col = b.data + (c % b.ne[1]) * b.nb[1] + ((c / b.ne[1]) % b.ne[2]) * b.nb[2] + (c / (b.ne[1] * b.ne[2])) * b.nb[3];
         }
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (c >= 0 && k0 < b.ne[0]) mx_load4((const float *) col + k0, i, v);
-        uint32_t h, lo;
-        const uint32_t e = mx_act4(v, h, lo);
-        // dword i (0 .. 5) of the 24 bytes: its bits start in the 24 of lane i + i / 3, at 8 (i % 3)
-        const int src = (lane & ~7) + i + i / 3, sh = 8 * (i % 3);
-        const uint32_t h0 = (uint32_t) __shfl((int) h, src & 63, 64), h1 = (uint32_t) __shfl((int) h, (src + 1) & 63, 64);
-        const uint32_t l0 = (uint32_t) __shfl((int) lo, src & 63, 64), l1 = (uint32_t) __shfl((int) lo, (src + 1) & 63, 64);
-        const uint32_t hw = (h0 >> sh) | (h1 << (24 - sh)), lw = (l0 >> sh) | (l1 << (24 - sh));
-        uint8_t * o = out + blk * MX_ACT_BLK;
-        if (i < 4) {
-            *(uint32_t *) (o + cg * 16 + 4 * i) = hw;
-            *(uint32_t *) (o + 512 + cg * 16 + 4 * i) = lw;
-        } else if (i < 6) {
-            *(uint32_t *) (o + 1024 + cg * 8 + 4 * (i - 4)) = hw;
-            *(uint32_t *) (o + 1280 + cg * 8 + 4 * (i - 4)) = lw;
-        } else if (i == 6) {
-            out[4 * MX_ACT_BLK + cg * 4 + blk] = (uint8_t) e;
+        v[r][0] = v[r][1] = mx_f4{0, 0, 0, 0};
+        if (c >= 0 && k0 < b.ne[0]) {
+            v[r][0] = *(const mx_f4_a4 *) (col + (k0 + 4 * i) * 4);
+            v[r][1] = *(const mx_f4_a4 *) (col + (k0 + 16 + 4 * i) * 4);
         }
     }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int cg = r * 16 + (tid >> 4);
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[r][k >> 2][k & 3]) & 0x7FFFFFFFu);
+        top = max(top, (uint32_t) dpp_i32<MI_DPP_QUAD_XOR1>((int) top));
+        top = max(top, (uint32_t) dpp_i32<MI_DPP_QUAD_XOR2>((int) top));
+        float f;
+        const uint32_t e = mx_step(top, f);
+        uint64_t h = 0, lo = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {  // place k: value k / 2 of the first four or of the second
+            uint32_t a, d;
+            mx_digits(v[r][k & 1][k >> 1], f, a, d);
+            h |= (uint64_t) a << (6 * k);
+            lo |= (uint64_t) d << (6 * k);
+        }
+        if (e == 255u) h = lo = 0;
+        // an even lane's six bytes and its neighbour's: dwords 0, 1 (its last two bytes and the neighbour's first two), 2 (the neighbour's other four)
+        const uint32_t hn = (uint32_t) dpp_i32<MI_DPP_QUAD_XOR1>((int) (uint32_t) h), ln = (uint32_t) dpp_i32<MI_DPP_QUAD_XOR1>((int) (uint32_t) lo);
+        uint8_t * o = s + blk * MX_ACT_BLK;
+        auto put = [&](const int d, const uint32_t hw, const uint32_t lw) {  // dword d of the 24 bytes
+            *(uint32_t *) (o + (d < 4 ? cg * 16 + 4 * d : 1024 + cg * 8 + 4 * (d - 4))) = hw;
+            *(uint32_t *) (o + (d < 4 ? 512 + cg * 16 + 4 * d : 1280 + cg * 8 + 4 * (d - 4))) = lw;
+        };
+        const int d0 = 3 * (i >> 1);
+        if (i & 1) put(d0 + 2, (uint32_t) (h >> 16), (uint32_t) (lo >> 16));
+        else {
+            put(d0, (uint32_t) h, (uint32_t) lo);
+            put(d0 + 1, (uint32_t) (h >> 32) | hn << 16, (uint32_t) (lo >> 32) | ln << 16);
+        }
+        if (i == 0) s[4 * MX_ACT_BLK + cg * 4 + blk] = (uint8_t) e;
+    }
+    __syncthreads();
+    uint8_t * out = act + ((int64_t) group * steps + step) * MX_ACT_STEP;
+    for (int at = tid; at < MX_ACT_STEP / 16; at += 256) ((mx_i4 *) out)[at] = ((const mx_i4 *) s)[at];
 }
 void launch_mx_act(hipStream_t s, const tdesc & b, void * act) {
     const int64_t cols = b.ne[1] * b.ne[2] * b.ne[3], steps = mx_steps(b.ne[0]);
     hipLaunchKernelGGL(k_mx_act<false>, dim3((unsigned) steps, (unsigned) ((cols + 31) / 32)), dim3(256), 0, s, b, cols, mx_lists{}, 1, (uint8_t *) act, (int) steps);
 }
 void launch_mx_group(hipStream_t s, const tdesc & ids, int64_t n_expert, void * ws) {
-    hipLaunchKernelGGL(k_mx_group, dim3((unsigned) n_expert), dim3(256), 0, s, ids, (int) n_expert, mx_lists_at(ws, mx_id_groups(n_expert, ids.ne[0] * ids.ne[1])));
+    hipLaunchKernelGGL(k_mx_group, dim3((unsigned) n_expert), dim3(1024), 0, s, ids, (int) n_expert, mx_lists_at(ws, mx_id_groups(n_expert, ids.ne[0] * ids.ne[1])));
 }
 void launch_mx_id_act(hipStream_t s, const tdesc & b, const tdesc & ids, int64_t n_expert, void * ws) {
     const int64_t cols = ids.ne[0] * ids.ne[1], steps = mx_steps(b.ne[0]), g = mx_id_groups(n_expert, cols);
@@ -558,6 +623,16 @@ template <bool ID, int CT, bool DW> __global__ void __launch_bounds__(512) k_mx_
     }
 }
 
+// Consecutive workgroups go to the eight dies in turn: each die has a run of tiles, four column tiles of a row tile after the other, then the next row tile's; the tiles that a die works on at a time
+// so share their digits and their weights in its L2
+__device__ __forceinline__ bool mx_tile_of(const mx_mm & p, const int row_tiles, int & rt, int & tile) {
+    const int n_tiles = (int) ((p.cols + 127) / 128), at = (int) (blockIdx.x & 7) * (int) (gridDim.x >> 3) + (int) (blockIdx.x >> 3);
+    const int band = at / (row_tiles * 4), in = at - band * row_tiles * 4, width = min(4, n_tiles - 4 * band);
+    if (width <= 0) return false;
+    rt = in / width;
+    tile = 4 * band + in - rt * width;
+    return rt < row_tiles;
+}
 // a wave's 32 RT rows by 32 columns to their places
 template <bool ID, int RT> __device__ __forceinline__ void mx_store_tile(const mx_mm & p, const mx_f16 (&acc)[RT], const int group, const int row0, const int e, const int r32, const int half) {
     constexpr int ROWS = 32 * RT;
@@ -596,11 +671,7 @@ template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, RT ==
         rt = blockIdx.x % row_tiles;
         tile = blockIdx.x / row_tiles;
     } else {
-        // consecutive workgroups go to the eight dies in turn: each die has a run of tiles, the column tiles of a row tile one after the other, so that the weights stay in its L2
-        const int n_tiles = (int) ((p.cols + 127) / 128), at = (int) (blockIdx.x & 7) * (int) (gridDim.x >> 3) + (int) (blockIdx.x >> 3);
-        tile = at % n_tiles;
-        rt = at / n_tiles;
-        if (rt >= row_tiles) return;
+        if (!mx_tile_of(p, row_tiles, rt, tile)) return;
     }
     const int row0 = rt * ROWS;
     int e = 0, group = tile * 4 + wave, groups = (int) ((p.cols + 31) / 32);
@@ -863,10 +934,7 @@ template <bool ID, int RT> __global__ void __launch_bounds__(512, 2) k_mx_wide(c
         rt = blockIdx.x % row_tiles;
         tile = blockIdx.x / row_tiles;
     } else {
-        const int n_tiles = (int) ((p.cols + 127) / 128), at = (int) (blockIdx.x & 7) * (int) (gridDim.x >> 3) + (int) (blockIdx.x >> 3);
-        tile = at % n_tiles;
-        rt = at / n_tiles;
-        if (rt >= row_tiles) return;
+        if (!mx_tile_of(p, row_tiles, rt, tile)) return;
     }
     const int row0 = min(rt * ROWS, p.n_rows - ROWS);  // (the last tile has some of the rows of the one before it, with the same result)
     int e = 0, group = tile * 4 + (wave & 3), groups = (int) ((p.cols + 31) / 32);
@@ -1013,7 +1081,7 @@ bool mx_product_ok(const tdesc & w, const tdesc & b) {
            (b.ne[1] * b.ne[2] * b.ne[3] + 31) / 32 <= 65535;
 }
 bool mx_id_ok(const tdesc & w, const tdesc & ids) {
-    return w.ne[2] <= MX_MAX_EXPERTS && ids.nb[0] % 4 == 0 && ids.nb[1] % 4 == 0 && ids.ne[0] * ids.ne[1] < ((int64_t) 1 << 30) && mx_id_groups(w.ne[2], ids.ne[0] * ids.ne[1]) <= 65535;
+    return w.ne[2] <= MX_MAX_EXPERTS && ids.nb[0] % 4 == 0 && ids.nb[1] % 4 == 0 && ids.ne[0] * ids.ne[1] < ((int64_t) 1 << 30) && ids.ne[0] > 0 && mx_id_groups(w.ne[2], ids.ne[0] * ids.ne[1]) <= 65535;
 }
 
 // ------------------------------------------------------------------------------------------------ ADD_ID
