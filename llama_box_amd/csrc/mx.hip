@@ -11,6 +11,10 @@
 #include "dev_util.h"
 #include "kernels.h"
 
+#ifndef MX_FEWI
+#define MX_FEWI 4
+#define MX_FEWD 8
+#endif
 #ifndef MX_SET
 #define MX_SET 1
 #endif
@@ -633,29 +637,41 @@ __device__ __forceinline__ bool mx_tile_of(const mx_mm & p, const int row_tiles,
     tile = 4 * band + in - rt * width;
     return rt < row_tiles;
 }
-// a wave's 32 RT rows by 32 columns to their places
-template <bool ID, int RT> __device__ __forceinline__ void mx_store_tile(const mx_mm & p, const mx_f16 (&acc)[RT], const int group, const int row0, const int e, const int r32, const int half) {
-    constexpr int ROWS = 32 * RT;
+// A wave's 32 RT rows by 32 columns to their places, by way of LDS of its own (mx_store_floats): a column's rows lie side by side there and leave in runs of 128 RT bytes, where a lane's own four would
+// go out 16 bytes here and there (1000 tokens of 32 experts, rows with a bias, four bytes at a time: 172 us)
+template <int RT> constexpr int mx_store_floats() { return 32 * (32 * RT + 4); }
+template <bool ID, int RT> __device__ __forceinline__ void mx_store_tile(const mx_mm & p, const mx_f16 (&acc)[RT], const int group, const int row0, const int e, const int lane, float * lds) {
+    constexpr int ROWS = 32 * RT, RUN = ROWS / 4, COLS = 64 / RUN;  // lanes of a column, columns at a time
+    const int r32 = lane & 31, half = lane >> 5, row = row0 + lane % RUN * 4;
     int64_t c = (int64_t) group * 32 + r32;
     if (ID) c = p.l.list[c];
-    if (c < 0 || (!ID && c >= p.cols)) return;
-    float * d = p.dst + c * p.ldd;
+    else if (c >= p.cols) c = -1;
     const float * bias = p.bias ? (const float *) ((const char *) p.bias + (int64_t) e * p.nb_bias) : nullptr;
-    const bool wide = ((((uintptr_t) d) | (uintptr_t) (p.ldd * 4)) & 15) == 0 && row0 + ROWS <= p.n_rows && !bias;
+    mx_f4 bv = {0, 0, 0, 0};
+    if (bias)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) bv[k] = bias[min(row + k, p.n_rows - 1)];
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = row0 + 32 * t + 8 * i + 4 * half;
-            if (wide) {
-                *(mx_f4 *) (d + row) = mx_f4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]};
-            } else {
+        for (int i = 0; i < 4; ++i) *(mx_f4 *) (lds + r32 * (ROWS + 4) + 32 * t + 8 * i + 4 * half) = mx_f4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]};
+    __builtin_amdgcn_wave_barrier();
+    const bool whole = ((((uintptr_t) p.dst) | (uintptr_t) (p.ldd * 4)) & 15) == 0;
+#pragma unroll 4
+    for (int c0 = 0; c0 < 32; c0 += COLS) {
+        const int cg = c0 + lane / RUN, to = __shfl((int) c, cg, 64);
+        mx_f4 v = *(const mx_f4 *) (lds + cg * (ROWS + 4) + lane % RUN * 4);
+        if (bias) v += bv;
+        if (to < 0) continue;
+        float * d = p.dst + to * p.ldd + row;
+        if (whole && row + 4 <= p.n_rows) *(mx_f4 *) d = v;
+        else
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (row + k < p.n_rows) d[row + k] = bias ? acc[t][4 * i + k] + bias[row + k] : acc[t][4 * i + k];
-            }
-        }
+            for (int k = 0; k < 4; ++k)
+                if (row + k < p.n_rows) d[k] = v[k];
+    }
 }
+
 // ---- many columns: 32 RT rows by four groups of columns a workgroup.  A wave has one group and all rows: its digits come straight from memory (no other wave reads them), the weights through LDS,
 // where their blocks are aligned ([block of the step][row] 16 bytes, and 4 scale bytes a row).  In a step of 128 values: the next step's digits are requested, the next step's weights (requested a step
 // ago) stored, the weights after those requested — one such item behind each product.  (Requested in a bunch in front of the products they hold up all four waves at once: 512 columns 62 us.)
@@ -663,8 +679,8 @@ template <bool ID, int RT> __device__ __forceinline__ void mx_store_tile(const m
 template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, RT == 8 ? 1 : 2) k_mx_tile(const mx_mm p, const int row_tiles) {
     constexpr int SET = RT < 4 ? RT : 4, SETS = RT / SET;
     constexpr int ROWS = 32 * RT, PLANE = ROWS * 16 + 64;  // (64: the four planes that a quad of lanes writes to lie on different banks)
-    __shared__ __align__(16) uint8_t s_w[2][4 * PLANE];
-    __shared__ __align__(16) uint8_t s_s[2][ROWS * 4];
+    constexpr int STAGE = 4 * PLANE + ROWS * 4, OUT = 4 * 4 * mx_store_floats<(RT < 4 ? RT : 4)>();
+    __shared__ __align__(16) uint8_t lds[2 * STAGE > OUT ? 2 * STAGE : OUT];  // two stages: the planes, their scales
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r32 = lane & 31, half = lane >> 5;
     int rt, tile;
     if (ID) {
@@ -710,8 +726,8 @@ template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, RT ==
         const uint32_t sh = DW ? (uint32_t) q : wsh[i];
         const int next = __builtin_amdgcn_update_dpp(0, wr[i].x, 0xF9, 0xF, 0xF, true);  // (the first dword of the quad's next lane: quad_perm 1, 2, 3, 3)
         const int d = !DW || q == 3 ? wd[i] : next;
-        *(mx_i4 *) (s_w[buf] + q * PLANE + (lrow + 64 * i) * 16) = mx_window(wr[i], d, sh);
-        s_s[buf][(lrow + 64 * i) * 4 + q] = (uint8_t) ((uint32_t) wr[i].x >> (8 * sh));
+        *(mx_i4 *) (lds + buf * STAGE + q * PLANE + (lrow + 64 * i) * 16) = mx_window(wr[i], d, sh);
+        lds[buf * STAGE + 4 * PLANE + (lrow + 64 * i) * 4 + q] = (uint8_t) ((uint32_t) wr[i].x >> (8 * sh));
     };
     const uint8_t * x = p.act + (int64_t) (live ? group : groups - 1) * p.steps * MX_ACT_STEP;
     const uint32_t x16 = (uint32_t) (half * MX_ACT_BLK + r32 * 16), x8 = (uint32_t) (half * MX_ACT_BLK + r32 * 8);
@@ -760,8 +776,8 @@ template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, RT ==
             const int j = g / SETS, t0 = (g % SETS) * SET;
 #pragma unroll
             for (int u = 0; u < SET; ++u) {
-                a[g & 1][u] = *(const mx_i4 *) (s_w[buf] + (2 * j + half) * PLANE + (32 * (t0 + u) + r32) * 16);
-                sw[g & 1][u] = (int) (*(const uint32_t *) (s_s[buf] + (32 * (t0 + u) + r32) * 4) >> (8 * half));
+                a[g & 1][u] = *(const mx_i4 *) (lds + buf * STAGE + (2 * j + half) * PLANE + (32 * (t0 + u) + r32) * 16);
+                sw[g & 1][u] = (int) (*(const uint32_t *) (lds + buf * STAGE + 4 * PLANE + (32 * (t0 + u) + r32) * 4) >> (8 * half));
             }
         };
         read(0);
@@ -799,7 +815,17 @@ template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, RT ==
         __syncthreads();
     }
     if (!live) return;
-    mx_store_tile<ID, RT>(p, acc, group, row0, e, r32, half);
+    // (behind the loop's last barrier: nobody reads the stages any more)
+    constexpr int PART = RT < 4 ? RT : 4;
+    float * out = (float *) lds + wave * mx_store_floats<PART>();
+#pragma unroll
+    for (int t0 = 0; t0 < RT; t0 += PART) {
+        mx_f16 part[PART];
+#pragma unroll
+        for (int t = 0; t < PART; ++t) part[t] = acc[t0 + t];
+        mx_store_tile<ID, PART>(p, part, group, row0 + 32 * t0, e, lane, out);
+        __builtin_amdgcn_wave_barrier();
+    }
 }
 // ---- many columns of rows that are whole 16-byte pieces (K a multiple of 512: 272 bytes): as k_mx_tile, but the weights go to LDS by DMA as they lie in memory, 512 values a stage and row by row, and a
 // lane moves its codes into place behind its LDS read.  Eight waves: a group of columns has two, which take the even and the odd quarters of a row's stage (68 bytes, four blocks each) and add up at the
@@ -928,7 +954,7 @@ template <bool ID, int RT> __global__ void __launch_bounds__(512, 2) k_mx_wide(c
     constexpr int ROWS = 32 * RT, PIECES = mx_wide_pieces<RT>();
     static_assert(PIECES <= 9, "a lane's pieces leave their row once");
     extern __shared__ __align__(16) uint8_t lds[];  // two stages of [row] 272 bytes
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r32 = lane & 31, half = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int rt, tile;
     if (ID) {
         rt = blockIdx.x % row_tiles;
@@ -984,7 +1010,8 @@ template <bool ID, int RT> __global__ void __launch_bounds__(512, 2) k_mx_wide(c
 #pragma unroll
             for (int k = 0; k < 4; ++k) sum[t][4 * i + k] += v[k];
         }
-    if (group < groups) mx_store_tile<ID, RT / 2>(p, sum, group, row0 + (wave < 4 ? 0 : ROWS / 2), e, r32, half);
+    __syncthreads();
+    if (group < groups) mx_store_tile<ID, RT / 2>(p, sum, group, row0 + (wave < 4 ? 0 : ROWS / 2), e, lane, (float *) lds + wave * mx_store_floats<RT / 2>());
 }
 static mx_mm mx_args(const tdesc & w, const tdesc & d, int64_t cols) {
     mx_mm p{};
@@ -1031,7 +1058,7 @@ template <bool ID, int RT> static void mx_launch_tile_of(hipStream_t s, const mx
     const int row_tiles = (p.n_rows + 32 * RT - 1) / (32 * RT);
     const dim3 grid((unsigned) ((row_tiles * col_tiles + 7) / 8 * 8));
     if (mx_pieces(p) && p.n_rows >= 32 * RT) {
-        constexpr size_t lds = 2 * mx_wide_pieces<RT>() * 8192;
+        constexpr size_t lds = std::max<size_t>(2 * mx_wide_pieces<RT>() * 8192, 8 * 4 * mx_store_floats<RT / 2>());
         static std::atomic<uint32_t> done{0};
         if (ensure_dyn_lds((const void *) k_mx_wide<ID, RT>, lds, done)) {
             hipLaunchKernelGGL((k_mx_wide<ID, RT>), grid, dim3(512), lds, s, p, row_tiles);
@@ -1059,7 +1086,7 @@ void launch_mx_mul_mat(hipStream_t s, const tdesc & w, const tdesc & b, const td
     p.act = (const uint8_t *) act;
     if (p.n_rows == 0 || p.cols == 0) return;
     if (!act) mx_launch_vec(s, p, b, nullptr);
-    else if (p.cols <= 32) mx_launch_few<false, 1>(s, p, 1, 8);
+    else if (p.cols <= 32) mx_launch_few<false, 1>(s, p, 1, MX_FEWD);
     else if (p.cols <= MX_FEW_COLS) mx_launch_few<false, 2>(s, p, 1, 4);
     else mx_launch_tile<false>(s, p, (p.cols + 127) / 128);
 }
@@ -1072,7 +1099,7 @@ void launch_mx_mul_mat_id(hipStream_t s, const tdesc & w, const tdesc & b, const
     if (!ws) return mx_launch_vec(s, p, b, &ids);
     p.act = (const uint8_t *) ws + mx_lists_bytes(g);
     p.l = mx_lists_at((void *) ws, g);
-    if (cols <= 32 * w.ne[2]) mx_launch_few<true, 1>(s, p, g, 8);
+    if (cols <= 32 * w.ne[2]) mx_launch_few<true, 1>(s, p, g, MX_FEWI);
     else mx_launch_tile<true>(s, p, mx_id_tiles(w.ne[2], cols));
 }
 // which operands the products take (type and shape; the rows of both are dense, whole blocks)
