@@ -11,9 +11,8 @@
 #include "dev_util.h"
 #include "kernels.h"
 
-#ifndef MX_FEWI
-#define MX_FEWI 4
-#define MX_FEWD 8
+#ifndef MX_VOCC
+#define MX_VOCC 3
 #endif
 #ifndef MX_SET
 #define MX_SET 1
@@ -266,25 +265,37 @@ __device__ __forceinline__ void mx_digits(const float v, const float f, uint32_t
     h = (m >> 4) | sign;
     l = (m & 15) | sign;
 }
-// the lane's four values (eight lanes a block) as codes: 24 bits of h and of l in the order of places, and the block's scale byte
-__device__ __forceinline__ uint32_t mx_act4(const float (&v)[4], uint32_t & h, uint32_t & l) {
-    float f;
-    const uint32_t e = mx_step(mx_top(v), f);
-    h = l = 0;
-    if (e == 255u) return e;  // (0 f is NaN for an infinity: the digits do not matter beside this scale, but they are numbers)
-    constexpr int place[4] = {0, 2, 1, 3};
+// Four lanes a block: lane i has the values 4i .. 4i + 3 (v[0]) and 16 + 4i .. 16 + 4i + 3 (v[1]), places 8i .. 8i + 7, 48 bits of h and of l; a pair of lanes has three dwords of each, put(d, ..) is given
+// dword d of the block's six.  -> the scale byte
+typedef mx_f4 __attribute__((aligned(4))) mx_f4_a4;
+template <class Put> __device__ __forceinline__ uint32_t mx_act_quad(const mx_f4 (&v)[2], const int i, Put && put) {
+    uint32_t top = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k >> 2][k & 3]) & 0x7FFFFFFFu);
+    top = max(top, (uint32_t) dpp_i32<MI_DPP_QUAD_XOR1>((int) top));
+    top = max(top, (uint32_t) dpp_i32<MI_DPP_QUAD_XOR2>((int) top));
+    float f;
+    const uint32_t e = mx_step(top, f);
+    uint64_t h = 0, l = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {  // place k: value k / 2 of the first four or of the second
         uint32_t a, b;
-        mx_digits(v[k], f, a, b);
-        h |= a << (6 * place[k]);
-        l |= b << (6 * place[k]);
+        mx_digits(v[k & 1][k >> 1], f, a, b);
+        h |= (uint64_t) a << (6 * k);
+        l |= (uint64_t) b << (6 * k);
+    }
+    if (e == 255u) h = l = 0;  // (0 f is NaN for an infinity: the digits do not matter beside this scale, but they are numbers)
+    // an even lane's six bytes and its neighbour's: dwords 0, 1 (its last two bytes and the neighbour's first two), 2 (the neighbour's other four)
+    const uint32_t hn = (uint32_t) dpp_i32<MI_DPP_QUAD_XOR1>((int) (uint32_t) h), ln = (uint32_t) dpp_i32<MI_DPP_QUAD_XOR1>((int) (uint32_t) l);
+    const int d = 3 * (i >> 1);
+    if (i & 1) put(d + 2, (uint32_t) (h >> 16), (uint32_t) (l >> 16));
+    else {
+        put(d, (uint32_t) h, (uint32_t) l);
+        put(d + 1, (uint32_t) (h >> 32) | hn << 16, (uint32_t) (l >> 32) | ln << 16);
     }
     return e;
 }
-// One workgroup a group of columns and a step of 128 values.  Four lanes a block: lane i has the values 4i .. 4i + 3 and 16 + 4i .. 16 + 4i + 3, places 8i .. 8i + 7, 48 bits of h and of l; a pair of lanes
-// has three dwords of each.  The 6272 bytes are put together in LDS and leave in 16-byte pieces.  ID: column c of the list is row (c % n_used) % b.ne[1] of token c / n_used
-typedef mx_f4 __attribute__((aligned(4))) mx_f4_a4;
+// One workgroup a group of columns and a step of 128 values.  The 6272 bytes are put together in LDS and leave in 16-byte pieces.  ID: column c of the list is row (c % n_used) % b.ne[1] of token c / n_used
 template <bool ID> __global__ void __launch_bounds__(256) k_mx_act(const tdesc b, const int64_t n_cols, const mx_lists l, const int n_used, uint8_t * __restrict__ act, const int steps) {
     __shared__ __align__(16) uint8_t s[MX_ACT_STEP];
     const int step = blockIdx.x, group = blockIdx.y, tid = threadIdx.x;
@@ -313,35 +324,11 @@ template <bool ID> __global__ void __launch_bounds__(256) k_mx_act(const tdesc b
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         const int cg = r * 16 + (tid >> 4);
-        uint32_t top = 0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[r][k >> 2][k & 3]) & 0x7FFFFFFFu);
-        top = max(top, (uint32_t) dpp_i32<MI_DPP_QUAD_XOR1>((int) top));
-        top = max(top, (uint32_t) dpp_i32<MI_DPP_QUAD_XOR2>((int) top));
-        float f;
-        const uint32_t e = mx_step(top, f);
-        uint64_t h = 0, lo = 0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {  // place k: value k / 2 of the first four or of the second
-            uint32_t a, d;
-            mx_digits(v[r][k & 1][k >> 1], f, a, d);
-            h |= (uint64_t) a << (6 * k);
-            lo |= (uint64_t) d << (6 * k);
-        }
-        if (e == 255u) h = lo = 0;
-        // an even lane's six bytes and its neighbour's: dwords 0, 1 (its last two bytes and the neighbour's first two), 2 (the neighbour's other four)
-        const uint32_t hn = (uint32_t) dpp_i32<MI_DPP_QUAD_XOR1>((int) (uint32_t) h), ln = (uint32_t) dpp_i32<MI_DPP_QUAD_XOR1>((int) (uint32_t) lo);
         uint8_t * o = s + blk * MX_ACT_BLK;
-        auto put = [&](const int d, const uint32_t hw, const uint32_t lw) {  // dword d of the 24 bytes
-            *(uint32_t *) (o + (d < 4 ? cg * 16 + 4 * d : 1024 + cg * 8 + 4 * (d - 4))) = hw;
-            *(uint32_t *) (o + (d < 4 ? 512 + cg * 16 + 4 * d : 1280 + cg * 8 + 4 * (d - 4))) = lw;
-        };
-        const int d0 = 3 * (i >> 1);
-        if (i & 1) put(d0 + 2, (uint32_t) (h >> 16), (uint32_t) (lo >> 16));
-        else {
-            put(d0, (uint32_t) h, (uint32_t) lo);
-            put(d0 + 1, (uint32_t) (h >> 32) | hn << 16, (uint32_t) (lo >> 32) | ln << 16);
-        }
+        const uint32_t e = mx_act_quad(v[r], i, [&](const int d, const uint32_t h, const uint32_t lo) {
+            *(uint32_t *) (o + (d < 4 ? cg * 16 + 4 * d : 1024 + cg * 8 + 4 * (d - 4))) = h;
+            *(uint32_t *) (o + (d < 4 ? 512 + cg * 16 + 4 * d : 1280 + cg * 8 + 4 * (d - 4))) = lo;
+        });
         if (i == 0) s[4 * MX_ACT_BLK + cg * 4 + blk] = (uint8_t) e;
     }
     __syncthreads();
@@ -382,7 +369,6 @@ __device__ __forceinline__ mx_i8 mx_op6(const mx_i4 a, const mx_i2 b) { return m
 // bytes come as 17 dwords and the codes are moved into place (GB/s over rows of 2176 bytes: 16 bytes at 17 b + 1 and a byte at 17 b 2335, the dwords around a block 4750, 17 dwords a lane 6960,
 // aligned 16-byte loads of something else 7500).  A scale byte stays where it is, byte j of its dword: the instruction picks it.
 // DW: rows of whole steps at whole dwords (K a multiple of 128); otherwise block by block, the dwords around each (none of them without a byte of the block).
-struct mx_w4 { mx_i4 a[4]; int s[4]; };  // codes of four blocks; dwords whose byte j is the scale of block j
 template <bool DW> struct mx_raw;
 template <> struct mx_raw<true> {
     mx_i4 v[4];
@@ -393,16 +379,11 @@ template <> struct mx_raw<true> {
         for (int i = 0; i < 4; ++i) v[i] = *(const mx_i4_a4 *) (p + 16 * i);
         d = *(const int *) (p + 64);
     }
-    __device__ __forceinline__ void place(mx_w4 & w) const {
+    __device__ __forceinline__ void place(const int j, mx_i4 & a, int & s) const {  // block j's codes; a dword whose byte j is its scale
         const int q[17] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w, v[2].x, v[2].y, v[2].z, v[2].w, v[3].x, v[3].y, v[3].z, v[3].w, d};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            w.a[0][i] = __builtin_amdgcn_alignbyte(q[i + 1], q[i], 1);
-            w.a[1][i] = __builtin_amdgcn_alignbyte(q[i + 5], q[i + 4], 2);
-            w.a[2][i] = __builtin_amdgcn_alignbyte(q[i + 9], q[i + 8], 3);
-            w.a[3][i] = q[i + 13];
-            w.s[i] = q[4 * i];
-        }
+        for (int i = 0; i < 4; ++i) a[i] = j == 3 ? q[i + 13] : (int) __builtin_amdgcn_alignbyte(q[4 * j + i + 1], q[4 * j + i], j + 1);
+        s = q[4 * j];
     }
 };
 // a block's codes out of the five dwords around it, sh the first one's bytes in front of the block
@@ -425,28 +406,25 @@ template <> struct mx_raw<false> {
             d[j] = *(const int *) (q + 16);
         }
     }
-    __device__ __forceinline__ void place(mx_w4 & w) const {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            w.a[j] = mx_window(v[j], d[j], sh[j]);
-            w.s[j] = (int) ((((uint32_t) v[j].x >> (8 * sh[j])) & 255u) << (8 * j));
-        }
+    __device__ __forceinline__ void place(const int j, mx_i4 & a, int & s) const {
+        a = mx_window(v[j], d[j], sh[j]);
+        s = (int) ((((uint32_t) v[j].x >> (8 * sh[j])) & 255u) << (8 * j));
     }
 };
-// acc += one block: w's block J by the digits h, l, whose scale bytes are byte J of sh, sl
-#define MX_MFMA(N, ACC, W, J, H, L, SH, SL)                                                                                                         \
-    ACC = __builtin_amdgcn_mfma_scale_f32_##N##_f8f6f4(mx_op4((W).a[J]), H, ACC, MX_FP4, MX_FP6, J, (W).s[J], J, (int) (SH));                     \
-    ACC = __builtin_amdgcn_mfma_scale_f32_##N##_f8f6f4(mx_op4((W).a[J]), L, ACC, MX_FP4, MX_FP6, J, (W).s[J], J, (int) (SL));
+// acc += one block: the codes A by the digits H, L; the scales are the bytes J of S, of SH and SL
+#define MX_MFMA(N, ACC, A, S, J, H, L, SH, SL)                                                                                 \
+    ACC = __builtin_amdgcn_mfma_scale_f32_##N##_f8f6f4(mx_op4(A), H, ACC, MX_FP4, MX_FP6, J, S, J, (int) (SH));              \
+    ACC = __builtin_amdgcn_mfma_scale_f32_##N##_f8f6f4(mx_op4(A), L, ACC, MX_FP4, MX_FP6, J, S, J, (int) (SL));
 
 // ---- one to a few columns: 16 rows a workgroup, its waves take four steps of 128 values in turn.  The workgroup quantises its columns itself, while its first weights are on the way: a launch in front
 // costs more.  A lane of v_mfma_scale_f32_16x16x128: row (column) lane % 16, step lane / 16 of the four.
 // ID: blockIdx.y is a column (u + n_used t) of at most 64; the first column of an expert takes all of its expert, the others' workgroups end at once.
-static constexpr int MX_VEC_REC = 48;     // LDS bytes of a block of one column: 16 of h, 16 of l, 8 of h, 8 of l
-template <bool ID, bool DW> __global__ void __launch_bounds__(512) k_mx_vec(const mx_mm p, const tdesc b, const tdesc ids, const int chunk) {
+static constexpr int MX_VEC_REC = 48;     // LDS bytes of a block of one column: 24 of h, 24 of l
+template <bool ID, bool DW> __global__ void __launch_bounds__(512, DW ? MX_VOCC : 2) k_mx_vec(const mx_mm p, const tdesc b, const tdesc ids, const int chunk) {
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ int s_cols[64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, r16 = lane & 15, q = lane >> 4;
-    const int row0 = (int) blockIdx.x * 16, blocks4 = p.steps * 4;
+    const int row0 = (int) blockIdx.x * 16, all = (p.steps + 3) / 4 * 16;  // blocks of a column, with those behind its last that the last turn takes (zeros)
     int e = 0, n = (int) p.cols;
     if (ID) {
         const int n_used = (int) ids.ne[0], slot = blockIdx.y;
@@ -459,8 +437,8 @@ template <bool ID, bool DW> __global__ void __launch_bounds__(512) k_mx_vec(cons
         if (wave == 0 && id == e) s_cols[__popcll(mine & ((1ull << lane) - 1ull))] = lane;
     }
     const uint8_t * w = p.w + (int64_t) e * p.nb2 + (int64_t) min(row0 + r16, p.n_rows - 1) * p.nb1;
-    uint8_t * s_rec = lds, * s_scale = lds + (size_t) chunk * blocks4 * MX_VEC_REC;  // [block][column of the chunk]; [step][column][block] scale bytes
-    float * s_part = (float *) (lds + (size_t) chunk * blocks4 * (MX_VEC_REC + 1));  // [wave][column][row]
+    uint8_t * s_rec = lds, * s_scale = lds + (size_t) chunk * all * MX_VEC_REC;  // [block][column of the chunk]; [step][column][block] scale bytes
+    float * s_part = (float *) (lds + (size_t) chunk * all * (MX_VEC_REC + 1));  // [wave][column][row]
     const float * bias = p.bias ? (const float *) ((const char *) p.bias + (int64_t) e * p.nb_bias) : nullptr;
     for (int c0 = 0; c0 < n; c0 += chunk) {
         const int m = min(chunk, n - c0);
@@ -468,9 +446,9 @@ template <bool ID, bool DW> __global__ void __launch_bounds__(512) k_mx_vec(cons
         const int last = p.steps - 1, stride = 4 * waves;
         int step = wave * 4 + q;  // (behind the last step: its weights again, and digits of zero)
         f0.load(w, min(step, last), p.blocks);
-        f1.load(w, min(step + stride, last), p.blocks);
+        if (wave * 4 + stride < p.steps) f1.load(w, min(step + stride, last), p.blocks);
         if (ID || c0) __syncthreads();  // (the columns' list; the last chunk's partial sums and digits are read)
-        const int i = threadIdx.x & 7, per = (int) blockDim.x >> 3;  // eight lanes a block
+        const int i = threadIdx.x & 3, per = (int) blockDim.x >> 2;  // four lanes a block
         for (int c = 0; c < m; ++c) {
             const char * col;
             if (ID) {
@@ -480,60 +458,54 @@ template <bool ID, bool DW> __global__ void __launch_bounds__(512) k_mx_vec(cons
                 const int cc = c0 + c, n1 = (int) b.ne[1], n2 = (int) b.ne[2];
                 col = b.data + (cc % n1) * b.nb[1] + (int64_t) ((cc / n1) % n2) * b.nb[2] + (int64_t) (cc / (n1 * n2)) * b.nb[3];
             }
-            for (int blk0 = threadIdx.x >> 3; blk0 < blocks4; blk0 += 4 * per) {
-                float v[4][4];
+            for (int blk0 = threadIdx.x >> 2; blk0 < all; blk0 += 2 * per) {
+                mx_f4 v[2][2];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mx_load4((const float *) col + min(blk0 + k * per, p.blocks - 1) * 32, i, v[k]);
+                for (int k = 0; k < 2; ++k) {
+                    const char * at = col + (min(blk0 + k * per, p.blocks - 1) * 32 + 4 * i) * 4;
+                    v[k][0] = *(const mx_f4_a4 *) at;
+                    v[k][1] = *(const mx_f4_a4 *) (at + 64);
+                }
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
+                for (int k = 0; k < 2; ++k) {
                     const int blk = blk0 + k * per;
-                    if (blk >= blocks4) break;
-                    uint32_t h, l, se = mx_act4(v[k], h, l);
-                    if (blk >= p.blocks) {
-                        h = l = 0;
-                        se = 127;
-                    }
-                    uint8_t * rec = s_rec + ((size_t) blk * chunk + c) * MX_VEC_REC;
-                    // (24 bits a lane: three bytes of h's 24, three of l's)
-#pragma unroll
-                    for (int t = 0; t < 3; ++t) {
-                        const int o = 3 * i + t;
-                        rec[o < 16 ? o : o + 16] = (uint8_t) (h >> (8 * t));
-                        rec[o < 16 ? o + 16 : o + 24] = (uint8_t) (l >> (8 * t));
-                    }
-                    if (i == 0) s_scale[((blk >> 2) * chunk + c) * 4 + (blk & 3)] = (uint8_t) se;
+                    if (blk >= all) break;
+                    if (blk >= p.blocks) v[k][0] = v[k][1] = mx_f4{0, 0, 0, 0};
+                    uint32_t * rec = (uint32_t *) (s_rec + (blk * chunk + c) * MX_VEC_REC);
+                    const uint32_t e = mx_act_quad(v[k], i, [&](const int d, const uint32_t h, const uint32_t l) {
+                        rec[d] = h;
+                        rec[6 + d] = l;
+                    });
+                    if (i == 0) s_scale[((blk >> 2) * chunk + c) * 4 + (blk & 3)] = (uint8_t) e;
                 }
             }
         }
         __syncthreads();
         mx_f4 acc = {0, 0, 0, 0};
         auto add = [&](const int st, const mx_raw<DW> & f) {
-            mx_w4 wt;
-            f.place(wt);
-            mx_i8 h[4], l[4];
-            uint32_t sx = 0x7F7F7F7Fu;
+            const int c = min(r16, m - 1);  // (a lane without a column: the last one's digits, for sums that nobody reads)
+            const uint32_t sx = *(const uint32_t *) (s_scale + (st * chunk + c) * 4), sl = sx - 0x04040404u;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) h[j] = l[j] = mx_i8{0, 0, 0, 0, 0, 0, 0, 0};
-            if (r16 < m && st <= last) {
-                sx = *(const uint32_t *) (s_scale + (st * chunk + r16) * 4);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint8_t * rec = s_rec + ((size_t) (st * 4 + j) * chunk + r16) * MX_VEC_REC;
-                    h[j] = mx_op6(*(const mx_i4 *) rec, *(const mx_i2 *) (rec + 32));
-                    l[j] = mx_op6(*(const mx_i4 *) (rec + 16), *(const mx_i2 *) (rec + 40));
-                }
+            for (int j = 0; j < 4; ++j) {
+                const uint8_t * rec = s_rec + ((st * 4 + j) * chunk + c) * MX_VEC_REC;
+                const mx_i4 h0 = *(const mx_i4 *) rec, l1 = *(const mx_i4 *) (rec + 32);
+                const mx_i2 h1 = *(const mx_i2 *) (rec + 16), l0 = *(const mx_i2 *) (rec + 24);
+                const mx_i8 h = {h0.x, h0.y, h0.z, h0.w, h1.x, h1.y, 0, 0}, l = {l0.x, l0.y, l1.x, l1.y, l1.z, l1.w, 0, 0};
+                mx_i4 a;
+                int sw;
+                f.place(j, a, sw);
+                if (j == 0) { MX_MFMA(16x16x128, acc, a, sw, 0, h, l, sx, sl) }
+                if (j == 1) { MX_MFMA(16x16x128, acc, a, sw, 1, h, l, sx, sl) }
+                if (j == 2) { MX_MFMA(16x16x128, acc, a, sw, 2, h, l, sx, sl) }
+                if (j == 3) { MX_MFMA(16x16x128, acc, a, sw, 3, h, l, sx, sl) }
+                if (j & 1) __builtin_amdgcn_sched_barrier(0);  // (the digits of all four blocks at a time would cost a third of the waves)
             }
-            const uint32_t sl = sx - 0x04040404u;
-            MX_MFMA(16x16x128, acc, wt, 0, h[0], l[0], sx, sl)
-            MX_MFMA(16x16x128, acc, wt, 1, h[1], l[1], sx, sl)
-            MX_MFMA(16x16x128, acc, wt, 2, h[2], l[2], sx, sl)
-            MX_MFMA(16x16x128, acc, wt, 3, h[3], l[3], sx, sl)
         };
         for (int s0 = wave * 4; s0 < p.steps; s0 += 2 * stride, step += 2 * stride) {  // (s0: the wave's, for all its lanes)
             add(step, f0);
-            f0.load(w, min(step + 2 * stride, last), p.blocks);
+            if (s0 + 2 * stride < p.steps) f0.load(w, min(step + 2 * stride, last), p.blocks);
             if (s0 + stride < p.steps) add(step + stride, f1);
-            f1.load(w, min(step + 3 * stride, last), p.blocks);
+            if (s0 + 3 * stride < p.steps) f1.load(w, min(step + 3 * stride, last), p.blocks);
         }
         if (r16 < m) *(mx_f4 *) (s_part + ((wave * chunk + r16) * 16 + 4 * q)) = acc;
         __syncthreads();
@@ -567,8 +539,8 @@ template <bool ID, int CT, bool DW> __global__ void __launch_bounds__(512) k_mx_
     for (int c = 0; c < CT; ++c)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
-    const int last = p.steps - 1;
-    mx_raw<DW> f;
+    const int last = p.steps - 1, stride = 2 * waves;
+    mx_raw<DW> f0, f1;  // the weights of two turns (of one, with two groups of columns)
     mx_i8 h[CT][4], l[CT][4];
     uint32_t sx[CT];
     auto fetch_x = [&](const int step) {
@@ -590,22 +562,29 @@ template <bool ID, int CT, bool DW> __global__ void __launch_bounds__(512) k_mx_
         }
     };
     int step = wave * 2 + half;
-    f.load(w, min(step, last), p.blocks);
+    f0.load(w, min(step, last), p.blocks);
+    if (CT == 1) f1.load(w, min(step + stride, last), p.blocks);
     fetch_x(step);
-    for (int s0 = wave * 2; s0 < p.steps; s0 += 2 * waves) {  // (s0: the wave's, for both halves)
-        mx_w4 wt;
-        f.place(wt);
-        step += 2 * waves;
-        f.load(w, min(step, last), p.blocks);
+    auto turn = [&](mx_raw<DW> & f) {
+        mx_i4 a[4];
+        int sw[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f.place(j, a[j], sw[j]);
+        f.load(w, min(step + (CT == 1 ? 2 : 1) * stride, last), p.blocks);
+        step += stride;
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
             const uint32_t sl = sx[c] - 0x04040404u;
-            MX_MFMA(32x32x64, acc[c], wt, 0, h[c][0], l[c][0], sx[c], sl)
-            MX_MFMA(32x32x64, acc[c], wt, 1, h[c][1], l[c][1], sx[c], sl)
-            MX_MFMA(32x32x64, acc[c], wt, 2, h[c][2], l[c][2], sx[c], sl)
-            MX_MFMA(32x32x64, acc[c], wt, 3, h[c][3], l[c][3], sx[c], sl)
+            MX_MFMA(32x32x64, acc[c], a[0], sw[0], 0, h[c][0], l[c][0], sx[c], sl)
+            MX_MFMA(32x32x64, acc[c], a[1], sw[1], 1, h[c][1], l[c][1], sx[c], sl)
+            MX_MFMA(32x32x64, acc[c], a[2], sw[2], 2, h[c][2], l[c][2], sx[c], sl)
+            MX_MFMA(32x32x64, acc[c], a[3], sw[3], 3, h[c][3], l[c][3], sx[c], sl)
         }
         fetch_x(step);
+    };
+    for (int s0 = wave * 2; s0 < p.steps; s0 += stride) {  // (s0: the wave's, for both halves)
+        turn(f0);
+        if (CT == 1 && (s0 += stride) < p.steps) turn(f1);
     }
     // [wave][group][column][row], the rows of a column 36 apart (of 32: no two quarters of a wave on the same banks)
     float * part_sums = (float *) lds;
@@ -1030,7 +1009,7 @@ static mx_mm mx_args(const tdesc & w, const tdesc & d, int64_t cols) {
 // k_mx_vec: a wave has two times four steps on the way; columns quantised at a time (0: a column does not fit)
 static constexpr size_t MX_VEC_LDS = 64 << 10;
 static int mx_vec_waves(int64_t K) { return (int) std::min<int64_t>(8, std::max<int64_t>(4, (mx_steps(K) + 7) / 8)); }
-static size_t mx_vec_lds(int64_t K, int64_t cols) { return (size_t) cols * (size_t) (mx_steps(K) * 4 * (MX_VEC_REC + 1)) + (size_t) (mx_vec_waves(K) * cols * 16 * 4); }
+static size_t mx_vec_lds(int64_t K, int64_t cols) { return (size_t) cols * (size_t) ((mx_steps(K) + 3) / 4 * 16 * (MX_VEC_REC + 1)) + (size_t) (mx_vec_waves(K) * cols * 16 * 4); }
 static int mx_vec_chunk(int64_t K, int64_t cols) {
     int64_t c = std::min<int64_t>(16, cols);
     while (c > 0 && mx_vec_lds(K, c) > MX_VEC_LDS) --c;
@@ -1074,7 +1053,10 @@ template <bool ID> static void mx_launch_tile(hipStream_t s, const mx_mm & p, in
     else if (wide(4)) mx_launch_tile_of<ID, 4>(s, p, col_tiles);
     else mx_launch_tile_of<ID, 2>(s, p, col_tiles);
 }
-template <bool ID, int CT> static void mx_launch_few(hipStream_t s, const mx_mm & p, int64_t groups, int waves) {
+// Four waves where the rows and groups alone fill the GPU, eight where they do not (us for 8 / 32 columns, four waves | eight: 4096 rows of 14336 18.3 / 21.2 | 18.6 / 20.3, 14336 of 4096 15.4 / 17.1 |
+// 17.4 / 18.5; 10 / 125 tokens of 32 experts of 4096 x 2048 32.8 / 71.5 | 43.9 / 90.1)
+template <bool ID, int CT> static void mx_launch_few(hipStream_t s, const mx_mm & p, int64_t groups) {
+    const int waves = CT == 1 && (p.n_rows + 31) / 32 * groups < 256 ? 8 : 4;
     const dim3 grid((unsigned) ((p.n_rows + 31) / 32), (unsigned) groups), block((unsigned) (64 * waves));
     const size_t lds = (size_t) waves * CT * 32 * 36 * 4;
     if (mx_dwords(p)) hipLaunchKernelGGL((k_mx_few<ID, CT, true>), grid, block, lds, s, p);
@@ -1086,8 +1068,8 @@ void launch_mx_mul_mat(hipStream_t s, const tdesc & w, const tdesc & b, const td
     p.act = (const uint8_t *) act;
     if (p.n_rows == 0 || p.cols == 0) return;
     if (!act) mx_launch_vec(s, p, b, nullptr);
-    else if (p.cols <= 32) mx_launch_few<false, 1>(s, p, 1, MX_FEWD);
-    else if (p.cols <= MX_FEW_COLS) mx_launch_few<false, 2>(s, p, 1, 4);
+    else if (p.cols <= 32) mx_launch_few<false, 1>(s, p, 1);
+    else if (p.cols <= MX_FEW_COLS) mx_launch_few<false, 2>(s, p, 1);
     else mx_launch_tile<false>(s, p, (p.cols + 127) / 128);
 }
 void launch_mx_mul_mat_id(hipStream_t s, const tdesc & w, const tdesc & b, const tdesc & ids, const tdesc & d, const void * ws, const float * bias, int64_t nb_bias) {
@@ -1099,7 +1081,7 @@ void launch_mx_mul_mat_id(hipStream_t s, const tdesc & w, const tdesc & b, const
     if (!ws) return mx_launch_vec(s, p, b, &ids);
     p.act = (const uint8_t *) ws + mx_lists_bytes(g);
     p.l = mx_lists_at((void *) ws, g);
-    if (cols <= 32 * w.ne[2]) mx_launch_few<true, 1>(s, p, g, MX_FEWI);
+    if (cols <= 32 * w.ne[2]) mx_launch_few<true, 1>(s, p, g);
     else mx_launch_tile<true>(s, p, mx_id_tiles(w.ne[2], cols));
 }
 // which operands the products take (type and shape; the rows of both are dense, whole blocks)
