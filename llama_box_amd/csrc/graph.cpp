@@ -304,7 +304,7 @@ bool supports_op(const ggml_tensor * op) {
             const int st = a->type, dt = op->type;
             if (st == GGML_TYPE_I32 && dt == GGML_TYPE_I32) return true;
             if ((st == GGML_TYPE_MXFP4 && dt == GGML_TYPE_F32) || (st == GGML_TYPE_F32 && dt == GGML_TYPE_MXFP4))
-                return ggml_abi_is_contiguous(a) && ggml_abi_is_contiguous(op) && (a->ne[0] % 32) == 0 && same_shape(a, op);
+                return ggml_abi_is_contiguous(a) && ggml_abi_is_contiguous(op) && (a->ne[0] % 32) == 0 && same_shape(a, op) && mx_rows_ok(TD(a));
             if ((st == GGML_TYPE_Q8_0 && dt == GGML_TYPE_F32) || (st == GGML_TYPE_F32 && dt == GGML_TYPE_Q8_0))  // K-shift of a quantised cache
                 return ggml_abi_is_contiguous(a) && ggml_abi_is_contiguous(op) && (a->ne[0] % 32) == 0;
             if ((kv_store_type(st) && dt == GGML_TYPE_F32) || (st == GGML_TYPE_F32 && kv_store_type(dt)))  // ... of a cache in one of the other types (kv_types.hip)
@@ -313,14 +313,14 @@ bool supports_op(const ggml_tensor * op) {
         }
         case GGML_OP_GET_ROWS:
             return b->type == GGML_TYPE_I32 && op->type == GGML_TYPE_F32 && rows_contig(a) && op->nb[0] == 4 &&
-                   (a->type == GGML_TYPE_MXFP4 || is_quant(a->type) || a->type == GGML_TYPE_F16 || a->type == GGML_TYPE_F32 || a->type == GGML_TYPE_BF16);
+                   ((a->type == GGML_TYPE_MXFP4 && mx_rows_ok(TD(op))) || is_quant(a->type) || a->type == GGML_TYPE_F16 || a->type == GGML_TYPE_F32 || a->type == GGML_TYPE_BF16);
         case GGML_OP_SET_ROWS:
             if (op->type == GGML_TYPE_BF16 && !bf16_rows_in_blocks(a))  // bf16 rows that are not whole, aligned groups of 32 values: the element-wise form (ops.hip)
                 return a->type == GGML_TYPE_F32 && b->type == GGML_TYPE_I64 && a->nb[0] == 4 && op->nb[0] == 2;
             if (kv_store_type(op->type))  // a cache row in q4_0 / q4_1 / q5_0 / q5_1 / iq4_nl / bf16: the type's from_float per block of 32 (kv_types.hip)
                 return a->type == GGML_TYPE_F32 && b->type == GGML_TYPE_I64 && a->nb[0] == 4 && (a->ne[0] % 32) == 0 && (a->nb[1] % 16) == 0 && (a->nb[2] % 16) == 0 && (a->nb[3] % 16) == 0 &&
                        op->nb[0] == ggml_abi_type_size(op->type);
-            if (op->type == GGML_TYPE_MXFP4) return a->type == GGML_TYPE_F32 && b->type == GGML_TYPE_I64 && a->nb[0] == 4 && (a->ne[0] % 32) == 0 && op->nb[0] == ggml_abi_type_size(op->type);
+            if (op->type == GGML_TYPE_MXFP4) return a->type == GGML_TYPE_F32 && b->type == GGML_TYPE_I64 && a->nb[0] == 4 && (a->ne[0] % 32) == 0 && op->nb[0] == ggml_abi_type_size(op->type) && mx_rows_ok(TD(a));
             if (op->type == GGML_TYPE_Q8_0) return a->type == GGML_TYPE_F32 && b->type == GGML_TYPE_I64 && a->nb[0] == 4 && (a->ne[0] % 32) == 0 && (a->nb[1] % 16) == 0 && (a->nb[2] % 16) == 0 && (a->nb[3] % 16) == 0;
             return a->type == GGML_TYPE_F32 && b->type == GGML_TYPE_I64 && a->nb[0] == 4 && (op->type == GGML_TYPE_F16 || op->type == GGML_TYPE_F32) &&
                    op->nb[0] == ggml_abi_type_size(op->type);
@@ -2928,7 +2928,7 @@ static int run_mul_mat_mx(exec_state & st, int i) {
     backend_ctx * c = st.c;
     ggml_tensor * n = st.g->nodes[i];
     const ggml_tensor * a = n->src[0], * b = n->src[1];
-    void * act = mx_vec_takes(b->ne[0], b->ne[1] * b->ne[2] * b->ne[3]) ? nullptr : (char *) c->ws + st.act_off;
+    void * act = mx_vec_takes(a->ne[0], a->ne[1], b->ne[1] * b->ne[2] * b->ne[3]) ? nullptr : (char *) c->ws + st.act_off;
     if (act && !c->act.holds(b, MI_ACT_MX)) {
         timed_scope ts(c, "quantize_act", (double) ggml_abi_nbytes(b));
         launch_mx_act(c->stream, TD(b), act);
@@ -2954,7 +2954,7 @@ static int run_mul_mat_id_mx(exec_state & st, int i) {
     ggml_cgraph * g = st.g;
     ggml_tensor * n = g->nodes[i];
     const ggml_tensor * a = n->src[0], * b = n->src[1], * ids = n->src[2];
-    void * ws = mx_id_vec_takes(b->ne[0], ids->ne[0] * ids->ne[1]) ? nullptr : (char *) c->ws + st.act_off;
+    void * ws = mx_id_vec_takes(a->ne[0], a->ne[1], ids->ne[0] * ids->ne[1]) ? nullptr : (char *) c->ws + st.act_off;
     bool lists = st.mx_node >= 0 && st.mx_ids == ids && st.mx_experts == a->ne[2] && c->act.kind == MI_ACT_MX_ID;
     for (int k = st.mx_node + 1; lists && k < i; ++k) lists = is_view_op(g->nodes[k]) || !ranges_overlap(g->nodes[k], ids);
     const bool cols = lists && c->act.holds(b, MI_ACT_MX_ID);

@@ -536,11 +536,12 @@ void launch_argsort_grouped(hipStream_t s, const tdesc & src, const tdesc & dst,
 
 // ---- microscaled 4-bit (mx.hip)
 // f32 rows -> MXFP4 and back; idx: the places of SET_ROWS (I64) / the rows of GET_ROWS (I32), null: row by row (CPY)
+bool mx_rows_ok(const tdesc & f32);  // sizes that the launches hold
 void launch_mx_store(hipStream_t s, const tdesc & a, const tdesc * idx, const tdesc & d);
 void launch_mx_read(hipStream_t s, const tdesc & a, const tdesc * idx, const tdesc & d);
 // MUL_MAT: w [K, N], b f32 rows of K, d dense.  act: mx_act_bytes(K, columns) that launch_mx_act has filled from b; null for the few columns that the product quantises itself (mx_vec_takes)
-bool mx_vec_takes(int64_t K, int64_t cols);
-bool mx_id_vec_takes(int64_t K, int64_t cols);
+bool mx_vec_takes(int64_t K, int64_t N, int64_t cols);
+bool mx_id_vec_takes(int64_t K, int64_t N, int64_t cols);
 bool mx_product_ok(const tdesc & w, const tdesc & b);
 size_t mx_act_bytes(int64_t K, int64_t cols);
 void launch_mx_act(hipStream_t s, const tdesc & b, void * act);

@@ -25,48 +25,40 @@ typedef int mx_i8 __attribute__((ext_vector_type(8)));
 typedef float mx_f4 __attribute__((ext_vector_type(4)));
 typedef float mx_f16 __attribute__((ext_vector_type(16)));
 typedef mx_i4 __attribute__((aligned(4))) mx_i4_a4;
-typedef uint16_t __attribute__((aligned(1))) mx_u16_a1;
-typedef float mx_f2 __attribute__((ext_vector_type(2)));
-typedef mx_f2 __attribute__((aligned(4))) mx_f2_a4;
+typedef uint32_t __attribute__((aligned(1))) mx_u32_a1;
+typedef mx_f4 __attribute__((aligned(4))) mx_f4_a4;
 
 static constexpr int MX_BLOCK = 17;  // bytes
 static constexpr int MX_FP4 = 4, MX_FP6 = 2;  // operand formats of the matrix instructions: E2M1, E2M3
 
 // ------------------------------------------------------------------------------------------------ rows
-// Eight lanes share a block: lane i of them has the values 2i, 2i + 1, 16 + 2i, 16 + 2i + 1, whose codes are the bytes 2i and 2i + 1.
-__device__ __forceinline__ void mx_load4(const float * blk, const int i, float (&v)[4]) {
-    const mx_f2 a = *(const mx_f2_a4 *) (blk + 2 * i), b = *(const mx_f2_a4 *) (blk + 16 + 2 * i);
-    v[0] = a.x;
-    v[1] = a.y;
-    v[2] = b.x;
-    v[3] = b.y;
-}
+// Four lanes share a block: lane i of them has the values 4i .. 4i + 3 (v[0]) and 16 + 4i .. 16 + 4i + 3 (v[1]), whose codes are the bytes 4i .. 4i + 3.
 // the bits of the block's largest magnitude (an infinity's or NaN's bits are larger than any number's)
-__device__ __forceinline__ uint32_t mx_top(const float (&v)[4]) {
+__device__ __forceinline__ uint32_t mx_top(const mx_f4 (&v)[2]) {
     uint32_t m = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) m = max(m, __float_as_uint(v[k]) & 0x7FFFFFFFu);
+    for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(v[k >> 2][k & 3]) & 0x7FFFFFFFu);
     m = max(m, (uint32_t) dpp_i32<MI_DPP_QUAD_XOR1>((int) m));
-    m = max(m, (uint32_t) dpp_i32<MI_DPP_QUAD_XOR2>((int) m));
-    return max(m, (uint32_t) dpp_i32<MI_DPP_HALF_MIRROR>((int) m));
+    return max(m, (uint32_t) dpp_i32<MI_DPP_QUAD_XOR2>((int) m));
 }
-// the nearest code, a tie to the lower one (of two magnitudes the smaller, of two zeros +0); m2: 2^(127 - e) in two factors that f32 holds
-__device__ __forceinline__ uint32_t mx_code(const float v, const float f0, const float f1) {
-    const float m = fabsf(v) * f0 * f1;
-    const uint32_t c = (uint32_t) (m > 0.25f) + (uint32_t) (m > 0.75f) + (uint32_t) (m > 1.25f) + (uint32_t) (m > 1.75f) + (uint32_t) (m > 2.5f) + (uint32_t) (m > 3.5f) + (uint32_t) (m > 5.0f);
+__device__ __forceinline__ void mx_load8(const char * at, const int i, mx_f4 (&v)[2]) {
+    v[0] = *(const mx_f4_a4 *) (at + 16 * i);
+    v[1] = *(const mx_f4_a4 *) (at + 64 + 16 * i);
+}
+// the nearest code of v 2^x, a tie to the lower one (of two magnitudes the smaller, of two zeros +0).  From 1 on a code is exponent and first bit of the mantissa, rounded down in a tie
+__device__ __forceinline__ uint32_t mx_code(const float v, const int x) {
+    const float m = __builtin_amdgcn_ldexpf(fabsf(v), x);
+    const uint32_t high = min(((__float_as_uint(m) + 0x1FFFFFu) >> 22) - 0xFCu, 7u), low = (uint32_t) (m > 0.25f) + (uint32_t) (m > 0.75f), c = m >= 1.0f ? high : low;
     return c ? c | ((__float_as_uint(v) >> 31) << 3) : 0u;
 }
-// -> the block's scale byte; the lane's two bytes of codes
-__device__ __forceinline__ int mx_quantise4(const float (&v)[4], uint32_t & codes) {
+// -> the block's scale byte; the lane's four bytes of codes
+__device__ __forceinline__ int mx_quantise8(const mx_f4 (&v)[2], uint32_t & codes) {
     const uint32_t top = mx_top(v);
+    const int e = top >= 0x7F800000u ? 255 : max((int) (top >> 23) - 2, 0);  // floor(log2) - 2 + 127 (a subnormal's is below every scale)
     codes = 0;
-    if (top >= 0x7F800000u) return 255;
-    int lg = (int) (top >> 23) - 127;                          // floor(log2) of a normal number
-    if (lg == -127) lg = -118 - __clz((int) (top | 1u));       // ... of a subnormal one: bits 2^-149; below every scale's range anyway
-    const int e = top ? max(lg + 125, 0) : 0;
-    const int half = (127 - e) / 2, rest = 127 - e - half;     // (127 - e: -127 .. 127)
-    const float f0 = __uint_as_float((uint32_t) (127 + half) << 23), f1 = __uint_as_float((uint32_t) (127 + rest) << 23);
-    codes = mx_code(v[0], f0, f1) | mx_code(v[2], f0, f1) << 4 | mx_code(v[1], f0, f1) << 8 | mx_code(v[3], f0, f1) << 12;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) codes |= (mx_code(v[0][k], 127 - e) | mx_code(v[1][k], 127 - e) << 4) << (8 * k);
+    if (e == 255) codes = 0;
     return e;
 }
 // 2^(e - 127) as f32 (e = 0: subnormal), NaN for 255
@@ -76,66 +68,100 @@ __device__ __forceinline__ float mx_value(const uint32_t code, const float scale
     const float m = 0.5f * (float) ((0xC8643210u >> (4 * (code & 7))) & 15u);
     return ((code & 8) ? -m : m) * scale;
 }
-struct mx_row_at { int64_t i1, i2, i3, blk; };
-__device__ __forceinline__ mx_row_at mx_row(const int64_t block, const int64_t per_row, const int64_t n1, const int64_t n2) {
-    mx_row_at r;
-    const int64_t row = block / per_row;
-    r.blk = block - row * per_row;
-    r.i1 = row % n1;
-    r.i2 = (row / n1) % n2;
-    r.i3 = row / (n1 * n2);
-    return r;
+__device__ __forceinline__ void mx_put8(char * at, const int i, const uint32_t c, const float s) {
+    mx_f4 v[2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        v[0][k] = mx_value((c >> (8 * k)) & 15, s);
+        v[1][k] = mx_value((c >> (8 * k + 4)) & 15, s);
+    }
+    *(mx_f4_a4 *) (at + 16 * i) = v[0];
+    *(mx_f4_a4 *) (at + 64 + 16 * i) = v[1];
 }
-// f32 rows -> blocks.  idx: SET_ROWS, the rows' places (one outside the destination is skipped); without: row i to row i
+// Row blockIdx.x, 64 blocks of it.  f32 rows -> blocks; idx: SET_ROWS, the rows' places (one outside the destination is skipped); without: row i to row i
 template <bool IDX> __global__ void __launch_bounds__(256) k_mx_store(const tdesc a, const tdesc idx, const tdesc d) {
-    const int64_t per_row = a.ne[0] / 32, block = ((int64_t) blockIdx.x * 256 + threadIdx.x) >> 3;
-    const int i = threadIdx.x & 7;
-    if (block >= per_row * a.ne[1] * a.ne[2] * a.ne[3]) return;  // (eight lanes leave together)
-    const mx_row_at r = mx_row(block, per_row, a.ne[1], a.ne[2]);
-    int64_t to = r.i1;
+    const uint32_t row = blockIdx.x, n1 = (uint32_t) a.ne[1], n2 = (uint32_t) a.ne[2], r23 = row / n1, i1 = row - r23 * n1, i3 = r23 / n2, i2 = r23 - i3 * n2;
+    const int blk = (int) (blockIdx.y * 64 + (threadIdx.x >> 2)), i = threadIdx.x & 3;
+    if (blk >= a.ne[0] / 32) return;  // (four lanes leave together)
+    int64_t to = i1;
     if (IDX) {
-        to = *(const int64_t *) (idx.data + r.i1 * idx.nb[0] + (r.i2 % idx.ne[1]) * idx.nb[1] + (r.i3 % idx.ne[2]) * idx.nb[2]);
+        to = *(const int64_t *) (idx.data + i1 * idx.nb[0] + (i2 % (uint32_t) idx.ne[1]) * idx.nb[1] + (i3 % (uint32_t) idx.ne[2]) * idx.nb[2]);
         if (to < 0 || to >= d.ne[1]) return;
     }
-    float v[4];
-    mx_load4((const float *) (a.data + r.i1 * a.nb[1] + r.i2 * a.nb[2] + r.i3 * a.nb[3]) + r.blk * 32, i, v);
+    mx_f4 v[2];
+    mx_load8(a.data + i1 * a.nb[1] + i2 * a.nb[2] + i3 * a.nb[3] + (int64_t) blk * 128, i, v);
     uint32_t codes;
-    const int e = mx_quantise4(v, codes);
-    uint8_t * out = (uint8_t *) d.data + to * d.nb[1] + r.i2 * d.nb[2] + r.i3 * d.nb[3] + r.blk * MX_BLOCK;
+    const int e = mx_quantise8(v, codes);
+    uint8_t * out = (uint8_t *) d.data + to * d.nb[1] + i2 * d.nb[2] + i3 * d.nb[3] + (int64_t) blk * MX_BLOCK;
     if (i == 0) out[0] = (uint8_t) e;
-    *(mx_u16_a1 *) (out + 1 + 2 * i) = (uint16_t) codes;
+    *(mx_u32_a1 *) (out + 1 + 4 * i) = codes;
 }
-// blocks -> f32 rows.  idx: GET_ROWS, the rows taken (one outside the source is skipped)
+// blocks -> f32 rows; idx: GET_ROWS, the rows taken (one outside the source is skipped)
 template <bool IDX> __global__ void __launch_bounds__(256) k_mx_read(const tdesc a, const tdesc idx, const tdesc d) {
-    const int64_t per_row = a.ne[0] / 32, block = ((int64_t) blockIdx.x * 256 + threadIdx.x) >> 3;
-    const int i = threadIdx.x & 7;
-    if (block >= per_row * d.ne[1] * d.ne[2] * d.ne[3]) return;
-    const mx_row_at r = mx_row(block, per_row, d.ne[1], d.ne[2]);
-    int64_t from = r.i1;
+    const uint32_t row = blockIdx.x, n1 = (uint32_t) d.ne[1], n2 = (uint32_t) d.ne[2], r23 = row / n1, i1 = row - r23 * n1, i3 = r23 / n2, i2 = r23 - i3 * n2;
+    const int blk = (int) (blockIdx.y * 64 + (threadIdx.x >> 2)), i = threadIdx.x & 3;
+    if (blk >= a.ne[0] / 32) return;
+    int64_t from = i1;
     if (IDX) {
-        from = *(const int32_t *) (idx.data + r.i1 * idx.nb[0] + r.i2 * idx.nb[1] + r.i3 * idx.nb[2]);
+        from = *(const int32_t *) (idx.data + i1 * idx.nb[0] + i2 * idx.nb[1] + i3 * idx.nb[2]);
         if (from < 0 || from >= a.ne[1]) return;
     }
-    const uint8_t * in = (const uint8_t *) a.data + from * a.nb[1] + r.i2 * a.nb[2] + r.i3 * a.nb[3] + r.blk * MX_BLOCK;
-    const float s = mx_scale(in[0]);
-    const uint32_t c = *(const mx_u16_a1 *) (in + 1 + 2 * i);
-    float * out = (float *) (d.data + r.i1 * d.nb[1] + r.i2 * d.nb[2] + r.i3 * d.nb[3]) + r.blk * 32 + 2 * i;
-    *(mx_f2_a4 *) out = mx_f2{mx_value(c & 15, s), mx_value((c >> 8) & 15, s)};
-    *(mx_f2_a4 *) (out + 16) = mx_f2{mx_value((c >> 4) & 15, s), mx_value(c >> 12, s)};
+    const uint8_t * in = (const uint8_t *) a.data + from * a.nb[1] + i2 * a.nb[2] + i3 * a.nb[3] + (int64_t) blk * MX_BLOCK;
+    mx_put8(d.data + i1 * d.nb[1] + i2 * d.nb[2] + i3 * d.nb[3] + (int64_t) blk * 128, i, *(const mx_u32_a1 *) (in + 1 + 4 * i), mx_scale(in[0]));
 }
+// Dense tensors (CPY): a workgroup has 256 blocks, whose 4352 bytes cross LDS so that they are read and written 16 bytes at a time (byte by byte as above, 14336 x 4096 values there and back: 151 us)
+static constexpr int MX_CPY = 256;
+__global__ void __launch_bounds__(256) k_mx_store_dense(const char * __restrict__ x, uint8_t * __restrict__ out, const int64_t blocks) {
+    __shared__ __align__(16) uint8_t s[MX_CPY * MX_BLOCK];
+    const int64_t b0 = (int64_t) blockIdx.x * MX_CPY;
+    const int n = (int) min((int64_t) MX_CPY, blocks - b0), tid = threadIdx.x, i = tid & 3;
+    mx_f4 v[4][2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) mx_load8(x + (b0 + min(64 * k + (tid >> 2), n - 1)) * 128, i, v[k]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int blk = 64 * k + (tid >> 2);
+        uint32_t codes;
+        const int e = mx_quantise8(v[k], codes);
+        if (i == 0) s[blk * MX_BLOCK] = (uint8_t) e;
+        *(mx_u32_a1 *) (s + blk * MX_BLOCK + 1 + 4 * i) = codes;
+    }
+    __syncthreads();
+    uint8_t * to = out + b0 * MX_BLOCK;
+    const int bytes = n * MX_BLOCK;
+    for (int at = tid; at < bytes / 16; at += 256) ((mx_i4 *) to)[at] = ((const mx_i4 *) s)[at];
+    for (int at = (bytes & ~15) + tid; at < bytes; at += 256) to[at] = s[at];
+}
+__global__ void __launch_bounds__(256) k_mx_read_dense(const uint8_t * __restrict__ in, char * __restrict__ out, const int64_t blocks) {
+    __shared__ __align__(16) uint8_t s[MX_CPY * MX_BLOCK];
+    const int64_t b0 = (int64_t) blockIdx.x * MX_CPY;
+    const int n = (int) min((int64_t) MX_CPY, blocks - b0), tid = threadIdx.x, i = tid & 3, bytes = n * MX_BLOCK;
+    const uint8_t * from = in + b0 * MX_BLOCK;
+    for (int at = tid; at < bytes / 16; at += 256) ((mx_i4 *) s)[at] = ((const mx_i4 *) from)[at];
+    for (int at = (bytes & ~15) + tid; at < bytes; at += 256) s[at] = from[at];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int blk = 64 * k + (tid >> 2);
+        if (blk < n) mx_put8(out + (b0 + blk) * 128, i, *(const mx_u32_a1 *) (s + blk * MX_BLOCK + 1 + 4 * i), mx_scale(s[blk * MX_BLOCK]));
+    }
+}
+// the launches' sizes: rows, 64 blocks of a row each
+static dim3 mx_rows_grid(const tdesc & t) { return dim3((unsigned) (t.ne[1] * t.ne[2] * t.ne[3]), (unsigned) ((t.ne[0] / 32 + 63) / 64)); }
+bool mx_rows_ok(const tdesc & f32) { return f32.ne[1] * f32.ne[2] * f32.ne[3] < ((int64_t) 1 << 31) && f32.ne[0] / 32 <= 64 * 65535; }
 void launch_mx_store(hipStream_t s, const tdesc & a, const tdesc * idx, const tdesc & d) {
     const int64_t n = (a.ne[0] / 32) * a.ne[1] * a.ne[2] * a.ne[3];
     if (n <= 0) return;
-    const dim3 grid((unsigned) ((n + 31) / 32));
-    if (idx) hipLaunchKernelGGL(k_mx_store<true>, grid, dim3(256), 0, s, a, *idx, d);
-    else hipLaunchKernelGGL(k_mx_store<false>, grid, dim3(256), 0, s, a, a, d);
+    if (idx) hipLaunchKernelGGL(k_mx_store<true>, mx_rows_grid(a), dim3(256), 0, s, a, *idx, d);
+    else if (((uintptr_t) d.data & 15) == 0) hipLaunchKernelGGL(k_mx_store_dense, dim3((unsigned) ((n + MX_CPY - 1) / MX_CPY)), dim3(256), 0, s, a.data, (uint8_t *) d.data, n);
+    else hipLaunchKernelGGL(k_mx_store<false>, mx_rows_grid(a), dim3(256), 0, s, a, a, d);
 }
 void launch_mx_read(hipStream_t s, const tdesc & a, const tdesc * idx, const tdesc & d) {
     const int64_t n = (a.ne[0] / 32) * d.ne[1] * d.ne[2] * d.ne[3];
     if (n <= 0) return;
-    const dim3 grid((unsigned) ((n + 31) / 32));
-    if (idx) hipLaunchKernelGGL(k_mx_read<true>, grid, dim3(256), 0, s, a, *idx, d);
-    else hipLaunchKernelGGL(k_mx_read<false>, grid, dim3(256), 0, s, a, a, d);
+    if (idx) hipLaunchKernelGGL(k_mx_read<true>, mx_rows_grid(d), dim3(256), 0, s, a, *idx, d);
+    else if (((uintptr_t) a.data & 15) == 0) hipLaunchKernelGGL(k_mx_read_dense, dim3((unsigned) ((n + MX_CPY - 1) / MX_CPY)), dim3(256), 0, s, (const uint8_t *) a.data, d.data, n);
+    else hipLaunchKernelGGL(k_mx_read<false>, mx_rows_grid(d), dim3(256), 0, s, a, a, d);
 }
 
 // ------------------------------------------------------------------------------------------------ activations
@@ -267,15 +293,9 @@ __device__ __forceinline__ void mx_digits(const float v, const float f, uint32_t
 }
 // Four lanes a block: lane i has the values 4i .. 4i + 3 (v[0]) and 16 + 4i .. 16 + 4i + 3 (v[1]), places 8i .. 8i + 7, 48 bits of h and of l; a pair of lanes has three dwords of each, put(d, ..) is given
 // dword d of the block's six.  -> the scale byte
-typedef mx_f4 __attribute__((aligned(4))) mx_f4_a4;
 template <class Put> __device__ __forceinline__ uint32_t mx_act_quad(const mx_f4 (&v)[2], const int i, Put && put) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k >> 2][k & 3]) & 0x7FFFFFFFu);
-    top = max(top, (uint32_t) dpp_i32<MI_DPP_QUAD_XOR1>((int) top));
-    top = max(top, (uint32_t) dpp_i32<MI_DPP_QUAD_XOR2>((int) top));
     float f;
-    const uint32_t e = mx_step(top, f);
+    const uint32_t e = mx_step(mx_top(v), f);
     uint64_t h = 0, l = 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {  // place k: value k / 2 of the first four or of the second
@@ -1015,9 +1035,11 @@ static int mx_vec_chunk(int64_t K, int64_t cols) {
     while (c > 0 && mx_vec_lds(K, c) > MX_VEC_LDS) --c;
     return (int) c;
 }
-static constexpr int64_t MX_VEC_COLS = 4, MX_VEC_ID_COLS = 32, MX_FEW_COLS = 64;
-bool mx_vec_takes(int64_t K, int64_t cols) { return cols <= MX_VEC_COLS && mx_vec_chunk(K, cols) >= cols; }
-bool mx_id_vec_takes(int64_t K, int64_t cols) { return cols <= MX_VEC_ID_COLS && mx_vec_chunk(K, cols) >= 1; }
+static constexpr int64_t MX_FEW_COLS = 64;
+// Every workgroup quantises its columns: two launches less (three with MUL_MAT_ID), for work that grows with columns and rows.  us, itself | k_mx_few: 4 columns of 4096 x 4096 8.2 | 10.7, 2 of 14336 x
+// 4096 13.5 | 15.4, 4 of 14336 x 4096 18.1 | 15.4, 4 of 4096 x 14336 20.2 | 18.3; expert columns, 4096 x 4096 of 32: 16 of them 36.8 | 42.2, 24 46.5 | 45.7, 32 59.0 | 57.9, 1024 x 1024: 32 9.3 | 15.2
+bool mx_vec_takes(int64_t K, int64_t N, int64_t cols) { return (cols == 1 || (cols <= 4 && cols * K * N <= 150000000)) && mx_vec_chunk(K, cols) >= cols; }
+bool mx_id_vec_takes(int64_t K, int64_t N, int64_t cols) { return (cols <= 24 || (cols <= 64 && cols * K * N <= 100000000)) && mx_vec_chunk(K, cols) >= 1; }
 // rows of whole steps, every one at a whole dword
 static bool mx_dwords(const mx_mm & p) { return p.blocks % 4 == 0 && p.nb1 % 4 == 0 && p.nb2 % 4 == 0 && ((uintptr_t) p.w & 3) == 0; }
 // ... of whole 16-byte pieces
