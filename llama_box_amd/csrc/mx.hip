@@ -11,12 +11,6 @@
 #include "dev_util.h"
 #include "kernels.h"
 
-#ifndef MX_VOCC
-#define MX_VOCC 3
-#endif
-#ifndef MX_SET
-#define MX_SET 1
-#endif
 namespace mi355x {
 
 typedef int mx_i4 __attribute__((ext_vector_type(4)));
@@ -436,13 +430,13 @@ template <> struct mx_raw<false> {
     ACC = __builtin_amdgcn_mfma_scale_f32_##N##_f8f6f4(mx_op4(A), H, ACC, MX_FP4, MX_FP6, J, S, J, (int) (SH));              \
     ACC = __builtin_amdgcn_mfma_scale_f32_##N##_f8f6f4(mx_op4(A), L, ACC, MX_FP4, MX_FP6, J, S, J, (int) (SL));
 
-// ---- one to a few columns: 16 rows a workgroup, its waves take four steps of 128 values in turn.  The workgroup quantises its columns itself, while its first weights are on the way: a launch in front
-// costs more.  A lane of v_mfma_scale_f32_16x16x128: row (column) lane % 16, step lane / 16 of the four.
+// ---- one to a few columns: 16 rows a workgroup, its waves take four steps of 128 values in turn.  The workgroup quantises its columns itself, while its first weights are on the way.  A lane of v_mfma_scale_f32_16x16x128: row (column) lane % 16, step lane / 16 of the four.
 // ID: blockIdx.y is a column (u + n_used t) of at most 64; the first column of an expert takes all of its expert, the others' workgroups end at once.
 static constexpr int MX_VEC_REC = 48;     // LDS bytes of a block of one column: 24 of h, 24 of l
-template <bool ID, bool DW> __global__ void __launch_bounds__(512, DW ? MX_VOCC : 2) k_mx_vec(const mx_mm p, const tdesc b, const tdesc ids, const int chunk) {
+template <bool ID, bool DW> __global__ void __launch_bounds__(512, DW ? 3 : 2) k_mx_vec(const mx_mm p, const tdesc b, const tdesc ids, const int chunk) {
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ int s_cols[64];
+    __shared__ int64_t s_at[64];  // where the workgroup's columns start in b
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, r16 = lane & 15, q = lane >> 4;
     const int row0 = (int) blockIdx.x * 16, all = (p.steps + 3) / 4 * 16;  // blocks of a column, with those behind its last that the last turn takes (zeros)
     int e = 0, n = (int) p.cols;
@@ -454,7 +448,14 @@ template <bool ID, bool DW> __global__ void __launch_bounds__(512, DW ? MX_VOCC 
         const uint64_t mine = __ballot(id == e);
         if (mine & ((1ull << slot) - 1ull)) return;
         n = __popcll(mine);
-        if (wave == 0 && id == e) s_cols[__popcll(mine & ((1ull << lane) - 1ull))] = lane;
+        if (wave == 0 && id == e) {
+            const int at = __popcll(mine & ((1ull << lane) - 1ull));
+            s_cols[at] = lane;
+            s_at[at] = ((lane % n_used) % (int) b.ne[1]) * b.nb[1] + (int64_t) (lane / n_used) * b.nb[2];
+        }
+    } else if ((int) threadIdx.x < n) {
+        const uint32_t c = threadIdx.x, n1 = (uint32_t) b.ne[1], n2 = (uint32_t) b.ne[2], c23 = c / n1, c3 = c23 / n2;
+        s_at[c] = (int64_t) (c - c23 * n1) * b.nb[1] + (int64_t) (c23 - c3 * n2) * b.nb[2] + (int64_t) c3 * b.nb[3];
     }
     const uint8_t * w = p.w + (int64_t) e * p.nb2 + (int64_t) min(row0 + r16, p.n_rows - 1) * p.nb1;
     uint8_t * s_rec = lds, * s_scale = lds + (size_t) chunk * all * MX_VEC_REC;  // [block][column of the chunk]; [step][column][block] scale bytes
@@ -467,37 +468,28 @@ template <bool ID, bool DW> __global__ void __launch_bounds__(512, DW ? MX_VOCC 
         int step = wave * 4 + q;  // (behind the last step: its weights again, and digits of zero)
         f0.load(w, min(step, last), p.blocks);
         if (wave * 4 + stride < p.steps) f1.load(w, min(step + stride, last), p.blocks);
-        if (ID || c0) __syncthreads();  // (the columns' list; the last chunk's partial sums and digits are read)
+        __syncthreads();  // (the columns' places; the last chunk's partial sums and digits are read)
         const int i = threadIdx.x & 3, per = (int) blockDim.x >> 2;  // four lanes a block
-        for (int c = 0; c < m; ++c) {
-            const char * col;
-            if (ID) {
-                const int cc = s_cols[c0 + c], n_used = (int) ids.ne[0];
-                col = b.data + ((cc % n_used) % (int) b.ne[1]) * b.nb[1] + (int64_t) (cc / n_used) * b.nb[2];
-            } else {
-                const int cc = c0 + c, n1 = (int) b.ne[1], n2 = (int) b.ne[2];
-                col = b.data + (cc % n1) * b.nb[1] + (int64_t) ((cc / n1) % n2) * b.nb[2] + (int64_t) (cc / (n1 * n2)) * b.nb[3];
+        for (int at0 = threadIdx.x >> 2; at0 < m * all; at0 += 2 * per) {
+            mx_f4 v[2][2];
+            int blk[2], c[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int at = min(at0 + k * per, m * all - 1);
+                c[k] = m == 1 ? 0 : at / all;
+                blk[k] = at - c[k] * all;
+                mx_load8(b.data + s_at[c0 + c[k]] + min(blk[k], p.blocks - 1) * 128, i, v[k]);
             }
-            for (int blk0 = threadIdx.x >> 2; blk0 < all; blk0 += 2 * per) {
-                mx_f4 v[2][2];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const char * at = col + (min(blk0 + k * per, p.blocks - 1) * 32 + 4 * i) * 4;
-                    v[k][0] = *(const mx_f4_a4 *) at;
-                    v[k][1] = *(const mx_f4_a4 *) (at + 64);
-                }
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const int blk = blk0 + k * per;
-                    if (blk >= all) break;
-                    if (blk >= p.blocks) v[k][0] = v[k][1] = mx_f4{0, 0, 0, 0};
-                    uint32_t * rec = (uint32_t *) (s_rec + (blk * chunk + c) * MX_VEC_REC);
-                    const uint32_t e = mx_act_quad(v[k], i, [&](const int d, const uint32_t h, const uint32_t l) {
-                        rec[d] = h;
-                        rec[6 + d] = l;
-                    });
-                    if (i == 0) s_scale[((blk >> 2) * chunk + c) * 4 + (blk & 3)] = (uint8_t) e;
-                }
+            for (int k = 0; k < 2; ++k) {
+                if (at0 + k * per >= m * all) break;
+                if (blk[k] >= p.blocks) v[k][0] = v[k][1] = mx_f4{0, 0, 0, 0};
+                uint32_t * rec = (uint32_t *) (s_rec + (blk[k] * chunk + c[k]) * MX_VEC_REC);
+                const uint32_t e = mx_act_quad(v[k], i, [&](const int d, const uint32_t h, const uint32_t l) {
+                    rec[d] = h;
+                    rec[6 + d] = l;
+                });
+                if (i == 0) s_scale[((blk[k] >> 2) * chunk + c[k]) * 4 + (blk[k] & 3)] = (uint8_t) e;
             }
         }
         __syncthreads();
@@ -845,7 +837,7 @@ template <int RT> struct mx_wide_args {
 };
 // one wave's share of a tile: quarter 2 half + ODD of every stage
 template <int RT, int ODD> __device__ __forceinline__ void mx_wide_sum(const mx_wide_args<RT> & p, uint8_t * lds, mx_f16 (&acc)[RT]) {
-    constexpr int SET = MX_SET, SETS = RT / SET, PIECES = mx_wide_pieces<RT>(), STAGE = PIECES * 8192, GROUPS = 4 * SETS, SLOTS = 2 * SET;
+    constexpr int SET = 1, SETS = RT / SET, PIECES = mx_wide_pieces<RT>(), STAGE = PIECES * 8192, GROUPS = 4 * SETS, SLOTS = 2 * SET;
     const int r32 = p.lane & 31, half = p.lane >> 5;
     const uint32_t lds0 = (uint32_t) (uintptr_t) lds;
     uint32_t first = p.first;
@@ -1026,19 +1018,23 @@ static mx_mm mx_args(const tdesc & w, const tdesc & d, int64_t cols) {
     p.cols = cols;
     return p;
 }
-// k_mx_vec: a wave has two times four steps on the way; columns quantised at a time (0: a column does not fit)
-static constexpr size_t MX_VEC_LDS = 64 << 10;
-static int mx_vec_waves(int64_t K) { return (int) std::min<int64_t>(8, std::max<int64_t>(4, (mx_steps(K) + 7) / 8)); }
-static size_t mx_vec_lds(int64_t K, int64_t cols) { return (size_t) cols * (size_t) ((mx_steps(K) + 3) / 4 * 16 * (MX_VEC_REC + 1)) + (size_t) (mx_vec_waves(K) * cols * 16 * 4); }
+// k_mx_vec: columns quantised at a time (0: a column does not fit).  A wave has two times four steps on the way; eight waves where the workgroups alone do not fill the GPU (us, four waves | eight: 1 / 8
+// columns of 4096 x 4096, 256 workgroups, 5.4 / 11.9 | 5.3 / 10.0, of 5632 x 2048, 352 workgroups, 4.9 / 9.6 | 6.6 / 11.1)
+static constexpr size_t MX_VEC_LDS = 60 << 10;
+static int mx_vec_waves(int64_t K, int64_t N, int64_t slots) { return (int) std::min<int64_t>(8, std::max<int64_t>((N + 15) / 16 * slots <= 256 ? 8 : 4, (mx_steps(K) + 7) / 8)); }
+static size_t mx_vec_lds(int64_t K, int64_t cols) { return (size_t) cols * (size_t) ((mx_steps(K) + 3) / 4 * 16 * (MX_VEC_REC + 1)) + (size_t) (8 * cols * 16 * 4); }
 static int mx_vec_chunk(int64_t K, int64_t cols) {
     int64_t c = std::min<int64_t>(16, cols);
     while (c > 0 && mx_vec_lds(K, c) > MX_VEC_LDS) --c;
     return (int) c;
 }
 static constexpr int64_t MX_FEW_COLS = 64;
-// Every workgroup quantises its columns: two launches less (three with MUL_MAT_ID), for work that grows with columns and rows.  us, itself | k_mx_few: 4 columns of 4096 x 4096 8.2 | 10.7, 2 of 14336 x
-// 4096 13.5 | 15.4, 4 of 14336 x 4096 18.1 | 15.4, 4 of 4096 x 14336 20.2 | 18.3; expert columns, 4096 x 4096 of 32: 16 of them 36.8 | 42.2, 24 46.5 | 45.7, 32 59.0 | 57.9, 1024 x 1024: 32 9.3 | 15.2
-bool mx_vec_takes(int64_t K, int64_t N, int64_t cols) { return (cols == 1 || (cols <= 4 && cols * K * N <= 150000000)) && mx_vec_chunk(K, cols) >= cols; }
+// Every workgroup quantises its columns: a launch less (two with MUL_MAT_ID), for work that grows with columns and rows.  us, k_mx_vec | k_mx_few: 2 / 4 columns of 14336 x 4096 13.5 / 18.4 | 17.3 / 17.4, of
+// 4096 x 14336 13.0 / 20.3 (two at a time) | 20.2 / 20.3, 4 / 8 of 4096 x 4096 7.1 / 10.0 | 11.8 / 11.9, of 5632 x 2048 6.7 / 9.6 | 9.1 / 9.1, 8 / 16 of 1024 x 1024 5.2 / 6.4 | 7.7 / 8.1; expert columns, of 32
+// experts of 4096 x 4096: 16 / 24 / 32 of them 36.8 / 46.5 / 59.0 | 42.2 / 45.7 / 57.9, of 1024 x 1024 32 9.3 | 15.2
+bool mx_vec_takes(int64_t K, int64_t N, int64_t cols) {
+    return (cols == 1 || (cols <= 16 && cols * K * N <= 150000000 && cols * K <= 3500 * mx_vec_waves(K, N, 1))) && mx_vec_chunk(K, cols) >= cols;
+}
 bool mx_id_vec_takes(int64_t K, int64_t N, int64_t cols) { return (cols <= 24 || (cols <= 64 && cols * K * N <= 100000000)) && mx_vec_chunk(K, cols) >= 1; }
 // rows of whole steps, every one at a whole dword
 static bool mx_dwords(const mx_mm & p) { return p.blocks % 4 == 0 && p.nb1 % 4 == 0 && p.nb2 % 4 == 0 && ((uintptr_t) p.w & 3) == 0; }
@@ -1048,7 +1044,7 @@ static bool mx_pieces(const mx_mm & p) { return p.blocks % 16 == 0 && p.nb1 % 16
 static void mx_launch_vec(hipStream_t s, const mx_mm & p, const tdesc & b, const tdesc * ids) {
     const int64_t K = b.ne[0];
     const int chunk = mx_vec_chunk(K, p.cols);
-    const dim3 block((unsigned) (64 * mx_vec_waves(K)));
+    const dim3 block((unsigned) (64 * mx_vec_waves(K, p.n_rows, ids ? p.cols : 1)));
     const unsigned rows = (unsigned) ((p.n_rows + 15) / 16);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(rows, ids ? (unsigned) p.cols : 1u), block, mx_vec_lds(K, chunk), s, p, b, ids ? *ids : b, chunk); };
     const bool dw = mx_dwords(p);
