@@ -313,7 +313,12 @@ template <class Put> __device__ __forceinline__ uint32_t mx_act_quad(const mx_f4
 template <bool ID> __global__ void __launch_bounds__(256) k_mx_act(const tdesc b, const int64_t n_cols, const mx_lists l, const int n_used, uint8_t * __restrict__ act, const int steps) {
     __shared__ __align__(16) uint8_t s[MX_ACT_STEP];
     const int step = blockIdx.x, group = blockIdx.y, tid = threadIdx.x;
-    if (ID && group >= l.total[0]) return;
+    int listed[2];
+    if (ID) {  // (requested together; behind the groups in use the list's room holds anything)
+        listed[0] = l.list[group * 32 + (tid >> 4)];
+        listed[1] = l.list[group * 32 + 16 + (tid >> 4)];
+        if (group >= l.total[0]) return;
+    }
     const int i = tid & 3, blk = (tid >> 2) & 3;
     const int64_t k0 = (int64_t) step * 128 + blk * 32;
     mx_f4 v[2][2];
@@ -322,7 +327,7 @@ template <bool ID> __global__ void __launch_bounds__(256) k_mx_act(const tdesc b
         int c = group * 32 + r * 16 + (tid >> 4);
         const char * col;
         if (ID) {
-            c = l.list[c];
+            c = listed[r];
             col = b.data + ((c % n_used) % (int) b.ne[1]) * b.nb[1] + (int64_t) (c / n_used) * b.nb[2];
         } else {
             const uint32_t n1 = (uint32_t) b.ne[1], n2 = (uint32_t) b.ne[2], c2 = (uint32_t) c / n1, c3 = c2 / n2;
@@ -628,8 +633,16 @@ __device__ __forceinline__ bool mx_tile_of(const mx_mm & p, const int row_tiles,
     tile = 4 * band + in - rt * width;
     return rt < row_tiles;
 }
+// MUL_MAT_ID: a tile of columns and all of its row tiles to one die, whose L2 then serves its digits; the tiles go to the dies in turn (us, row tiles to the dies in turn | tiles: 2048 tokens of 128 experts,
+// 8 each, of 1536 x 2048 199 | 189, 600 of 32, 4 each, of 1024 x 1024 29.6 | 27.6, 1000 of 4096 x 2048 115 | 117)
+__device__ __forceinline__ void mx_id_tile_of(const int row_tiles, int & rt, int & tile) {
+    const int at = (int) (blockIdx.x >> 3);
+    rt = at % row_tiles;
+    tile = at / row_tiles * 8 + (int) (blockIdx.x & 7);
+}
 // A wave's 32 RT rows by 32 columns to their places, by way of LDS of its own (mx_store_floats): a column's rows lie side by side there and leave in runs of 128 RT bytes, where a lane's own four would
-// go out 16 bytes here and there (1000 tokens of 32 experts, rows with a bias, four bytes at a time: 172 us)
+// go out 16 bytes here and there (1000 tokens of 32 experts, rows with a bias, four bytes at a time: 172 us).  The result is not for this kernel's L2, which would write it back all at once at the end (2048
+// columns of 4096 x 16384 187 us, past it 170)
 template <int RT> constexpr int mx_store_floats() { return 32 * (32 * RT + 4); }
 template <bool ID, int RT> __device__ __forceinline__ void mx_store_tile(const mx_mm & p, const mx_f16 (&acc)[RT], const int group, const int row0, const int e, const int lane, float * lds) {
     constexpr int ROWS = 32 * RT, RUN = ROWS / 4, COLS = 64 / RUN;  // lanes of a column, columns at a time
@@ -655,7 +668,7 @@ template <bool ID, int RT> __device__ __forceinline__ void mx_store_tile(const m
         if (bias) v += bv;
         if (to < 0) continue;
         float * d = p.dst + to * p.ldd + row;
-        if (whole && row + 4 <= p.n_rows) *(mx_f4 *) d = v;
+        if (whole && row + 4 <= p.n_rows) __builtin_nontemporal_store(v, (mx_f4 *) d);
         else
 #pragma unroll
             for (int k = 0; k < 4; ++k)
@@ -675,8 +688,7 @@ template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, RT ==
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r32 = lane & 31, half = lane >> 5;
     int rt, tile;
     if (ID) {
-        rt = blockIdx.x % row_tiles;
-        tile = blockIdx.x / row_tiles;
+        mx_id_tile_of(row_tiles, rt, tile);
     } else {
         if (!mx_tile_of(p, row_tiles, rt, tile)) return;
     }
@@ -800,12 +812,22 @@ template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, RT ==
     }
     take_x();
     __syncthreads();
+    if (!live) {  // a wave without columns: its share of the weights alone, with the barriers of the others
+        for (int step = 0, buf = 0; step < p.steps; ++step, buf ^= 1) {
+#pragma unroll
+            for (int i = 0; i < RT / 2; ++i) {
+                store_w(i, buf ^ 1);
+                fetch_w(i, min(step + 2, last));
+            }
+            __syncthreads();
+        }
+        return;
+    }
     for (int step = 0, buf = 0; step < p.steps; ++step, buf ^= 1) {
         multiply(buf, step);
         take_x();
         __syncthreads();
     }
-    if (!live) return;
     // (behind the loop's last barrier: nobody reads the stages any more)
     constexpr int PART = RT < 4 ? RT : 4;
     float * out = (float *) lds + wave * mx_store_floats<PART>();
@@ -834,6 +856,7 @@ template <int RT> struct mx_wide_args {
     uint32_t jump, wrap;
     const uint8_t * x;    // the group's digits
     int stages, wave, lane;
+    bool idle;            // a wave without columns
 };
 // one wave's share of a tile: quarter 2 half + ODD of every stage
 template <int RT, int ODD> __device__ __forceinline__ void mx_wide_sum(const mx_wide_args<RT> & p, uint8_t * lds, mx_f16 (&acc)[RT]) {
@@ -885,6 +908,15 @@ template <int RT, int ODD> __device__ __forceinline__ void mx_wide_sum(const mx_
     };
 #pragma unroll
     for (int n = 0; n < PIECES; ++n) dma(n, 0, 0);
+    if (p.idle) {  // its share of the weights alone, with the barriers of the others (1000 tokens of 32 experts: 116 us with products of a neighbour's digits, 107)
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        for (int stage = 0, buf = 0; stage < p.stages; ++stage, buf ^= 1) {
+#pragma unroll
+            for (int n = 0; n < PIECES; ++n) dma(n, min(stage + 1, p.stages - 1), buf ^ 1);
+            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < 3; ++i)
 #pragma unroll
@@ -949,8 +981,7 @@ template <bool ID, int RT> __global__ void __launch_bounds__(512, 2) k_mx_wide(c
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int rt, tile;
     if (ID) {
-        rt = blockIdx.x % row_tiles;
-        tile = blockIdx.x / row_tiles;
+        mx_id_tile_of(row_tiles, rt, tile);
     } else {
         if (!mx_tile_of(p, row_tiles, rt, tile)) return;
     }
@@ -973,6 +1004,7 @@ template <bool ID, int RT> __global__ void __launch_bounds__(512, 2) k_mx_wide(c
     q.wrap = (uint32_t) p.nb1 - 272u;
     q.x = p.act + (int64_t) min(group, groups - 1) * p.steps * MX_ACT_STEP;
     q.stages = p.steps / 4;
+    q.idle = group >= groups;
     q.wave = wave;
     q.lane = lane;
     mx_f16 acc[RT];
@@ -1054,7 +1086,7 @@ static void mx_launch_vec(hipStream_t s, const mx_mm & p, const tdesc & b, const
 }
 template <bool ID, int RT> static void mx_launch_tile_of(hipStream_t s, const mx_mm & p, int64_t col_tiles) {
     const int row_tiles = (p.n_rows + 32 * RT - 1) / (32 * RT);
-    const dim3 grid((unsigned) ((row_tiles * col_tiles + 7) / 8 * 8));
+    const dim3 grid((unsigned) (ID ? (col_tiles + 7) / 8 * 8 * row_tiles : (row_tiles * col_tiles + 7) / 8 * 8));
     if (mx_pieces(p) && p.n_rows >= 32 * RT) {
         constexpr size_t lds = std::max<size_t>(2 * mx_wide_pieces<RT>() * 8192, 8 * 4 * mx_store_floats<RT / 2>());
         static std::atomic<uint32_t> done{0};
