@@ -140,9 +140,9 @@ __global__ void __launch_bounds__(256) k_mx_read_dense(const uint8_t * __restric
         if (blk < n) mx_put8(out + (b0 + blk) * 128, i, *(const mx_u32_a1 *) (s + blk * MX_BLOCK + 1 + 4 * i), mx_scale(s[blk * MX_BLOCK]));
     }
 }
-// the launches' sizes: rows, 64 blocks of a row each
+// the launches' sizes: rows, 64 blocks of a row each (a launch has less than 2^32 threads in x)
 static dim3 mx_rows_grid(const tdesc & t) { return dim3((unsigned) (t.ne[1] * t.ne[2] * t.ne[3]), (unsigned) ((t.ne[0] / 32 + 63) / 64)); }
-bool mx_rows_ok(const tdesc & f32) { return f32.ne[1] * f32.ne[2] * f32.ne[3] < ((int64_t) 1 << 31) && f32.ne[0] / 32 <= 64 * 65535; }
+bool mx_rows_ok(const tdesc & f32) { return f32.ne[1] * f32.ne[2] * f32.ne[3] < ((int64_t) 1 << 24) && f32.ne[0] / 32 <= 64 * 65535; }
 void launch_mx_store(hipStream_t s, const tdesc & a, const tdesc * idx, const tdesc & d) {
     const int64_t n = (a.ne[0] / 32) * a.ne[1] * a.ne[2] * a.ne[3];
     if (n <= 0) return;
@@ -535,90 +535,77 @@ template <bool ID, bool DW> __global__ void __launch_bounds__(512, DW ? 3 : 2) k
     }
 }
 
-// ---- up to a few groups of columns: 32 rows by CT groups a workgroup, its waves take two steps in turn, everything straight from memory; the waves' sums are added in LDS in their order
-template <bool ID, int CT, bool DW> __global__ void __launch_bounds__(512) k_mx_few(const mx_mm p) {
+// ---- a few groups of columns: 32 rows by one group a workgroup, its waves take two steps in turn, everything straight from memory; the waves' sums are added in LDS in their order
+template <bool ID, bool DW> __global__ void __launch_bounds__(512) k_mx_few(const mx_mm p) {
     extern __shared__ __align__(16) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, r32 = lane & 31, half = lane >> 5;
-    const int group0 = blockIdx.y * CT, row0 = (int) blockIdx.x * 32;
+    const int group = blockIdx.y, row0 = (int) blockIdx.x * 32;
     int e = 0;
     if (ID) {
-        if (group0 >= p.l.total[0]) return;
-        e = p.l.owner[group0];
+        if (group >= p.l.total[0]) return;
+        e = p.l.owner[group];
     }
     const uint8_t * w = p.w + (int64_t) e * p.nb2 + (int64_t) min(row0 + r32, p.n_rows - 1) * p.nb1;
-    const uint8_t * x = p.act + (int64_t) group0 * p.steps * MX_ACT_STEP;
-    const int64_t group_bytes = (int64_t) p.steps * MX_ACT_STEP;
-    bool live[CT];  // the lane's columns
+    const uint8_t * x = p.act + (int64_t) group * p.steps * MX_ACT_STEP;
+    const bool live = ID ? p.l.list[group * 32 + r32] >= 0 : (int64_t) group * 32 + r32 < p.cols;  // the lane's column
+    mx_f16 acc;
 #pragma unroll
-    for (int c = 0; c < CT; ++c) live[c] = ID ? p.l.list[(group0 + c) * 32 + r32] >= 0 : (int64_t) (group0 + c) * 32 + r32 < p.cols;
-    mx_f16 acc[CT];
-#pragma unroll
-    for (int c = 0; c < CT; ++c)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
+    for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
     const int last = p.steps - 1, stride = 2 * waves;
-    mx_raw<DW> f0, f1;  // the weights of two turns (of one, with two groups of columns)
-    mx_i8 h[CT][4], l[CT][4];
-    uint32_t sx[CT];
+    mx_raw<DW> f0, f1;  // the weights of two turns
+    mx_i8 h[4], l[4];
+    uint32_t sx;
     auto fetch_x = [&](const int step) {
+        sx = 0x7F7F7F7Fu;
 #pragma unroll
-        for (int c = 0; c < CT; ++c) {
-            sx[c] = 0x7F7F7F7Fu;
+        for (int j = 0; j < 4; ++j) h[j] = l[j] = mx_i8{0, 0, 0, 0, 0, 0, 0, 0};
+        if (live && step <= last) {
+            const uint8_t * xs = x + (int64_t) step * MX_ACT_STEP;
+            sx = *(const uint32_t *) (xs + 4 * MX_ACT_BLK + r32 * 4);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) h[c][j] = l[c][j] = mx_i8{0, 0, 0, 0, 0, 0, 0, 0};
-            if (live[c] && step <= last) {
-                const uint8_t * xs = x + c * group_bytes + (int64_t) step * MX_ACT_STEP;
-                sx[c] = *(const uint32_t *) (xs + 4 * MX_ACT_BLK + r32 * 4);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint8_t * xb = xs + j * MX_ACT_BLK;
-                    h[c][j] = mx_op6(*(const mx_i4 *) (xb + r32 * 16), *(const mx_i2 *) (xb + 1024 + r32 * 8));
-                    l[c][j] = mx_op6(*(const mx_i4 *) (xb + 512 + r32 * 16), *(const mx_i2 *) (xb + 1280 + r32 * 8));
-                }
+            for (int j = 0; j < 4; ++j) {
+                const uint8_t * xb = xs + j * MX_ACT_BLK;
+                h[j] = mx_op6(*(const mx_i4 *) (xb + r32 * 16), *(const mx_i2 *) (xb + 1024 + r32 * 8));
+                l[j] = mx_op6(*(const mx_i4 *) (xb + 512 + r32 * 16), *(const mx_i2 *) (xb + 1280 + r32 * 8));
             }
         }
     };
     int step = wave * 2 + half;
     f0.load(w, min(step, last), p.blocks);
-    if (CT == 1) f1.load(w, min(step + stride, last), p.blocks);
+    f1.load(w, min(step + stride, last), p.blocks);
     fetch_x(step);
     auto turn = [&](mx_raw<DW> & f) {
         mx_i4 a[4];
         int sw[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) f.place(j, a[j], sw[j]);
-        f.load(w, min(step + (CT == 1 ? 2 : 1) * stride, last), p.blocks);
+        f.load(w, min(step + 2 * stride, last), p.blocks);
         step += stride;
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-            const uint32_t sl = sx[c] - 0x04040404u;
-            MX_MFMA(32x32x64, acc[c], a[0], sw[0], 0, h[c][0], l[c][0], sx[c], sl)
-            MX_MFMA(32x32x64, acc[c], a[1], sw[1], 1, h[c][1], l[c][1], sx[c], sl)
-            MX_MFMA(32x32x64, acc[c], a[2], sw[2], 2, h[c][2], l[c][2], sx[c], sl)
-            MX_MFMA(32x32x64, acc[c], a[3], sw[3], 3, h[c][3], l[c][3], sx[c], sl)
-        }
+        const uint32_t sl = sx - 0x04040404u;
+        MX_MFMA(32x32x64, acc, a[0], sw[0], 0, h[0], l[0], sx, sl)
+        MX_MFMA(32x32x64, acc, a[1], sw[1], 1, h[1], l[1], sx, sl)
+        MX_MFMA(32x32x64, acc, a[2], sw[2], 2, h[2], l[2], sx, sl)
+        MX_MFMA(32x32x64, acc, a[3], sw[3], 3, h[3], l[3], sx, sl)
         fetch_x(step);
     };
     for (int s0 = wave * 2; s0 < p.steps; s0 += stride) {  // (s0: the wave's, for both halves)
         turn(f0);
-        if (CT == 1 && (s0 += stride) < p.steps) turn(f1);
+        if ((s0 += stride) < p.steps) turn(f1);
     }
-    // [wave][group][column][row], the rows of a column 36 apart (of 32: no two quarters of a wave on the same banks)
+    // [wave][column][row], the rows of a column 36 apart (of 32: no two quarters of a wave on the same banks)
     float * part_sums = (float *) lds;
 #pragma unroll
-    for (int c = 0; c < CT; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) *(mx_f4 *) (part_sums + ((wave * CT + c) * 32 + r32) * 36 + 8 * i + 4 * half) = mx_f4{acc[c][4 * i], acc[c][4 * i + 1], acc[c][4 * i + 2], acc[c][4 * i + 3]};
+    for (int i = 0; i < 4; ++i) *(mx_f4 *) (part_sums + (wave * 32 + r32) * 36 + 8 * i + 4 * half) = mx_f4{acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]};
     __syncthreads();
     const float * bias = p.bias ? (const float *) ((const char *) p.bias + (int64_t) e * p.nb_bias) : nullptr;
-    for (int at = threadIdx.x; at < CT * 32 * 32; at += blockDim.x) {
-        const int row = at & 31, cg = at >> 5;  // column cg of the CT groups
-        int64_t c = (int64_t) group0 * 32 + cg;
+    for (int at = threadIdx.x; at < 32 * 32; at += blockDim.x) {
+        const int row = at & 31, cg = at >> 5;
+        int64_t c = (int64_t) group * 32 + cg;
         if (ID) c = p.l.list[c];
         else if (c >= p.cols) c = -1;
         if (c < 0 || row0 + row >= p.n_rows) continue;
         float v = 0.0f;
-        for (int k = 0; k < waves; ++k) v += part_sums[(k * CT * 32 + cg) * 36 + row];
+        for (int k = 0; k < waves; ++k) v += part_sums[(k * 32 + cg) * 36 + row];
         p.dst[c * p.ldd + row0 + row] = bias ? v + bias[row0 + row] : v;
     }
 }
@@ -974,7 +961,8 @@ template <int RT, int ODD> __device__ __forceinline__ void mx_wide_sum(const mx_
         sx = sxn;
     }
 }
-template <bool ID, int RT> __global__ void __launch_bounds__(512, 2) k_mx_wide(const mx_mm p, const int row_tiles) {
+// (RT = 2: two workgroups a CU, 10 tokens of 32 experts of 2048 x 4096 44 us, one 57)
+template <bool ID, int RT> __global__ void __launch_bounds__(512, RT == 2 ? 4 : 2) k_mx_wide(const mx_mm p, const int row_tiles) {
     constexpr int ROWS = 32 * RT, PIECES = mx_wide_pieces<RT>();
     static_assert(PIECES <= 9, "a lane's pieces leave their row once");
     extern __shared__ __align__(16) uint8_t lds[];  // two stages of [row] 272 bytes
@@ -1061,14 +1049,21 @@ static int mx_vec_chunk(int64_t K, int64_t cols) {
     while (c > 0 && mx_vec_lds(K, c) > MX_VEC_LDS) --c;
     return (int) c;
 }
-static constexpr int64_t MX_FEW_COLS = 64;
-// Every workgroup quantises its columns: a launch less (two with MUL_MAT_ID), for work that grows with columns and rows.  us, k_mx_vec | k_mx_few: 2 / 4 columns of 14336 x 4096 13.5 / 18.4 | 17.3 / 17.4, of
-// 4096 x 14336 13.0 / 20.3 (two at a time) | 20.2 / 20.3, 4 / 8 of 4096 x 4096 7.1 / 10.0 | 11.8 / 11.9, of 5632 x 2048 6.7 / 9.6 | 9.1 / 9.1, 8 / 16 of 1024 x 1024 5.2 / 6.4 | 7.7 / 8.1; expert columns, of 32
-// experts of 4096 x 4096: 16 / 24 / 32 of them 36.8 / 46.5 / 59.0 | 42.2 / 45.7 / 57.9, of 1024 x 1024 32 9.3 | 15.2
-bool mx_vec_takes(int64_t K, int64_t N, int64_t cols) {
-    return (cols == 1 || (cols <= 16 && cols * K * N <= 150000000 && cols * K <= 3500 * mx_vec_waves(K, N, 1))) && mx_vec_chunk(K, cols) >= cols;
+// Costs of a product by k_mx_few and in tiles of 32 rt rows, in quarters of a us at 4096 values a row: 256 workgroups at a time, a tile's by its groups of columns.  What they compare, us, k_mx_few | tiles of 64
+// rows: 32 columns of 4096 x 14336 18.8 | 14.4, of 4096 x 32000 30.4 | 18.6, of 14336 x 8192 23.3 | 29.0, 64 of 4096 x 4096 11.8 | 14.7, 128 17.9 | 19.5, 256 29.7 | 21.2; 4 / 18 columns an expert, 32 experts
+// of 2048 x 4096 49 / 87 | 36 / 58, 8 of 2080 x 512 16.0 | 18.7.  Tiles of 64 | 128 | 256 rows: 256 columns of 4096 x 14336 35.9 | 26.6 | 34.8, 384 51.5 | 47.6 | 37.5
+static int64_t mx_few_cost(int64_t N, int64_t groups) { return ((N + 31) / 32 * groups + 255) / 256 * 22; }
+static int64_t mx_tile_cost(int rt, int64_t N, int64_t tiles, int64_t groups) {
+    const int64_t rounds = ((N + 32 * rt - 1) / (32 * rt) * tiles + 255) / 256, g = std::min<int64_t>(groups, 4);
+    return rounds * (rt == 2 ? 20 + 9 * g : rt == 4 ? 47 + 11 * g : 70 + 17 * g);
 }
-bool mx_id_vec_takes(int64_t K, int64_t N, int64_t cols) { return (cols <= 24 || (cols <= 64 && cols * K * N <= 100000000)) && mx_vec_chunk(K, cols) >= 1; }
+// Every workgroup quantises its columns: a launch less (two with MUL_MAT_ID), for work that grows with columns and rows.  us, k_mx_vec | the faster of the others: 2 / 4 columns of 4096 x 14336 13.5 / 18.4 |
+// 13.7 / 13.7, 2 of 14336 x 4096 13.0 | 20.0, 4 / 8 of 4096 x 4096 6.9 / 10.0 | 11.6 / 11.6, of 2048 x 5632 6.6 / 9.5 | 8.9 / 8.8, of 2080 x 5000 8.5 / 12.3 | 10.7 / 10.5, 16 of 1024 x 1024 6.5 | 7.9; expert
+// columns, 16 / 24 of 32 experts of 2048 x 4096 25.0 / 31.5 | 25.9 / 26.8, of 4096 x 4096 35.5 / 45.7 | 36.7 / 39.2, 64 of 1024 x 1024 11.5 | 14.1, of 128 experts of 2048 x 768 20.1 | 21.7
+bool mx_vec_takes(int64_t K, int64_t N, int64_t cols) {
+    return (cols == 1 || (cols <= 16 && cols * K * N <= 150000000 && cols * K <= 4096 * mx_vec_waves(K, N, 1))) && mx_vec_chunk(K, cols) >= cols;
+}
+bool mx_id_vec_takes(int64_t K, int64_t N, int64_t cols) { return (cols <= 16 || (cols <= 64 && cols * K * N <= 110000000)) && mx_vec_chunk(K, cols) >= 1; }
 // rows of whole steps, every one at a whole dword
 static bool mx_dwords(const mx_mm & p) { return p.blocks % 4 == 0 && p.nb1 % 4 == 0 && p.nb2 % 4 == 0 && ((uintptr_t) p.w & 3) == 0; }
 // ... of whole 16-byte pieces
@@ -1098,20 +1093,23 @@ template <bool ID, int RT> static void mx_launch_tile_of(hipStream_t s, const mx
     if (mx_dwords(p)) hipLaunchKernelGGL((k_mx_tile<ID, RT, true>), grid, dim3(256), 0, s, p, row_tiles);
     else hipLaunchKernelGGL((k_mx_tile<ID, RT, false>), grid, dim3(256), 0, s, p, row_tiles);
 }
-template <bool ID> static void mx_launch_tile(hipStream_t s, const mx_mm & p, int64_t col_tiles) {
-    auto wide = [&](int rt) { return (p.n_rows + 32 * rt - 1) / (32 * rt) * col_tiles >= 192; };
-    if (wide(8)) mx_launch_tile_of<ID, 8>(s, p, col_tiles);
-    else if (wide(4)) mx_launch_tile_of<ID, 4>(s, p, col_tiles);
-    else mx_launch_tile_of<ID, 2>(s, p, col_tiles);
+template <bool ID> static void mx_launch_tile(hipStream_t s, const mx_mm & p, int64_t tiles, int rt) {
+    if (rt == 8) mx_launch_tile_of<ID, 8>(s, p, tiles);
+    else if (rt == 4) mx_launch_tile_of<ID, 4>(s, p, tiles);
+    else mx_launch_tile_of<ID, 2>(s, p, tiles);
+}
+static int mx_tile_rows(int64_t N, int64_t tiles, int64_t groups) {
+    const int64_t c2 = mx_tile_cost(2, N, tiles, groups), c4 = mx_tile_cost(4, N, tiles, groups), c8 = mx_tile_cost(8, N, tiles, groups);
+    return c8 <= c4 && c8 <= c2 ? 8 : c4 <= c2 ? 4 : 2;
 }
 // Four waves where the rows and groups alone fill the GPU, eight where they do not (us for 8 / 32 columns, four waves | eight: 4096 rows of 14336 18.3 / 21.2 | 18.6 / 20.3, 14336 of 4096 15.4 / 17.1 |
 // 17.4 / 18.5; 10 / 125 tokens of 32 experts of 4096 x 2048 32.8 / 71.5 | 43.9 / 90.1)
-template <bool ID, int CT> static void mx_launch_few(hipStream_t s, const mx_mm & p, int64_t groups) {
-    const int waves = CT == 1 && (p.n_rows + 31) / 32 * groups < 256 ? 8 : 4;
+template <bool ID> static void mx_launch_few(hipStream_t s, const mx_mm & p, int64_t groups) {
+    const int waves = (p.n_rows + 31) / 32 * groups < 256 ? 8 : 4;
     const dim3 grid((unsigned) ((p.n_rows + 31) / 32), (unsigned) groups), block((unsigned) (64 * waves));
-    const size_t lds = (size_t) waves * CT * 32 * 36 * 4;
-    if (mx_dwords(p)) hipLaunchKernelGGL((k_mx_few<ID, CT, true>), grid, block, lds, s, p);
-    else hipLaunchKernelGGL((k_mx_few<ID, CT, false>), grid, block, lds, s, p);
+    const size_t lds = (size_t) waves * 32 * 36 * 4;
+    if (mx_dwords(p)) hipLaunchKernelGGL((k_mx_few<ID, true>), grid, block, lds, s, p);
+    else hipLaunchKernelGGL((k_mx_few<ID, false>), grid, block, lds, s, p);
 }
 // act: null where mx_vec_takes
 void launch_mx_mul_mat(hipStream_t s, const tdesc & w, const tdesc & b, const tdesc & d, const void * act) {
@@ -1119,9 +1117,11 @@ void launch_mx_mul_mat(hipStream_t s, const tdesc & w, const tdesc & b, const td
     p.act = (const uint8_t *) act;
     if (p.n_rows == 0 || p.cols == 0) return;
     if (!act) mx_launch_vec(s, p, b, nullptr);
-    else if (p.cols <= 32) mx_launch_few<false, 1>(s, p, 1);
-    else if (p.cols <= MX_FEW_COLS) mx_launch_few<false, 2>(s, p, 1);
-    else mx_launch_tile<false>(s, p, (p.cols + 127) / 128);
+    else {
+        const int64_t groups = (p.cols + 31) / 32, tiles = (p.cols + 127) / 128;
+        if (mx_few_cost(p.n_rows, groups) < mx_tile_cost(2, p.n_rows, tiles, groups)) mx_launch_few<false>(s, p, groups);
+        else mx_launch_tile<false>(s, p, tiles, mx_tile_rows(p.n_rows, tiles, groups));
+    }
 }
 void launch_mx_mul_mat_id(hipStream_t s, const tdesc & w, const tdesc & b, const tdesc & ids, const tdesc & d, const void * ws, const float * bias, int64_t nb_bias) {
     const int64_t cols = ids.ne[0] * ids.ne[1], g = mx_id_groups(w.ne[2], cols);
@@ -1132,16 +1132,26 @@ void launch_mx_mul_mat_id(hipStream_t s, const tdesc & w, const tdesc & b, const
     if (!ws) return mx_launch_vec(s, p, b, &ids);
     p.act = (const uint8_t *) ws + mx_lists_bytes(g);
     p.l = mx_lists_at((void *) ws, g);
-    if (cols <= 32 * w.ne[2]) mx_launch_few<true, 1>(s, p, g);
-    else mx_launch_tile<true>(s, p, mx_id_tiles(w.ne[2], cols));
+    // With fewer than 64 columns an expert the weights' way from memory counts for more than the products: tiles of 256 rows where there are two rounds of them, of 64 (two workgroups a CU) elsewhere.  us, 64 |
+    // 256 rows, 10 / 28 columns an expert: 32 experts of 2048 x 4096 44 / 68 | 46 / 56, of 1024 x 1024 15.7 / 19.6 | 20.6 / 23.4, 128 of 2048 x 768 40 / 51 | 48 / 55
+    const int64_t tiles = mx_id_tiles(w.ne[2], cols), each = cols / w.ne[2];
+    if (mx_few_cost(p.n_rows, g) < mx_tile_cost(2, p.n_rows, tiles, each / 32 + 1)) mx_launch_few<true>(s, p, g);
+    else if (each >= 64) mx_launch_tile<true>(s, p, tiles, mx_tile_rows(p.n_rows, tiles, 4));
+    else mx_launch_tile<true>(s, p, tiles, each >= 16 && p.n_rows / 256 * tiles >= 512 ? 8 : 2);
 }
-// which operands the products take (type and shape; the rows of both are dense, whole blocks)
+// Which operands the products take (type and shape; the rows of both are dense, whole blocks).  The kernels hold offsets inside a tile of 256 rows and inside a group's digits in 32 bits, and a launch less than
+// 2^32 threads in x
+static constexpr int64_t MX_MAX_ROW = 1 << 23;  // bytes between rows
+static bool mx_grid_ok(int64_t N, int64_t tiles) { return N < (1 << 26) && (N + 63) / 64 * (tiles + 7) < (1 << 22); }
 bool mx_product_ok(const tdesc & w, const tdesc & b) {
-    return w.ne[0] % 32 == 0 && w.ne[0] > 0 && w.ne[1] < ((int64_t) 1 << 31) - 256 && w.ne[0] < ((int64_t) 1 << 31) - 256 && w.nb[0] == MX_BLOCK && b.nb[0] == 4 && b.nb[1] % 4 == 0 && b.nb[2] % 4 == 0 && b.nb[3] % 4 == 0 &&
-           (b.ne[1] * b.ne[2] * b.ne[3] + 31) / 32 <= 65535;
+    const int64_t cols = b.ne[1] * b.ne[2] * b.ne[3];
+    return w.ne[0] % 32 == 0 && w.ne[0] > 0 && w.nb[0] == MX_BLOCK && w.ne[0] / 32 * MX_BLOCK <= MX_MAX_ROW && (int64_t) w.nb[1] <= MX_MAX_ROW && b.nb[0] == 4 && b.nb[1] % 4 == 0 && b.nb[2] % 4 == 0 &&
+           b.nb[3] % 4 == 0 && (cols + 31) / 32 <= 65535 && mx_grid_ok(w.ne[1], (cols + 127) / 128);
 }
 bool mx_id_ok(const tdesc & w, const tdesc & ids) {
-    return w.ne[2] <= MX_MAX_EXPERTS && ids.nb[0] % 4 == 0 && ids.nb[1] % 4 == 0 && ids.ne[0] * ids.ne[1] < ((int64_t) 1 << 30) && ids.ne[0] > 0 && mx_id_groups(w.ne[2], ids.ne[0] * ids.ne[1]) <= 65535;
+    const int64_t cols = ids.ne[0] * ids.ne[1];
+    return w.ne[2] > 0 && w.ne[2] <= MX_MAX_EXPERTS && ids.nb[0] % 4 == 0 && ids.nb[1] % 4 == 0 && ids.ne[0] > 0 && ids.ne[2] == 1 && ids.ne[3] == 1 && cols < ((int64_t) 1 << 30) &&
+           mx_id_groups(w.ne[2], cols) <= 65535 && mx_grid_ok(w.ne[1], mx_id_tiles(w.ne[2], cols));
 }
 
 // ------------------------------------------------------------------------------------------------ ADD_ID

@@ -90,3 +90,21 @@ def test_expert_products_taken_and_refused(ask, g):
     bad = g.add_id(y, g.new(L.F32, 40, 8), ids)
     bad.contents.src[2].contents.ne[0] = 2
     assert not ask(bad)                                                            # an id for every row
+
+
+def test_sizes_refused(ask, g):
+    """what the launches and the kernels' 32-bit offsets do not hold"""
+    x = g.new(L.F32, 96, 4)
+    assert not ask(g.mul_mat(g.new(L.MXFP4, 1 << 24, 2), g.new(L.F32, 1 << 24, 1)))        # rows of more than 8 MiB
+    far = g.new(L.MXFP4, 96, 50)
+    far.contents.nb[1] = (1 << 23) + 17
+    assert not ask(g.mul_mat(far, x))
+    far.contents.nb[1] = (1 << 23) - 3
+    assert ask(g.mul_mat(far, x))
+    assert not ask(g.mul_mat(g.new(L.MXFP4, 96, 1 << 26), x))                              # rows, and rows times columns
+    assert not ask(g.mul_mat(g.new(L.MXFP4, 96, 1 << 20), g.new(L.F32, 96, 1 << 18)))
+    assert not ask(g.set_rows(g.new(L.MXFP4, 32, 50), g.new(L.F32, 32, 1 << 24), g.new(L.I64, 1 << 24)))
+    w, one = g.new(L.MXFP4, 64, 40, 8), g.new(L.F32, 64, 1, 5)
+    y = g.mul_mat_id(w, one, g.new(L.I32, 3, 5))
+    y.contents.src[0].contents.ne[2] = 0                                                   # no experts
+    assert not ask(y)
