@@ -939,7 +939,7 @@ static bool quant_consumers_only(const exec_state & st, int at, const ggml_tenso
     if (n_cons == 0 || n_cons != use_count(st, t)) return false;
     for (int j = at + 1; j <= last; ++j) {
         const ggml_tensor * u = g->nodes[j];
-        if (u->op == GGML_OP_MUL_MAT && is_quant(u->src[0]->type) && u->src[1] != t) return false;
+        if (u->op == GGML_OP_MUL_MAT && (is_quant(u->src[0]->type) || u->src[0]->type == GGML_TYPE_MXFP4) && u->src[1] != t) return false;
         if (u->op == GGML_OP_MUL_MAT_ID) return false;
     }
     return true;
@@ -968,7 +968,7 @@ static bool q80_panel_consumers_only(const exec_state & st, int at, const ggml_t
     if (n_cons == 0 || n_cons != use_count(st, t)) return false;
     for (int j = at + 1; j <= last; ++j) {  // (the activation area is shared: no other quantised mat-mul may run before the last reader)
         const ggml_tensor * u = g->nodes[j];
-        if (u->op == GGML_OP_MUL_MAT && is_quant(u->src[0]->type) && u->src[1] != t) return false;
+        if (u->op == GGML_OP_MUL_MAT && (is_quant(u->src[0]->type) || u->src[0]->type == GGML_TYPE_MXFP4) && u->src[1] != t) return false;
         if (u->op == GGML_OP_MUL_MAT_ID) return false;
     }
     return true;
@@ -2974,9 +2974,10 @@ static int run_mul_mat_id_mx(exec_state & st, int i) {
         st.mx_ids = ids;
         st.mx_experts = a->ne[2];
     }
-    // (the bias: the result alone reads the product, of the same ids, and is not stored over what the launch still reads)
+    // (the bias: the result alone reads the product, of the same ids, has a row for every expert, and is not stored over what the launch still reads — src1 itself where it makes the digits)
     ggml_tensor * ad = i + 1 < g->n_nodes && !st.done[i + 1] ? g->nodes[i + 1] : nullptr;
-    const bool bias = c->opt.fusion && ad && ad->op == GGML_OP_ADD_ID && ad->src[0] == n && ad->src[2] == ids && single_use(st, n) && is_f32_contig(ad) && supports_op(ad) && !ranges_overlap(ad, ad->src[1]) && !ranges_overlap(ad, ids);
+    const bool bias = c->opt.fusion && ad && ad->op == GGML_OP_ADD_ID && ad->src[0] == n && ad->src[2] == ids && single_use(st, n) && is_f32_contig(ad) && supports_op(ad) && ad->src[1]->ne[1] >= a->ne[2] &&
+                      !ranges_overlap(ad, ad->src[1]) && !ranges_overlap(ad, ids) && (ws || !ranges_overlap(ad, b));
     timed_scope ts(c, "mul_mat_id_mxfp4", (double) ggml_abi_nbytes(a) / (double) std::max<int64_t>(1, a->ne[2]) * (double) std::min<int64_t>(a->ne[2], ggml_abi_nelements(ids)));
     launch_mx_mul_mat_id(c->stream, TD(a), TD(b), TD(ids), TD(bias ? ad : n), ws, bias ? (const float *) ad->src[1]->data : nullptr, bias ? (int64_t) ad->src[1]->nb[1] : 0);
     c->st.kernel_launches++;

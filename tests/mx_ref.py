@@ -68,10 +68,10 @@ def experts(x, w, ids, bias=None):
     """x [T, 1 or U, K], w [E, N, packed], ids [T, U] -> (float64 [T, U, N], magnitudes); NaN rows of zeros magnitude where the id names no expert"""
     T, U = ids.shape
     y, m = np.zeros((T, U, w.shape[1])), np.zeros((T, U, w.shape[1]))
-    for t in range(T):
-        for u in range(U):
-            if 0 <= ids[t, u] < w.shape[0]:
-                y[t, u], m[t, u] = product(x[t, u % x.shape[1]], w[ids[t, u]])
-                if bias is not None:
-                    y[t, u] += bias[ids[t, u]].astype(np.float64)
+    for e in range(w.shape[0]):
+        t, u = np.nonzero(ids == e)
+        if len(t):
+            y[t, u], m[t, u] = product(x[t, u % x.shape[1]], w[e])
+            if bias is not None:
+                y[t, u] += bias[e].astype(np.float64)
     return y, m

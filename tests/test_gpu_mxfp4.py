@@ -74,6 +74,26 @@ def test_convert_sizes(backend, rows):
     assert np.array_equal(back.reshape(-1, 160), mx_ref.values(mx_ref.quantise(x)).astype(np.float32))
 
 
+@pytest.mark.parametrize("first", [1, 16])
+def test_convert_in_place_of_rows(backend, first):
+    """some rows of a table written and read back: blocks that start at any byte"""
+    r = rng_of(33, first)
+    K, R, n = 96, 40, 9
+    table, x = weights(r, R, K), acts(r, n, K)
+
+    def build(g):
+        H = g.H
+        t = g.new(L.MXFP4, (K, R), table)
+        put = H.ggml_cpy(g.ctx, g.new(L.F32, (K, n), x), H.ggml_view_2d(g.ctx, t, K, n, t.contents.nb[1], first * t.contents.nb[1]))
+        return [H.ggml_cast(g.ctx, put, L.F32), H.ggml_cast(g.ctx, H.ggml_view_2d(g.ctx, t, K, R - 1, t.contents.nb[1], t.contents.nb[1]), L.F32)]
+
+    part, rest = T.run_case(build, backend)
+    want = table.copy()
+    want[first:first + n] = mx_ref.quantise(x)
+    assert np.array_equal(part.reshape(n, K), mx_ref.values(want[first:first + n]).astype(np.float32))
+    assert np.array_equal(rest.reshape(R - 1, K), mx_ref.values(want[1:]).astype(np.float32))
+
+
 @pytest.mark.parametrize("scale", [0, 1, 2, 127, 253, 254, 255])
 def test_every_code(backend, scale):
     codes = np.arange(16, dtype=np.uint8)
@@ -202,6 +222,33 @@ def test_product_strided_and_batched_activations(backend):
     mx_ref.check("permuted", b, want.swapaxes(1, 2), mags.swapaxes(1, 2), K)
 
 
+# rows and columns that take tiles of 64, 128 and 256 rows; K: whole 16-byte pieces, whole dwords, anything
+@pytest.mark.parametrize("N,M", [(1001, 600), (2083, 1000), (4129, 1000)])
+@pytest.mark.parametrize("K", [1024, 384, 160])
+def test_product_tiles(backend, K, N, M):
+    r = rng_of(34, K, N)
+    w, x = weights(r, N, K), acts(r, M, K)
+    want, mags = mx_ref.product(x, w)
+    mx_ref.check("tiles", mul_mat(backend, w, x, K, N, M), want, mags, K)
+
+
+@pytest.mark.parametrize("M", [1, 20, 700])
+def test_product_rows_far_apart(backend, M):
+    """a matrix that is some columns of a much wider one: its rows lie half a megabyte apart"""
+    r = rng_of(35, M)
+    K, N, wide = 512, 300, 1 << 20
+    w, x = weights(r, N, K), acts(r, M, K)
+    block = np.zeros((N, wide // 32 * 17), np.uint8)
+    block[:, 17 * 64:17 * 80] = w
+
+    def build(g):
+        m = g.new(L.MXFP4, (wide, N), block)
+        return g.H.ggml_mul_mat(g.ctx, g.H.ggml_view_2d(g.ctx, m, K, N, m.contents.nb[1], 17 * 64), g.new(L.F32, (K, M), x))
+
+    want, mags = mx_ref.product(x, w)
+    mx_ref.check("far", T.run_case(build, backend)[0].reshape(M, N), want, mags, K)
+
+
 def test_product_one_column_like_many(backend):
     """what a token gets does not hang on the kernel that its batch takes by more than the sums' roundings"""
     r = rng_of(14)
@@ -269,6 +316,51 @@ def test_experts(backend, K, N, E, U, Tn, shared, bias, plog):
     got = run_experts(backend, w, x, ids, b, K, N, view_ids=bias)
     rel = mx_ref.check("experts", got, want, mags, K, extra=np.abs(b[ids]) if bias else 0.0)
     plog(f"mxfp4 experts K={K} N={N} E={E} U={U} T={Tn}: rel {rel:.2e}")
+
+
+@pytest.mark.parametrize("N", [1001, 2083, 4129])
+@pytest.mark.parametrize("K", [1024, 384, 160])
+def test_experts_tiles(backend, K, N):
+    """tiles of 64, 128 and 256 rows; two experts, of which one has one column more than whole tiles"""
+    r = rng_of(36, K, N)
+    Tn = 900
+    w, x, b = weights(r, 2, N, K), acts(r, Tn, 1, K), r.standard_normal((2, N)).astype(np.float32)
+    ids = (np.arange(Tn) >= 385).astype(np.int32)[r.permutation(Tn)][:, None]
+    want, mags = mx_ref.experts(x, w, ids, b)
+    mx_ref.check("tiles", run_experts(backend, w, x, ids, b, K, N), want, mags, K, extra=np.abs(b[ids]))
+
+
+def test_bias_of_fewer_experts(backend):
+    """ids behind the bias rows' last: the product alone (ADD_ID), also where the two could be one launch"""
+    r = rng_of(37)
+    K, N, E, U, Tn = 128, 70, 6, 2, 40
+    w, x, ids, b = weights(r, E, N, K), acts(r, Tn, 1, K), choose(r, Tn, U, E), r.standard_normal((4, N)).astype(np.float32)
+
+    def build(g):
+        i = g.new(L.I32, (U, Tn), ids)
+        y = g.H.ggml_mul_mat_id(g.ctx, g.new(L.MXFP4, (K, N, E), w), g.new(L.F32, (K, 1, Tn), x), i)
+        return g.H.ggml_add_id(g.ctx, y, g.new(L.F32, (N, 4), b), i)
+
+    want, mags = mx_ref.experts(x, w, ids, np.concatenate([b, np.zeros((2, N), np.float32)]))
+    mx_ref.check("bias", T.run_case(build, backend)[0].reshape(Tn, U, N), want, mags, K, extra=np.abs(want))
+
+
+@pytest.mark.parametrize("Tn", [1, 60])
+def test_bias_result_in_the_activations_memory(backend, Tn):
+    """the block of activations that nobody reads any more taken for the sum with the bias, as the graph allocator does"""
+    r = rng_of(38, Tn)
+    K, N, E = 2048, 2048, 4
+    w, x, b = weights(r, E, N, K), acts(r, Tn, 1, K), r.standard_normal((E, N)).astype(np.float32)
+    ids = r.integers(0, E, (Tn, 1)).astype(np.int32)
+    g = T.G(backend)
+    try:
+        H, i, src = g.H, g.new(L.I32, (1, Tn), ids), g.new(L.F32, (K, 1, Tn), x)
+        y = H.ggml_add_id(g.ctx, H.ggml_mul_mat_id(g.ctx, g.new(L.MXFP4, (K, N, E), w), src, i), g.new(L.F32, (N, E), b), i)
+        got, = g.compute([y], same_block=[(y, src)])
+    finally:
+        g.free()
+    want, mags = mx_ref.experts(x, w, ids, b)
+    mx_ref.check("in place", got.reshape(Tn, 1, N), want, mags, K, extra=np.abs(b[ids]))
 
 
 @pytest.mark.parametrize("Tn", [1, 5, 90])
@@ -364,6 +456,65 @@ def test_fusion_off_gives_the_same(backend):
     finally:
         backend.set_option("fusion", 1)
     assert np.array_equal(np.asarray(a), np.asarray(b))
+
+
+@pytest.mark.parametrize("Tn", [1, 3, 40, 150])
+def test_feed_forward_of_a_dense_model(backend, Tn):
+    """norm -> gate, up -> SwiGLU -> down -> + input, alone in its graph (whatever is fused there) and with every stage kept: each product against 64 bits on what it was given"""
+    r = rng_of(39, Tn)
+    K, F = 512, 736
+    x, nw, gw, uw, dw = acts(r, Tn, K), r.standard_normal(K).astype(np.float32), weights(r, F, K), weights(r, F, K), weights(r, K, F)
+
+    def build(g, stages):
+        H, c = g.H, g.ctx
+        src = g.new(L.F32, (K, Tn), x)
+        n = H.ggml_mul(c, H.ggml_rms_norm(c, src, 1e-5), g.new(L.F32, (K,), nw))
+        gate, up = H.ggml_mul_mat(c, g.new(L.MXFP4, (K, F), gw), n), H.ggml_mul_mat(c, g.new(L.MXFP4, (K, F), uw), n)
+        act = H.ggml_swiglu_split(c, gate, up)
+        down = H.ggml_mul_mat(c, g.new(L.MXFP4, (F, K), dw), act)
+        return [H.ggml_add(c, down, src)] + ([n, gate, up, act, down] if stages else [])
+
+    y, n, gate, up, act, down = [np.asarray(o).reshape(Tn, -1) for o in T.run_case(lambda g: build(g, True), backend)]
+    for name, got, src, m, k in (("gate", gate, n, gw, K), ("up", up, n, uw, K), ("down", down, act, dw, F)):
+        want, mags = mx_ref.product(src, m)
+        mx_ref.check(name, got, want, mags, k)
+    assert np.array_equal(y, down + x)
+    alone, = T.run_case(lambda g: build(g, False), backend)
+    assert np.array_equal(np.asarray(alone).reshape(y.shape), y)
+
+
+@pytest.mark.parametrize("M", [1, 8, 40])
+@pytest.mark.parametrize("kind", [L.Q4_K, L.Q8_0])
+def test_between_products_of_other_formats(backend, kind, M):
+    """normed rows whose readers are products by another block format, and a product by an MXFP4 matrix between the two: both use the scratch for activations..
+    The other format moves an activation i by at most half a step of its block, d_i = top_i / 254 (blocks of 256 for Q4_K, 32 for Q8_0).  A sum of w_ji e_i with |e_i| <= d_i and no common sign has a
+    mean square of at most sum w_ji^2 d_i^2, so the whole is off by at most the 2-norm of sqrt(sum_i w_ji^2 d_i^2) (even steps would leave 1 / sqrt 3 of it): with the values twelve times the others
+    some tenth of the whole, where digits of the other product would leave nothing right."""
+    r = rng_of(40, M, kind)
+    K, N = 512, 256
+    x, z, nw, mw = acts(r, M, K), acts(r, M, K), r.standard_normal(K).astype(np.float32), weights(r, N, K)
+    ws = [T.rand_blocks(kind, N * K // L.TYPE_BLCK[kind], K, r) for _ in range(2)]
+
+    def build(g):
+        H, c = g.H, g.ctx
+        n = H.ggml_mul(c, H.ggml_rms_norm(c, g.new(L.F32, (K, M), x), 1e-5), g.new(L.F32, (K,), nw))
+        a = H.ggml_mul_mat(c, g.new(kind, (K, N), ws[0]), n)
+        m = H.ggml_mul_mat(c, g.new(L.MXFP4, (K, N), mw), g.new(L.F32, (K, M), z))
+        b = H.ggml_mul_mat(c, g.new(kind, (K, N), ws[1]), n)
+        return [a, m, b]
+
+    a, m, b = [np.asarray(o).reshape(M, N) for o in T.run_case(build, backend)]
+    want, mags = mx_ref.product(z, mw)
+    mx_ref.check("between", m, want, mags, K)
+    x64 = x.astype(np.float64)
+    n = x64 / np.sqrt((x64 * x64).mean(-1, keepdims=True) + 1e-5) * nw
+    for got, blocks in ((a, ws[0]), (b, ws[1])):
+        f = np.empty((N, K), np.float32)
+        T.oracle().oracle_dequantize_row(kind, np.ascontiguousarray(blocks).ctypes.data_as(C.c_void_p), f.ctypes.data_as(C.c_void_p), N * K)
+        f, size = f.astype(np.float64), 256 if kind == L.Q4_K else 32
+        d = np.repeat(np.abs(n).reshape(M, K // size, size).max(-1), size, axis=-1) / 254
+        want, off = n @ f.T, np.linalg.norm(np.sqrt(d * d @ (f * f).T))
+        assert off < 0.25 * np.linalg.norm(want) and np.linalg.norm(got - want) <= off
 
 
 @pytest.mark.parametrize("Tn", [1, 6, 80])
