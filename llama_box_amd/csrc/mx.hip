@@ -665,12 +665,12 @@ template <bool ID, int RT> __device__ __forceinline__ void mx_store_tile(const m
 
 // ---- many columns: 32 RT rows by four groups of columns a workgroup.  A wave has one group and all rows: its digits come straight from memory (no other wave reads them), the weights through LDS,
 // where their blocks are aligned ([block of the step][row] 16 bytes, and 4 scale bytes a row).  In a step of 128 values: the next step's digits are requested, the next step's weights (requested a step
-// ago) stored, the weights after those requested — one such item behind each product.  (Requested in a bunch in front of the products they hold up all four waves at once: 512 columns 62 us.)
+// ago) stored, the weights after those requested — one such item behind each product.  (Requested in a bunch in front of the products they hold up all four waves at once.)  RT = 4 with two workgroups a
+// CU beats RT = 8 (us: 1024 / 2048 columns of 2080 x 14336 54 / 97 | 59 / 114, of 4064 x 14336 91 / 168 | 93 / 182)
 #define MX_MFMA1(A, B, C, BYTE, SA, SB) __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, C, MX_FP4, MX_FP6, BYTE, SA, BYTE, (int) (SB))
-template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, RT == 8 ? 1 : 2) k_mx_tile(const mx_mm p, const int row_tiles) {
-    constexpr int SET = RT < 4 ? RT : 4, SETS = RT / SET;
+template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, 2) k_mx_tile(const mx_mm p, const int row_tiles) {
     constexpr int ROWS = 32 * RT, PLANE = ROWS * 16 + 64;  // (64: the four planes that a quad of lanes writes to lie on different banks)
-    constexpr int STAGE = 4 * PLANE + ROWS * 4, OUT = 4 * 4 * mx_store_floats<(RT < 4 ? RT : 4)>();
+    constexpr int STAGE = 4 * PLANE + ROWS * 4, OUT = 4 * 4 * mx_store_floats<RT>();
     __shared__ __align__(16) uint8_t lds[2 * STAGE > OUT ? 2 * STAGE : OUT];  // two stages: the planes, their scales
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r32 = lane & 31, half = lane >> 5;
     int rt, tile;
@@ -750,9 +750,9 @@ template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, RT ==
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
     const int last = p.steps - 1;
-    // in groups of SET tiles and a half step: an accumulator's next product comes SET instructions later, and the next group's weights are read meanwhile
+    // the two blocks of a half in turn: an accumulator's next product comes RT instructions later, and the next block's weights are read meanwhile
     auto multiply = [&](const int buf, const int step) {
-        constexpr int GROUPS = 2 * SETS, ITEMS = 9 + 3 * (RT / 2), SLOTS = GROUPS * 2 * SET, PER = (ITEMS + SLOTS - 1) / SLOTS;
+        constexpr int ITEMS = 9 + 3 * (RT / 2), PER = (ITEMS + 4 * RT - 1) / (4 * RT);
         const int next = min(step + 1, last), after = min(step + 2, last);  // (behind the last step: loads that nobody uses)
         const uint32_t sh = sx >> (8 * half), sl = sh - 0x00040004u;
         auto item = [&](const int n) {
@@ -760,30 +760,28 @@ template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, RT ==
             else if (n < ITEMS && (n - 9) % 3 == 0) store_w((n - 9) / 3, buf ^ 1);
             else if (n < ITEMS && (n - 9) % 3 == 1) fetch_w((n - 9) / 3, after);
         };
-        mx_i4 a[2][SET];
-        int sw[2][SET];
-        auto read = [&](const int g) {
-            const int j = g / SETS, t0 = (g % SETS) * SET;
+        mx_i4 a[2][RT];
+        int sw[2][RT];
+        auto read = [&](const int j) {
 #pragma unroll
-            for (int u = 0; u < SET; ++u) {
-                a[g & 1][u] = *(const mx_i4 *) (lds + buf * STAGE + (2 * j + half) * PLANE + (32 * (t0 + u) + r32) * 16);
-                sw[g & 1][u] = (int) (*(const uint32_t *) (lds + buf * STAGE + 4 * PLANE + (32 * (t0 + u) + r32) * 4) >> (8 * half));
+            for (int t = 0; t < RT; ++t) {
+                a[j][t] = *(const mx_i4 *) (lds + buf * STAGE + (2 * j + half) * PLANE + (32 * t + r32) * 16);
+                sw[j][t] = (int) (*(const uint32_t *) (lds + buf * STAGE + 4 * PLANE + (32 * t + r32) * 4) >> (8 * half));
             }
         };
         read(0);
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-            const int j = g / SETS, t0 = (g % SETS) * SET;
-            if (g + 1 < GROUPS) read(g + 1);
+        for (int j = 0; j < 2; ++j) {
+            if (j == 0) read(1);
             const mx_i8 hx = mx_op6(h4[j], h2[j]), lx = mx_op6(l4[j], l2[j]);
 #pragma unroll
-            for (int u = 0; u < 2 * SET; ++u) {
-                const int t = u % SET;
-                const mx_i8 wx = mx_op4(a[g & 1][t]);
-                if (j == 0) acc[t0 + t] = u < SET ? MX_MFMA1(wx, hx, acc[t0 + t], 0, sw[g & 1][t], sh) : MX_MFMA1(wx, lx, acc[t0 + t], 0, sw[g & 1][t], sl);
-                else acc[t0 + t] = u < SET ? MX_MFMA1(wx, hx, acc[t0 + t], 2, sw[g & 1][t], sh) : MX_MFMA1(wx, lx, acc[t0 + t], 2, sw[g & 1][t], sl);
+            for (int u = 0; u < 2 * RT; ++u) {
+                const int t = u % RT;
+                const mx_i8 wx = mx_op4(a[j][t]);
+                if (j == 0) acc[t] = u < RT ? MX_MFMA1(wx, hx, acc[t], 0, sw[j][t], sh) : MX_MFMA1(wx, lx, acc[t], 0, sw[j][t], sl);
+                else acc[t] = u < RT ? MX_MFMA1(wx, hx, acc[t], 2, sw[j][t], sh) : MX_MFMA1(wx, lx, acc[t], 2, sw[j][t], sl);
 #pragma unroll
-                for (int k = 0; k < PER; ++k) item((g * 2 * SET + u) * PER + k);
+                for (int k = 0; k < PER; ++k) item((j * 2 * RT + u) * PER + k);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -816,16 +814,7 @@ template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, RT ==
         __syncthreads();
     }
     // (behind the loop's last barrier: nobody reads the stages any more)
-    constexpr int PART = RT < 4 ? RT : 4;
-    float * out = (float *) lds + wave * mx_store_floats<PART>();
-#pragma unroll
-    for (int t0 = 0; t0 < RT; t0 += PART) {
-        mx_f16 part[PART];
-#pragma unroll
-        for (int t = 0; t < PART; ++t) part[t] = acc[t0 + t];
-        mx_store_tile<ID, PART>(p, part, group, row0 + 32 * t0, e, lane, out);
-        __builtin_amdgcn_wave_barrier();
-    }
+    mx_store_tile<ID, RT>(p, acc, group, row0, e, lane, (float *) lds + wave * mx_store_floats<RT>());
 }
 // ---- many columns of rows that are whole 16-byte pieces (K a multiple of 512: 272 bytes): as k_mx_tile, but the weights go to LDS by DMA as they lie in memory, 512 values a stage and row by row, and a
 // lane moves its codes into place behind its LDS read.  Eight waves: a group of columns has two, which take the even and the odd quarters of a row's stage (68 bytes, four blocks each) and add up at the
@@ -943,8 +932,8 @@ template <int RT, int ODD> __device__ __forceinline__ void mx_wide_sum(const mx_
                 if (i == 1) acc[t0 + t] = MX_MFMA1(wx[g & 1][t], dx, acc[t0 + t], 1, sw[g & 1][t], sd);
                 if (i == 2) acc[t0 + t] = MX_MFMA1(wx[g & 1][t], dx, acc[t0 + t], 2, sw[g & 1][t], sd);
                 if (i == 3) acc[t0 + t] = MX_MFMA1(wx[g & 1][t], dx, acc[t0 + t], 3, sw[g & 1][t], sd);
-                if (u < SET) place((g + 1) % GROUPS, u);
-                else read((g + 2) % GROUPS, u - SET, g + 2 < GROUPS ? at : at_next);
+                if (u < SET) read((g + 2) % GROUPS, u, g + 2 < GROUPS ? at : at_next);
+                else place((g + 1) % GROUPS, u - SET);
                 // requests, the n-th slot of block i: the last block's digits in block 0, then the digits of block i - 1 of the next stage, and behind those of block 0 the next stage's
                 // weights (together with the last block's digits they hold up both: 2048 columns of 4096 x 16384 190 us, 185 like this)
                 constexpr int PER = 8 / RT;
@@ -1090,8 +1079,10 @@ template <bool ID, int RT> static void mx_launch_tile_of(hipStream_t s, const mx
             return;
         }
     }
-    if (mx_dwords(p)) hipLaunchKernelGGL((k_mx_tile<ID, RT, true>), grid, dim3(256), 0, s, p, row_tiles);
-    else hipLaunchKernelGGL((k_mx_tile<ID, RT, false>), grid, dim3(256), 0, s, p, row_tiles);
+    if constexpr (RT < 8) {
+        if (mx_dwords(p)) hipLaunchKernelGGL((k_mx_tile<ID, RT, true>), grid, dim3(256), 0, s, p, row_tiles);
+        else hipLaunchKernelGGL((k_mx_tile<ID, RT, false>), grid, dim3(256), 0, s, p, row_tiles);
+    } else mx_launch_tile_of<ID, 4>(s, p, col_tiles);
 }
 template <bool ID> static void mx_launch_tile(hipStream_t s, const mx_mm & p, int64_t tiles, int rt) {
     if (rt == 8) mx_launch_tile_of<ID, 8>(s, p, tiles);
