@@ -103,7 +103,8 @@ template <bool IDX> __global__ void __launch_bounds__(256) k_mx_read(const tdesc
     const uint8_t * in = (const uint8_t *) a.data + from * a.nb[1] + i2 * a.nb[2] + i3 * a.nb[3] + (int64_t) blk * MX_BLOCK;
     mx_put8(d.data + i1 * d.nb[1] + i2 * d.nb[2] + i3 * d.nb[3] + (int64_t) blk * 128, i, *(const mx_u32_a1 *) (in + 1 + 4 * i), mx_scale(in[0]));
 }
-// Dense tensors (CPY): a workgroup has 256 blocks, whose 4352 bytes cross LDS so that they are read and written 16 bytes at a time (byte by byte as above, 14336 x 4096 values there and back: 151 us)
+// Dense tensors (CPY): a workgroup has 256 blocks, whose 4352 bytes cross LDS so that they are read and written 16 bytes at a time.  Bytes bound it: 14336 x 4096 values there and back, 532 MB, 113 us, 4.7
+// TB/s, a large copy's rate (byte by byte as above: 151 us)
 static constexpr int MX_CPY = 256;
 __global__ void __launch_bounds__(256) k_mx_store_dense(const char * __restrict__ x, uint8_t * __restrict__ out, const int64_t blocks) {
     __shared__ __align__(16) uint8_t s[MX_CPY * MX_BLOCK];
@@ -435,7 +436,9 @@ template <> struct mx_raw<false> {
     ACC = __builtin_amdgcn_mfma_scale_f32_##N##_f8f6f4(mx_op4(A), H, ACC, MX_FP4, MX_FP6, J, S, J, (int) (SH));              \
     ACC = __builtin_amdgcn_mfma_scale_f32_##N##_f8f6f4(mx_op4(A), L, ACC, MX_FP4, MX_FP6, J, S, J, (int) (SL));
 
-// ---- one to a few columns: 16 rows a workgroup, its waves take four steps of 128 values in turn.  The workgroup quantises its columns itself, while its first weights are on the way.  A lane of v_mfma_scale_f32_16x16x128: row (column) lane % 16, step lane / 16 of the four.
+// ---- one to a few columns: 16 rows a workgroup, its waves take four steps of 128 values in turn.  The workgroup quantises its columns itself, while its first weights are on the way.  A lane of
+// v_mfma_scale_f32_16x16x128: row (column) lane % 16, step lane / 16 of the four.  The weights' bytes bound it, behind the launch (us, with the 3.5 of a step's one launch: one column of 14336 x 4096,
+// 31 MB, 10.2; of 4096 x 4096 5.1; a token's 4 experts of 2048 x 4096, 18 MB, 8.8).
 // ID: blockIdx.y is a column (u + n_used t) of at most 64; the first column of an expert takes all of its expert, the others' workgroups end at once.
 static constexpr int MX_VEC_REC = 48;     // LDS bytes of a block of one column: 24 of h, 24 of l
 template <bool ID, bool DW> __global__ void __launch_bounds__(512, DW ? 3 : 2) k_mx_vec(const mx_mm p, const tdesc b, const tdesc ids, const int chunk) {
@@ -535,7 +538,8 @@ template <bool ID, bool DW> __global__ void __launch_bounds__(512, DW ? 3 : 2) k
     }
 }
 
-// ---- a few groups of columns: 32 rows by one group a workgroup, its waves take two steps in turn, everything straight from memory; the waves' sums are added in LDS in their order
+// ---- a few groups of columns: 32 rows by one group a workgroup, its waves take two steps in turn, everything straight from memory; the waves' sums are added in LDS in their order.  (Two groups a
+// workgroup would read the weights once for both; their digits do not fit in registers beside the weights of two turns: 64 columns of 4096 x 4096 22.4 us, 11.8 like this)
 template <bool ID, bool DW> __global__ void __launch_bounds__(512) k_mx_few(const mx_mm p) {
     extern __shared__ __align__(16) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, r32 = lane & 31, half = lane >> 5;
@@ -818,7 +822,10 @@ template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, 2) k_
 }
 // ---- many columns of rows that are whole 16-byte pieces (K a multiple of 512: 272 bytes): as k_mx_tile, but the weights go to LDS by DMA as they lie in memory, 512 values a stage and row by row, and a
 // lane moves its codes into place behind its LDS read.  Eight waves: a group of columns has two, which take the even and the odd quarters of a row's stage (68 bytes, four blocks each) and add up at the
-// end; the second wave of a SIMD issues while the first one's product runs (one wave alone, eight blocks a stage: 512 columns 46 us).  In a quarter that starts at a unit of 8 bytes (the odd ones: at its
+// end; the second wave of a SIMD issues while the first one's product runs (one wave alone, eight blocks a stage: 512 columns 46 us).  512 / 1900 columns of 4096 x 14336: 43 / 150 us, 2.8 / 3.0 10^15
+// operations a second of the 7.9 that the instruction reaches alone: 3.6 us a stage, of which the matrix pipe works 51 % (2.25 GHz).  Without the DMA a stage takes 2.9 us, without the digits' loads 3.4,
+// without both 2.7: 170 KB a stage and CU on the one path from L2 (its address unit works 64 % of the time).  What left the time as it was: rows in LDS 144 bytes apart, without a bank conflict (whole
+// rows: half of LDS's cycles), and a product of another tile between the two of a tile.  In a quarter that starts at a unit of 8 bytes (the odd ones: at its
 // second half) block i starts at byte i of a unit, and needs the two units behind it: one 16-byte read a block (the unit between two blocks is kept) and up to four byte shifts.
 __device__ __forceinline__ void mx_dma16(const uint8_t * base, const uint32_t off, const uint32_t lds) {  // lane i's 16 bytes at base + off to LDS[lds + 16 i]; base and lds of the wave
     uint32_t keep;

@@ -577,3 +577,28 @@ def test_same_result_every_time(backend):
     a, = T.run_case(lambda g: ffn_block(g, z), backend)
     for _ in range(3):
         assert np.array_equal(np.asarray(a), np.asarray(T.run_case(lambda g: ffn_block(g, z), backend)[0]))
+
+
+@pytest.mark.parametrize("K,N,M", [(256, 300, 2), (256, 1027, 40), (512, 4100, 700), (160, 2048, 500)])
+def test_result_in_host_memory(backend, K, N, M):
+    """a graph whose last node is such a product, asked to leave its result in pinned host memory: every form stores there, in rows that are whole 16-byte pieces and that are not"""
+    H = L.host()
+    result_to = backend.proc("ggml_backend_mi355x_result_to", C.c_int, [C.c_void_p, L.TP, C.c_void_p, C.c_size_t])
+    r = rng_of(41, K, N)
+    g, pin = T.G(backend), None
+    try:
+        w, x = weights(r, N, K), acts(r, M, K)
+        out = H.ggml_mul_mat(g.ctx, g.new(L.MXFP4, (K, N), w), g.new(L.F32, (K, M), x))
+        ref = g.compute([out])[0].reshape(M, N)
+        pin = H.ggml_backend_buft_alloc_buffer(H.ggml_backend_dev_host_buffer_type(backend.dev), M * N * 4)
+        base = H.ggml_backend_buffer_get_base(pin)
+        for _ in range(3):
+            C.memset(base, 0x55, M * N * 4)
+            assert result_to(backend.backend, out, base, M * N * 4) == 1
+            assert H.ggml_backend_graph_compute_async(backend.backend, g.gf) == 0
+            backend.synchronize()
+            assert np.array_equal(np.ctypeslib.as_array(C.cast(base, C.POINTER(C.c_float)), (M, N)), ref)
+    finally:
+        if pin:
+            H.ggml_backend_buffer_free(pin)
+        g.free()
