@@ -438,10 +438,10 @@ template <> struct mx_raw<false> {
 
 // ---- one to a few columns: 16 rows a workgroup, its waves take four steps of 128 values in turn.  The workgroup quantises its columns itself, while its first weights are on the way.  A lane of
 // v_mfma_scale_f32_16x16x128: row (column) lane % 16, step lane / 16 of the four.  The weights' bytes bound it, behind the launch (us, with the 3.5 of a step's one launch: one column of 14336 x 4096,
-// 31 MB, 10.2; of 4096 x 4096 5.1; a token's 4 experts of 2048 x 4096, 18 MB, 8.8).
+// 31 MB, 10.2; of 4096 x 4096 4.5; a token's 4 experts of 2048 x 4096, 18 MB, 6.6).  ONE: a wave has one turn, and no registers for the weights of a second (half as many, twice the waves: 8.7 us)
 // ID: blockIdx.y is a column (u + n_used t) of at most 64; the first column of an expert takes all of its expert, the others' workgroups end at once.
 static constexpr int MX_VEC_REC = 48;     // LDS bytes of a block of one column: 24 of h, 24 of l
-template <bool ID, bool DW> __global__ void __launch_bounds__(512, DW ? 3 : 2) k_mx_vec(const mx_mm p, const tdesc b, const tdesc ids, const int chunk) {
+template <bool ID, bool DW, bool ONE> __global__ void __launch_bounds__(512, ONE ? 4 : DW ? 3 : 2) k_mx_vec(const mx_mm p, const tdesc b, const tdesc ids, const int chunk) {
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ int s_cols[64];
     __shared__ int64_t s_at[64];  // where the workgroup's columns start in b
@@ -475,7 +475,7 @@ template <bool ID, bool DW> __global__ void __launch_bounds__(512, DW ? 3 : 2) k
         const int last = p.steps - 1, stride = 4 * waves;
         int step = wave * 4 + q;  // (behind the last step: its weights again, and digits of zero)
         f0.load(w, min(step, last), p.blocks);
-        if (wave * 4 + stride < p.steps) f1.load(w, min(step + stride, last), p.blocks);
+        if (!ONE && wave * 4 + stride < p.steps) f1.load(w, min(step + stride, last), p.blocks);
         __syncthreads();  // (the columns' places; the last chunk's partial sums and digits are read)
         const int i = threadIdx.x & 3, per = (int) blockDim.x >> 2;  // four lanes a block
         for (int at0 = threadIdx.x >> 2; at0 < m * all; at0 += 2 * per) {
@@ -521,7 +521,8 @@ template <bool ID, bool DW> __global__ void __launch_bounds__(512, DW ? 3 : 2) k
                 if (j & 1) __builtin_amdgcn_sched_barrier(0);  // (the digits of all four blocks at a time would cost a third of the waves)
             }
         };
-        for (int s0 = wave * 4; s0 < p.steps; s0 += 2 * stride, step += 2 * stride) {  // (s0: the wave's, for all its lanes)
+        if (ONE && wave * 4 < p.steps) add(step, f0);
+        for (int s0 = wave * 4; !ONE && s0 < p.steps; s0 += 2 * stride, step += 2 * stride) {  // (s0: the wave's, for all its lanes)
             add(step, f0);
             if (s0 + 2 * stride < p.steps) f0.load(w, min(step + 2 * stride, last), p.blocks);
             if (s0 + stride < p.steps) add(step + stride, f1);
@@ -1035,10 +1036,10 @@ static mx_mm mx_args(const tdesc & w, const tdesc & d, int64_t cols) {
     p.cols = cols;
     return p;
 }
-// k_mx_vec: columns quantised at a time (0: a column does not fit).  A wave has two times four steps on the way; eight waves where the workgroups alone do not fill the GPU (us, four waves | eight: 1 / 8
-// columns of 4096 x 4096, 256 workgroups, 5.4 / 11.9 | 5.3 / 10.0, of 5632 x 2048, 352 workgroups, 4.9 / 9.6 | 6.6 / 11.1)
+// k_mx_vec: columns quantised at a time (0: a column does not fit); waves: one turn where eight make it one, and eight where the workgroups alone do not fill the GPU (us, four waves | eight: a column of
+// 4096 x 4096, 256 workgroups, 5.2 | 4.5, of 2048 x 5632, 352 workgroups, one turn in both, 4.0 | 4.5, of 2048 x 32000 8.5 | 12.0, of 4096 x 14336 11.1 | 9.8; 5 columns of 2080 x 1001 7.7 | 6.2)
 static constexpr size_t MX_VEC_LDS = 60 << 10;
-static int mx_vec_waves(int64_t K, int64_t N, int64_t slots) { return (int) std::min<int64_t>(8, std::max<int64_t>((N + 15) / 16 * slots <= 256 ? 8 : 4, (mx_steps(K) + 7) / 8)); }
+static int mx_vec_waves(int64_t K, int64_t N, int64_t slots) { return (int) std::min<int64_t>(8, std::max<int64_t>((N + 15) / 16 * slots <= 256 ? 8 : 4, (mx_steps(K) + 3) / 4)); }
 static size_t mx_vec_lds(int64_t K, int64_t cols) { return (size_t) cols * (size_t) ((mx_steps(K) + 3) / 4 * 16 * (MX_VEC_REC + 1)) + (size_t) (8 * cols * 16 * 4); }
 static int mx_vec_chunk(int64_t K, int64_t cols) {
     int64_t c = std::min<int64_t>(16, cols);
@@ -1053,9 +1054,9 @@ static int64_t mx_tile_cost(int rt, int64_t N, int64_t tiles, int64_t groups) {
     const int64_t rounds = ((N + 32 * rt - 1) / (32 * rt) * tiles + 255) / 256, g = std::min<int64_t>(groups, 4);
     return rounds * (rt == 2 ? 20 + 9 * g : rt == 4 ? 47 + 11 * g : 70 + 17 * g);
 }
-// Every workgroup quantises its columns: a launch less (two with MUL_MAT_ID), for work that grows with columns and rows.  us, k_mx_vec | the faster of the others: 2 / 4 columns of 4096 x 14336 13.5 / 18.4 |
-// 13.7 / 13.7, 2 of 14336 x 4096 13.0 | 20.0, 4 / 8 of 4096 x 4096 6.9 / 10.0 | 11.6 / 11.6, of 2048 x 5632 6.6 / 9.5 | 8.9 / 8.8, of 2080 x 5000 8.5 / 12.3 | 10.7 / 10.5, 16 of 1024 x 1024 6.5 | 7.9; expert
-// columns, 16 / 24 of 32 experts of 2048 x 4096 25.0 / 31.5 | 25.9 / 26.8, of 4096 x 4096 35.5 / 45.7 | 36.7 / 39.2, 64 of 1024 x 1024 11.5 | 14.1, of 128 experts of 2048 x 768 20.1 | 21.7
+// Every workgroup quantises its columns: a launch less (two with MUL_MAT_ID), for work that grows with columns and rows.  us, k_mx_vec | the faster of the others: 2 / 3 columns of 4096 x 14336 11.5 / 14.2 |
+// 13.7, 2 of 14336 x 4096 12.9 | 20.1, 4 / 8 of 4096 x 4096 6.5 / 9.4 | 11.7, 8 / 12 of 2048 x 5632 8.9 / 11.2 | 9.0, 6 / 8 of 2080 x 5000 9.8 / 12.0 | 10.6, 16 of 1024 x 1024 6.2 | 7.9; expert columns,
+// 16 / 24 of 32 experts of 2048 x 4096 23.0 / 29.1 | 25.7 / 26.1, of 4096 x 4096 32.8 / 41.4 | 35.6 / 38.8, 64 of 1024 x 1024 9.7 | 14.2, of 128 experts of 2048 x 768 18.5 | 21.7
 bool mx_vec_takes(int64_t K, int64_t N, int64_t cols) {
     return (cols == 1 || (cols <= 16 && cols * K * N <= 150000000 && cols * K <= 4096 * mx_vec_waves(K, N, 1))) && mx_vec_chunk(K, cols) >= cols;
 }
@@ -1071,9 +1072,9 @@ static void mx_launch_vec(hipStream_t s, const mx_mm & p, const tdesc & b, const
     const dim3 block((unsigned) (64 * mx_vec_waves(K, p.n_rows, ids ? p.cols : 1)));
     const unsigned rows = (unsigned) ((p.n_rows + 15) / 16);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(rows, ids ? (unsigned) p.cols : 1u), block, mx_vec_lds(K, chunk), s, p, b, ids ? *ids : b, chunk); };
-    const bool dw = mx_dwords(p);
-    if (ids) dw ? go(k_mx_vec<true, true>) : go(k_mx_vec<true, false>);
-    else dw ? go(k_mx_vec<false, true>) : go(k_mx_vec<false, false>);
+    const bool dw = mx_dwords(p), one = p.steps <= (int) block.x / 64 * 4;
+    if (ids) one ? (dw ? go(k_mx_vec<true, true, true>) : go(k_mx_vec<true, false, true>)) : dw ? go(k_mx_vec<true, true, false>) : go(k_mx_vec<true, false, false>);
+    else one ? (dw ? go(k_mx_vec<false, true, true>) : go(k_mx_vec<false, false, true>)) : dw ? go(k_mx_vec<false, true, false>) : go(k_mx_vec<false, false, false>);
 }
 template <bool ID, int RT> static void mx_launch_tile_of(hipStream_t s, const mx_mm & p, int64_t col_tiles) {
     const int row_tiles = (p.n_rows + 32 * RT - 1) / (32 * RT);
