@@ -617,8 +617,9 @@ template <bool ID, bool DW> __global__ void __launch_bounds__(512) k_mx_few(cons
 
 // Consecutive workgroups go to the eight dies in turn: each die has a run of tiles, four column tiles of a row tile after the other, then the next row tile's; the tiles that a die works on at a time
 // so share their digits and their weights in its L2
-__device__ __forceinline__ bool mx_tile_of(const mx_mm & p, const int row_tiles, int & rt, int & tile) {
-    const int n_tiles = (int) ((p.cols + 127) / 128), at = (int) (blockIdx.x & 7) * (int) (gridDim.x >> 3) + (int) (blockIdx.x >> 3);
+// (block of blocks, both counted from a multiple of 8)
+__device__ __forceinline__ bool mx_tile_of(const mx_mm & p, const int block, const int blocks, const int row_tiles, int & rt, int & tile) {
+    const int n_tiles = (int) ((p.cols + 127) / 128), at = (block & 7) * (blocks >> 3) + (block >> 3);
     const int band = at / (row_tiles * 4), in = at - band * row_tiles * 4, width = min(4, n_tiles - 4 * band);
     if (width <= 0) return false;
     rt = in / width;
@@ -682,7 +683,7 @@ template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, 2) k_
     if (ID) {
         mx_id_tile_of(row_tiles, rt, tile);
     } else {
-        if (!mx_tile_of(p, row_tiles, rt, tile)) return;
+        if (!mx_tile_of(p, blockIdx.x, gridDim.x, row_tiles, rt, tile)) return;
     }
     const int row0 = rt * ROWS;
     int e = 0, group = tile * 4 + wave, groups = (int) ((p.cols + 31) / 32);
@@ -823,7 +824,7 @@ template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, 2) k_
 }
 // ---- many columns of rows that are whole 16-byte pieces (K a multiple of 512: 272 bytes): as k_mx_tile, but the weights go to LDS by DMA as they lie in memory, 512 values a stage and row by row, and a
 // lane moves its codes into place behind its LDS read.  Eight waves: a group of columns has two, which take the even and the odd quarters of a row's stage (68 bytes, four blocks each) and add up at the
-// end; the second wave of a SIMD issues while the first one's product runs (one wave alone, eight blocks a stage: 512 columns 46 us).  512 / 1900 columns of 4096 x 14336: 43 / 150 us, 2.8 / 3.0 10^15
+// end; the second wave of a SIMD issues while the first one's product runs (one wave alone, eight blocks a stage: 512 columns 46 us).  512 / 1900 columns of 4096 x 14336: 43 / 145 us, 2.8 / 3.1 10^15
 // operations a second of the 7.9 that the instruction reaches alone: 3.6 us a stage, of which the matrix pipe works 51 % (2.25 GHz).  Without the DMA a stage takes 2.9 us, without the digits' loads 3.4,
 // without both 2.7: 170 KB a stage and CU on the one path from L2 (its address unit works 64 % of the time).  What left the time as it was: rows in LDS 144 bytes apart, without a bank conflict (whole
 // rows: half of LDS's cycles), and a product of another tile between the two of a tile.  In a quarter that starts at a unit of 8 bytes (the odd ones: at its
@@ -958,19 +959,12 @@ template <int RT, int ODD> __device__ __forceinline__ void mx_wide_sum(const mx_
         sx = sxn;
     }
 }
-// (RT = 2: two workgroups a CU, 10 tokens of 32 experts of 2048 x 4096 44 us, one 57)
-template <bool ID, int RT> __global__ void __launch_bounds__(512, RT == 2 ? 4 : 2) k_mx_wide(const mx_mm p, const int row_tiles) {
+// where the workgroups of low tiles begin behind `head` row tiles
+__host__ __device__ static inline int mx_tail_at(const int head, const int64_t cols) { return (int) ((head * ((cols + 127) / 128) + 7) / 8 * 8); }
+template <bool ID, int RT> __device__ __forceinline__ void mx_wide_tile(const mx_mm & p, const int row0, const int tile, uint8_t * lds) {
     constexpr int ROWS = 32 * RT, PIECES = mx_wide_pieces<RT>();
     static_assert(PIECES <= 9, "a lane's pieces leave their row once");
-    extern __shared__ __align__(16) uint8_t lds[];  // two stages of [row] 272 bytes
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int rt, tile;
-    if (ID) {
-        mx_id_tile_of(row_tiles, rt, tile);
-    } else {
-        if (!mx_tile_of(p, row_tiles, rt, tile)) return;
-    }
-    const int row0 = min(rt * ROWS, p.n_rows - ROWS);  // (the last tile has some of the rows of the one before it, with the same result)
     int e = 0, group = tile * 4 + (wave & 3), groups = (int) ((p.cols + 31) / 32);
     if (ID) {
         if (tile >= p.l.total[1]) return;
@@ -1022,6 +1016,26 @@ template <bool ID, int RT> __global__ void __launch_bounds__(512, RT == 2 ? 4 : 
     __syncthreads();
     if (group < groups) mx_store_tile<ID, RT / 2>(p, sum, group, row0 + (wave < 4 ? 0 : ROWS / 2), e, lane, (float *) lds + wave * mx_store_floats<RT / 2>());
 }
+// (RT = 2: two workgroups a CU, 10 tokens of 32 experts of 2048 x 4096 44 us, one 57.)  The last tile has some of the rows of the one before it, with the same result.  Behind the first `head` row tiles of
+// RT = 8 the rows are in tiles of `low` = 128 or 64 rows, in the launch's last workgroups (row_tiles: their number, or head where there are none)
+template <bool ID, int RT> __global__ void __launch_bounds__(512, RT == 2 ? 4 : 2) k_mx_wide(const mx_mm p, const int row_tiles, const int head, const int low) {
+    extern __shared__ __align__(16) uint8_t lds[];  // two stages of [row] 272 bytes
+    int rt, tile;
+    if (ID) {
+        mx_id_tile_of(row_tiles, rt, tile);
+        mx_wide_tile<ID, RT>(p, min(rt * 32 * RT, p.n_rows - 32 * RT), tile, lds);
+        return;
+    }
+    const int first = RT == 8 ? mx_tail_at(head, p.cols) : (int) gridDim.x;
+    if ((int) blockIdx.x < first) {
+        if (mx_tile_of(p, blockIdx.x, first, RT == 8 ? head : row_tiles, rt, tile)) mx_wide_tile<ID, RT>(p, min(rt * 32 * RT, p.n_rows - 32 * RT), tile, lds);
+    } else if (RT == 8) {
+        if (!mx_tile_of(p, (int) blockIdx.x - first, (int) gridDim.x - first, row_tiles, rt, tile)) return;
+        const int row0 = min(head * 256 + rt * low, p.n_rows - low);
+        if (low == 128) mx_wide_tile<ID, 4>(p, row0, tile, lds);
+        else mx_wide_tile<ID, 2>(p, row0, tile, lds);
+    }
+}
 static mx_mm mx_args(const tdesc & w, const tdesc & d, int64_t cols) {
     mx_mm p{};
     p.w = (const uint8_t *) w.data;
@@ -1046,14 +1060,6 @@ static int mx_vec_chunk(int64_t K, int64_t cols) {
     while (c > 0 && mx_vec_lds(K, c) > MX_VEC_LDS) --c;
     return (int) c;
 }
-// Costs of a product by k_mx_few and in tiles of 32 rt rows, in quarters of a us at 4096 values a row: 256 workgroups at a time, a tile's by its groups of columns.  What they compare, us, k_mx_few | tiles of 64
-// rows: 32 columns of 4096 x 14336 18.8 | 14.4, of 4096 x 32000 30.4 | 18.6, of 14336 x 8192 23.3 | 29.0, 64 of 4096 x 4096 11.8 | 14.7, 128 17.9 | 19.5, 256 29.7 | 21.2; 4 / 18 columns an expert, 32 experts
-// of 2048 x 4096 49 / 87 | 36 / 58, 8 of 2080 x 512 16.0 | 18.7.  Tiles of 64 | 128 | 256 rows: 256 columns of 4096 x 14336 35.9 | 26.6 | 34.8, 384 51.5 | 47.6 | 37.5
-static int64_t mx_few_cost(int64_t N, int64_t groups) { return ((N + 31) / 32 * groups + 255) / 256 * 22; }
-static int64_t mx_tile_cost(int rt, int64_t N, int64_t tiles, int64_t groups) {
-    const int64_t rounds = ((N + 32 * rt - 1) / (32 * rt) * tiles + 255) / 256, g = std::min<int64_t>(groups, 4);
-    return rounds * (rt == 2 ? 20 + 9 * g : rt == 4 ? 47 + 11 * g : 70 + 17 * g);
-}
 // Every workgroup quantises its columns: a launch less (two with MUL_MAT_ID), for work that grows with columns and rows.  us, k_mx_vec | the faster of the others: 2 / 3 columns of 4096 x 14336 11.5 / 14.2 |
 // 13.7, 2 of 14336 x 4096 12.9 | 20.1, 4 / 8 of 4096 x 4096 6.5 / 9.4 | 11.7, 8 / 12 of 2048 x 5632 8.9 / 11.2 | 9.0, 6 / 8 of 2080 x 5000 9.8 / 12.0 | 10.6, 16 of 1024 x 1024 6.2 | 7.9; expert columns,
 // 16 / 24 of 32 experts of 2048 x 4096 23.0 / 29.1 | 25.7 / 26.1, of 4096 x 4096 32.8 / 41.4 | 35.6 / 38.8, 64 of 1024 x 1024 9.7 | 14.2, of 128 experts of 2048 x 768 18.5 | 21.7
@@ -1076,6 +1082,29 @@ static void mx_launch_vec(hipStream_t s, const mx_mm & p, const tdesc & b, const
     if (ids) one ? (dw ? go(k_mx_vec<true, true, true>) : go(k_mx_vec<true, false, true>)) : dw ? go(k_mx_vec<true, true, false>) : go(k_mx_vec<true, false, false>);
     else one ? (dw ? go(k_mx_vec<false, true, true>) : go(k_mx_vec<false, false, true>)) : dw ? go(k_mx_vec<false, true, false>) : go(k_mx_vec<false, false, false>);
 }
+// Costs of a product by k_mx_few and in tiles of 32 rt rows, in quarters of a us at 4096 values a row: 256 workgroups at a time, a tile's by its groups of columns.  What they compare, us, k_mx_few | tiles of 64
+// rows: 32 columns of 4096 x 14336 18.8 | 14.4, of 4096 x 32000 30.4 | 18.6, of 14336 x 8192 23.3 | 29.0, 64 of 4096 x 4096 11.8 | 14.7, 128 17.9 | 19.5, 256 29.7 | 21.2; 4 / 18 columns an expert, 32 experts
+// of 2048 x 4096 49 / 87 | 36 / 58, 8 of 2080 x 512 16.0 | 18.7.  Tiles of 64 | 128 | 256 rows: 256 columns of 4096 x 14336 35.9 | 26.6 | 34.8, 384 51.5 | 47.6 | 37.5
+static int64_t mx_few_cost(int64_t N, int64_t groups) { return ((N + 31) / 32 * groups + 255) / 256 * 22; }
+static int64_t mx_tile_cost(int rt, int64_t N, int64_t tiles, int64_t groups) {
+    const int64_t rounds = ((N + 32 * rt - 1) / (32 * rt) * tiles + 255) / 256, g = std::min<int64_t>(groups, 4);
+    return rounds * (rt == 2 ? 20 + 9 * g : rt == 4 ? 47 + 11 * g : 70 + 17 * g);
+}
+// A product in tiles of 256 rows whose last round of 256 workgroups is far from full: that round's rows in lower tiles where it ends earlier by the costs above.  -> the cost; low: their height (0: none), head:
+// the row tiles in front of them.  us, without | with: 640 columns of 4096 x 14336 72.6 | 62.1, 768 73.0 | 67.1, 1900 (840 tiles, or 765 and 150 of
+// 128 rows) 154 | 145, 2048 of 4096 x 5632 75.9 | 70.3, 2200 of 14336 x 4096 217 | 191
+static int64_t mx_tail(int64_t N, int64_t tiles, int & head, int & low) {
+    const int64_t all = (N + 255) / 256, whole = all * tiles / 256, full = std::min(all, whole * 256 / tiles), idle = whole * 256 - full * tiles, c8 = mx_tile_cost(8, N, tiles, 4);
+    head = (int) all;
+    low = 0;
+    if (whole == 0 || full == all) return c8;
+    auto cost = [&](int rt) { return whole * mx_tile_cost(8, 1, 1, 4) + (std::max<int64_t>(0, (N - 256 * full + 32 * rt - 1) / (32 * rt) * tiles - idle) + 255) / 256 * mx_tile_cost(rt, 1, 1, 4); };
+    const int64_t c4 = cost(4), c2 = cost(2);
+    if (c8 <= std::min(c4, c2)) return c8;
+    head = (int) full;
+    low = c2 < c4 ? 64 : 128;
+    return std::min(c4, c2);
+}
 template <bool ID, int RT> static void mx_launch_tile_of(hipStream_t s, const mx_mm & p, int64_t col_tiles) {
     const int row_tiles = (p.n_rows + 32 * RT - 1) / (32 * RT);
     const dim3 grid((unsigned) (ID ? (col_tiles + 7) / 8 * 8 * row_tiles : (row_tiles * col_tiles + 7) / 8 * 8));
@@ -1083,7 +1112,11 @@ template <bool ID, int RT> static void mx_launch_tile_of(hipStream_t s, const mx
         constexpr size_t lds = std::max<size_t>(2 * mx_wide_pieces<RT>() * 8192, 8 * 4 * mx_store_floats<RT / 2>());
         static std::atomic<uint32_t> done{0};
         if (ensure_dyn_lds((const void *) k_mx_wide<ID, RT>, lds, done)) {
-            hipLaunchKernelGGL((k_mx_wide<ID, RT>), grid, dim3(512), lds, s, p, row_tiles);
+            int head = row_tiles, low = 0;
+            if (!ID && RT == 8) mx_tail(p.n_rows, col_tiles, head, low);
+            const int tail = low ? (p.n_rows - 256 * head + low - 1) / low : 0;
+            if (low) hipLaunchKernelGGL((k_mx_wide<ID, RT>), dim3((unsigned) (mx_tail_at(head, p.cols) + (tail * col_tiles + 7) / 8 * 8)), dim3(512), lds, s, p, tail, head, low);
+            else hipLaunchKernelGGL((k_mx_wide<ID, RT>), grid, dim3(512), lds, s, p, row_tiles, head, 0);
             return;
         }
     }
@@ -1097,8 +1130,9 @@ template <bool ID> static void mx_launch_tile(hipStream_t s, const mx_mm & p, in
     else if (rt == 4) mx_launch_tile_of<ID, 4>(s, p, tiles);
     else mx_launch_tile_of<ID, 2>(s, p, tiles);
 }
-static int mx_tile_rows(int64_t N, int64_t tiles, int64_t groups) {
-    const int64_t c2 = mx_tile_cost(2, N, tiles, groups), c4 = mx_tile_cost(4, N, tiles, groups), c8 = mx_tile_cost(8, N, tiles, groups);
+static int mx_tile_rows(int64_t N, int64_t tiles, int64_t groups, bool tail) {
+    int head, low;
+    const int64_t c2 = mx_tile_cost(2, N, tiles, groups), c4 = mx_tile_cost(4, N, tiles, groups), c8 = tail && groups >= 4 ? mx_tail(N, tiles, head, low) : mx_tile_cost(8, N, tiles, groups);
     return c8 <= c4 && c8 <= c2 ? 8 : c4 <= c2 ? 4 : 2;
 }
 // Four waves where the rows and groups alone fill the GPU, eight where they do not (us for 8 / 32 columns, four waves | eight: 4096 rows of 14336 18.3 / 21.2 | 18.6 / 20.3, 14336 of 4096 15.4 / 17.1 |
@@ -1119,7 +1153,7 @@ void launch_mx_mul_mat(hipStream_t s, const tdesc & w, const tdesc & b, const td
     else {
         const int64_t groups = (p.cols + 31) / 32, tiles = (p.cols + 127) / 128;
         if (mx_few_cost(p.n_rows, groups) < mx_tile_cost(2, p.n_rows, tiles, groups)) mx_launch_few<false>(s, p, groups);
-        else mx_launch_tile<false>(s, p, tiles, mx_tile_rows(p.n_rows, tiles, groups));
+        else mx_launch_tile<false>(s, p, tiles, mx_tile_rows(p.n_rows, tiles, groups, mx_pieces(p)));
     }
 }
 void launch_mx_mul_mat_id(hipStream_t s, const tdesc & w, const tdesc & b, const tdesc & ids, const tdesc & d, const void * ws, const float * bias, int64_t nb_bias) {
@@ -1135,7 +1169,7 @@ void launch_mx_mul_mat_id(hipStream_t s, const tdesc & w, const tdesc & b, const
     // 256 rows, 10 / 28 columns an expert: 32 experts of 2048 x 4096 44 / 68 | 46 / 56, of 1024 x 1024 15.7 / 19.6 | 20.6 / 23.4, 128 of 2048 x 768 40 / 51 | 48 / 55
     const int64_t tiles = mx_id_tiles(w.ne[2], cols), each = cols / w.ne[2];
     if (mx_few_cost(p.n_rows, g) < mx_tile_cost(2, p.n_rows, tiles, each / 32 + 1)) mx_launch_few<true>(s, p, g);
-    else if (each >= 64) mx_launch_tile<true>(s, p, tiles, mx_tile_rows(p.n_rows, tiles, 4));
+    else if (each >= 64) mx_launch_tile<true>(s, p, tiles, mx_tile_rows(p.n_rows, tiles, 4, false));
     else mx_launch_tile<true>(s, p, tiles, each >= 16 && p.n_rows / 256 * tiles >= 512 ? 8 : 2);
 }
 // Which operands the products take (type and shape; the rows of both are dense, whole blocks).  The kernels hold offsets inside a tile of 256 rows and inside a group's digits in 32 bits, and a launch less than

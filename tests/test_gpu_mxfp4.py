@@ -232,6 +232,15 @@ def test_product_tiles(backend, K, N, M):
     mx_ref.check("tiles", mul_mat(backend, w, x, K, N, M), want, mags, K)
 
 
+@pytest.mark.parametrize("K,N,M", [(512, 8200, 1100), (1024, 4300, 2500)])
+def test_product_low_tiles_behind_tall_ones(backend, K, N, M):
+    """products whose last rows are in tiles of 64 and of 128 rows behind whole rounds of tiles of 256"""
+    r = rng_of(42, K, N)
+    w, x = weights(r, N, K), acts(r, M, K)
+    want, mags = mx_ref.product(x, w)
+    mx_ref.check("low tiles", mul_mat(backend, w, x, K, N, M), want, mags, K)
+
+
 @pytest.mark.parametrize("M", [1, 20, 700])
 def test_product_rows_far_apart(backend, M):
     """a matrix that is some columns of a much wider one: its rows lie half a megabyte apart"""
