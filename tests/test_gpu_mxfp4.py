@@ -339,6 +339,18 @@ def test_experts_tiles(backend, K, N):
     mx_ref.check("tiles", run_experts(backend, w, x, ids, b, K, N), want, mags, K, extra=np.abs(b[ids]))
 
 
+@pytest.mark.parametrize("K", [512, 1536])
+def test_experts_short_tiles(backend, K):
+    """tall tiles of one, two, three and four groups of columns, beside an expert without any"""
+    r = rng_of(43, K)
+    N, counts = 2500, [129, 1, 0, 33, 200, 96, 310, 64, 512, 65, 127, 160]
+    E, Tn = len(counts), sum(counts)
+    w, x, b = weights(r, E, N, K), acts(r, Tn, 1, K), r.standard_normal((E, N)).astype(np.float32)
+    ids = np.repeat(np.arange(E, dtype=np.int32), counts)[r.permutation(Tn)][:, None]
+    want, mags = mx_ref.experts(x, w, ids, b)
+    mx_ref.check("short", run_experts(backend, w, x, ids, b, K, N), want, mags, K, extra=np.abs(b[ids]))
+
+
 def test_bias_of_fewer_experts(backend):
     """ids behind the bias rows' last: the product alone (ADD_ID), also where the two could be one launch"""
     r = rng_of(37)
