@@ -174,10 +174,21 @@ class _Memory:
         self.__cuda_array_interface__ = {"shape": shape, "typestr": "<f4", "data": (address, False), "strides": None, "version": 2}
 
 
+class _Event(C.Structure):
+    """struct ggml_backend_event (include/ggml_abi.h) around an event of torch's: its context is the hipEvent_t"""
+
+    _fields_ = [("device", C.c_void_p), ("context", C.c_void_p)]
+
+    def __init__(self, device):
+        self.torch = torch.cuda.Event()
+        self.torch.record()  # (its first record makes it)
+        super().__init__(device, self.torch.cuda_event)
+
+
 class _Graph:
     """The graph of one case with its tensors in the backend's memory, as an engine keeps them."""
 
-    backend = None  # one for the process, as an engine has
+    backend = None  # one for the process, as an engine has, with the two events that order its stream and torch's
 
     def __init__(self, s):
         import llama_box_amd as L
@@ -185,6 +196,9 @@ class _Graph:
         self.L, self.H = L, L.host()
         if _Graph.backend is None:
             _Graph.backend = L.Backend(0)
+            _Graph.begun, _Graph.done = _Event(_Graph.backend.dev), _Event(_Graph.backend.dev)
+            for f in (L.host().ggml_backend_event_wait, L.host().ggml_backend_event_record):
+                f.restype, f.argtypes = None, [C.c_void_p, C.c_void_p]
         H, c = self.H, s["case"]
         self.kept = _Kept(L)
         weights, work = self.kept.ctxs  # weights; everything else
@@ -227,8 +241,15 @@ class _Graph:
         self.out = torch.as_tensor(_Memory(self.kept, out.contents.data, shape), device="cuda")
 
     def __call__(self):
-        if self.H.ggml_backend_graph_compute_async(_Graph.backend.backend, self.graph) != 0:
+        # the backend's stream behind what torch's stream holds (the last reader of the output, too), torch's behind the graph
+        H, backend, begun, done = self.H, _Graph.backend.backend, _Graph.begun, _Graph.done
+        stream = torch.cuda.current_stream()
+        begun.torch.record(stream)
+        H.ggml_backend_event_wait(backend, C.addressof(begun))
+        if H.ggml_backend_graph_compute_async(backend, self.graph) != 0:
             raise RuntimeError("graph_compute failed")
+        H.ggml_backend_event_record(C.addressof(done), backend)
+        stream.wait_event(done.torch)
         return self.out
 
 
