@@ -1,0 +1,78 @@
+"""The calls of perf/operators.py that go through the backend, used beside torch's own work as a program would: no wait for the device between the two."""
+import importlib.util
+import os
+
+import pytest
+
+import harness as T
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(built):
+    spec = importlib.util.spec_from_file_location("operator_calls", os.path.join(T.REPO, "perf", "operators.py"))
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    yield m
+    m.own = False
+
+
+CASES = [
+    {"kind": "store", "width": 96, "rows": 300, "taken": 17},
+    {"kind": "convert", "width": 1024, "rows": 2000, "taken": 2000},
+    {"kind": "read", "width": 1024, "rows": 900, "taken": 700},
+    {"kind": "product", "width": 1056, "out": 1001, "cols": 1},
+    {"kind": "product", "width": 2048, "out": 4096, "cols": 700},
+    {"kind": "experts", "width": 256, "out": 333, "experts": 5, "used": 2, "tokens": 3, "shared": False},
+    {"kind": "experts", "width": 512, "out": 1024, "experts": 8, "used": 3, "tokens": 500, "shared": True},
+]
+
+
+def close(a, b, case):
+    """rows equal; products: f32 sums of 2 K products on one side and K on the other, each as far from the true sum as mx_ref.check derives in the 2-norm (sqrt(2 K) + 1 roundings of 2^-24)"""
+    import torch
+
+    if case["kind"] in ("store", "convert", "read"):
+        return torch.equal(a, b)
+    return float((a.double() - b.double()).norm() / b.double().norm()) <= 2.0**-24 * 2 * ((2 * case["width"]) ** 0.5 + 1)
+
+
+def by_name(case):
+    return "-".join(str(v) for v in case.values())
+
+
+@pytest.mark.parametrize("case", CASES, ids=by_name)
+def test_result_is_read_by_torch_at_once(ops, case):
+    """a call's result, filled by torch just before it and read by torch just behind it"""
+    import torch
+
+    ops.own = False
+    want = ops.run(ops.prepare(case, 5)).clone()
+    ops.own = True
+    s = ops.prepare(case, 5)
+    out = ops.run(s)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        out.fill_(float("nan"))
+        got = ops.run(s).clone()
+        assert got.data_ptr() != out.data_ptr()
+        assert close(got, want, case)
+
+
+def test_call_waits_for_torch(ops):
+    """torch still reads the last result, behind other work of its stream, when the next call comes"""
+    import torch
+
+    case = {"kind": "product", "width": 2048, "out": 4096, "cols": 40}
+    ops.own = True
+    a = ops.prepare(case, 7)
+    first = ops.run(a).clone()
+    torch.cuda.synchronize()
+    out = ops.run(a)
+    torch.cuda._sleep(20_000_000)  # (some 10 ms of the stream's time)
+    out.fill_(3.0)
+    kept = out.clone()
+    again = ops.run(a).clone()
+    torch.cuda.synchronize()
+    assert bool((kept == 3.0).all()) and torch.equal(again, first)
