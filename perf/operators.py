@@ -152,28 +152,6 @@ def _plain(s):
 
 
 # ------------------------------------------------------------------------------------------ the framework's operators
-class _Kept:
-    """What the backend's memory of one case hangs on: given back when neither the graph nor an output of it is left."""
-
-    def __init__(self, L):
-        self.H, self.bufs = L.host(), []
-        self.ctxs = [self.H.ggml_init(L.InitParams(0, None, True)) for _ in range(2)]
-
-    def __del__(self):
-        for b in self.bufs:
-            self.H.ggml_backend_buffer_free(b)
-        for k in self.ctxs:
-            self.H.ggml_free(k)
-
-
-class _Memory:
-    """f32 memory of the backend as an array that torch reads in place; the tensor made of it keeps it, and it keeps the memory"""
-
-    def __init__(self, kept, address, shape):
-        self.kept = kept
-        self.__cuda_array_interface__ = {"shape": shape, "typestr": "<f4", "data": (address, False), "strides": None, "version": 2}
-
-
 class _Event(C.Structure):
     """struct ggml_backend_event (include/ggml_abi.h) around an event of torch's: its context is the hipEvent_t"""
 
@@ -186,61 +164,64 @@ class _Event(C.Structure):
 
 
 class _Graph:
-    """The graph of one case with its tensors in the backend's memory, as an engine keeps them."""
+    """The graph of one case, as an engine keeps it. Its tensors lie where the state's lie: every call takes their addresses anew and reads and writes them there."""
 
     backend = None  # one for the process, as an engine has, with the two events that order its stream and torch's
 
     def __init__(self, s):
         import llama_box_amd as L
 
-        self.L, self.H = L, L.host()
+        self.H = H = L.host()
         if _Graph.backend is None:
             _Graph.backend = L.Backend(0)
             _Graph.begun, _Graph.done = _Event(_Graph.backend.dev), _Event(_Graph.backend.dev)
-            for f in (L.host().ggml_backend_event_wait, L.host().ggml_backend_event_record):
+            for f in (H.ggml_backend_event_wait, H.ggml_backend_event_record):
                 f.restype, f.argtypes = None, [C.c_void_p, C.c_void_p]
-        H, c = self.H, s["case"]
-        self.kept = _Kept(L)
-        weights, work = self.kept.ctxs  # weights; everything else
-        data = []
+        self.ctx = ctx = H.ggml_init(L.InitParams(0, None, True))
+        self.theirs, self.room = [], []  # (tensor, the state's name for it); memory between two operators
 
-        def put(ctx, kind, ne, t):
-            r = H.ggml_new_tensor_4d(ctx, kind, *(list(ne) + [1] * (4 - len(ne))))
-            data.append((r, t))
-            return r
+        def of_state(t, key):
+            self.theirs.append((t.contents, key))
+            return t
 
-        k = c["kind"]
-        K = c["width"]
+        def leaf(kind, ne, key):
+            return of_state(H.ggml_new_tensor_4d(ctx, kind, *(list(ne) + [1] * (4 - len(ne)))), key)
+
+        def between(t):
+            self.room.append(torch.empty(H.ggml_nbytes(t), dtype=torch.uint8, device="cuda"))
+            t.contents.data = self.room[-1].data_ptr()
+            return t
+
+        c = s["case"]
+        k, K = c["kind"], c["width"]
         if k == "store":
-            table = put(work, L.MXFP4, (K, c["rows"]), s["table"])
-            stored = H.ggml_set_rows(work, table, put(work, L.F32, (K, c["taken"]), s["x"]), put(work, L.I64, (c["taken"],), s["slots"]))
-            out, shape = H.ggml_get_rows(work, stored, put(work, L.I32, (s["order"].numel(),), s["order"])), (s["order"].numel(), K)
+            n = s["order"].numel()
+            stored = of_state(H.ggml_set_rows(ctx, leaf(L.MXFP4, (K, c["rows"]), "table"), leaf(L.F32, (K, c["taken"]), "x"), leaf(L.I64, (c["taken"],), "slots")), "table")
+            out, shape = H.ggml_get_rows(ctx, stored, leaf(L.I32, (n,), "order")), (n, K)
         elif k == "convert":
-            x = put(work, L.F32, (K, c["rows"]), s["x"])
-            out, shape = H.ggml_cast(work, H.ggml_cast(work, x, L.MXFP4), L.F32), (c["rows"], K)
+            out, shape = H.ggml_cast(ctx, between(H.ggml_cast(ctx, leaf(L.F32, (K, c["rows"]), "x"), L.MXFP4)), L.F32), (c["rows"], K)
         elif k == "read":
-            out, shape = H.ggml_get_rows(work, put(weights, L.MXFP4, (K, c["rows"]), s["table"]), put(work, L.I32, (s["order"].numel(),), s["order"])), (s["order"].numel(), K)
+            n = s["order"].numel()
+            out, shape = H.ggml_get_rows(ctx, leaf(L.MXFP4, (K, c["rows"]), "table"), leaf(L.I32, (n,), "order")), (n, K)
         elif k == "product":
-            out, shape = H.ggml_mul_mat(work, put(weights, L.MXFP4, (K, c["out"]), s["w"]), put(work, L.F32, (K, c["cols"]), s["x"])), (c["cols"], c["out"])
+            out, shape = H.ggml_mul_mat(ctx, leaf(L.MXFP4, (K, c["out"]), "w"), leaf(L.F32, (K, c["cols"]), "x")), (c["cols"], c["out"])
         else:
             T, U, N = c["tokens"], c["used"], c["out"]
-            ids = put(work, L.I32, (U, T), s["ids"])
-            y = H.ggml_mul_mat_id(work, put(weights, L.MXFP4, (K, N, c["experts"]), s["w"]), put(work, L.F32, (K, 1 if c["shared"] else U, T), s["x"]), ids)
-            out, shape = H.ggml_add_id(work, y, put(weights, L.F32, (N, c["experts"]), s["bias"]), ids), (T, U, N)
+            ids = leaf(L.I32, (U, T), "ids")
+            y = between(H.ggml_mul_mat_id(ctx, leaf(L.MXFP4, (K, N, c["experts"]), "w"), leaf(L.F32, (K, 1 if c["shared"] else U, T), "x"), ids))
+            out, shape = H.ggml_add_id(ctx, y, leaf(L.F32, (N, c["experts"]), "bias"), ids), (T, U, N)
         H.ggml_set_output(out)
-        self.graph = H.ggml_new_graph(work)
+        self.graph = H.ggml_new_graph(ctx)
         H.ggml_build_forward_expand(self.graph, out)
-        for ctx, usage in ((weights, 1), (work, 0)):
-            buf = H.ggml_backend_alloc_ctx_tensors_from_buft(ctx, _Graph.backend.buft)
-            if buf:  # (none for a context without tensors)
-                H.ggml_backend_buffer_set_usage(buf, usage)
-                self.kept.bufs.append(buf)
-        for r, t in data:
-            a = t.contiguous().cpu().numpy()
-            H.ggml_backend_tensor_set(r, a.ctypes.data_as(C.c_void_p), 0, a.nbytes)
-        self.out = torch.as_tensor(_Memory(self.kept, out.contents.data, shape), device="cuda")
+        self.out = torch.empty(shape, device="cuda")
+        out.contents.data = self.out.data_ptr()
 
-    def __call__(self):
+    def __del__(self):
+        self.H.ggml_free(self.ctx)
+
+    def __call__(self, s):
+        for t, key in self.theirs:
+            t.data = s[key].data_ptr()
         # the backend's stream behind what torch's stream holds (the last reader of the output, too), torch's behind the graph
         H, backend, begun, done = self.H, _Graph.backend.backend, _Graph.begun, _Graph.done
         stream = torch.cuda.current_stream()
@@ -290,7 +271,7 @@ def prepare(case, seed):
 
 
 def run(s):
-    return s["graph"]() if own else _plain(s)
+    return s["graph"](s) if own else _plain(s)
 
 
 # ------------------------------------------------------------------------------------------ what a pass cannot do without
