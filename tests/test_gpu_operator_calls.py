@@ -76,3 +76,30 @@ def test_call_waits_for_torch(ops):
     again = ops.run(a).clone()
     torch.cuda.synchronize()
     assert bool((kept == 3.0).all()) and torch.equal(again, first)
+
+
+@pytest.mark.parametrize("case", CASES, ids=by_name)
+def test_inputs_changed_between_two_calls(ops, case):
+    """a call takes what the state's tensors hold and which tensors they are when it comes: written anew in place behind other work of torch's stream, and exchanged for others"""
+    import torch
+
+    ops.own = False
+    plain = [ops.prepare(case, seed) for seed in (11, 12)]
+    names = [k for k, v in plain[0].items() if isinstance(v, torch.Tensor)]
+    given = [{k: p[k].clone() for k in names} for p in plain]
+    want = [ops.run(p).clone() for p in plain]
+    stored = [p.get("table") for p in plain]
+    ops.own = True
+    s = ops.prepare(case, 11)
+    got = [ops.run(s).clone()]
+    torch.cuda._sleep(5_000_000)
+    for k in names:
+        s[k].copy_(given[1][k])
+    got.append(ops.run(s).clone())
+    for k in names:
+        s[k] = given[0][k]
+    got.append(ops.run(s).clone())
+    for g, w in zip(got, (want[0], want[1], want[0])):
+        assert close(g, w, case)
+    if case["kind"] == "store":
+        assert torch.equal(s["table"], stored[0])  # (the rows are in the state's own table)
