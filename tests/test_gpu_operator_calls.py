@@ -1,105 +1,26 @@
-"""The calls of perf/operators.py that go through the backend, used beside torch's own work as a program would: no wait for the device between the two."""
-import importlib.util
+"""The calls of perf/operators.py that go through the backend, used beside torch's own work as a program would: no wait for the device between the two (checks: operator_calls_worker.py)."""
 import os
+import re
+import subprocess
+import sys
 
 import pytest
 
-import harness as T
+import llama_box_amd as L
 
-pytestmark = pytest.mark.gpu
+WORKER = os.path.join(L.REPO, "tests", "operator_calls_worker.py")
+CHECKS = [(c, k) for c in ("result_is_read_at_once", "call_waits", "inputs_changed") for k in ("store", "convert", "read", "product", "experts") if (c, k) != ("call_waits", "store")]
 
 
 @pytest.fixture(scope="module")
-def ops(built):
-    spec = importlib.util.spec_from_file_location("operator_calls", os.path.join(T.REPO, "perf", "operators.py"))
-    m = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(m)
-    yield m
-    m.own = False
+def said(built):
+    r = subprocess.run([sys.executable, "-u", WORKER], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-3000:]
+    return r.stdout
 
 
-CASES = [
-    {"kind": "store", "width": 96, "rows": 300, "taken": 17},
-    {"kind": "convert", "width": 1024, "rows": 2000, "taken": 2000},
-    {"kind": "read", "width": 1024, "rows": 900, "taken": 700},
-    {"kind": "product", "width": 1056, "out": 1001, "cols": 1},
-    {"kind": "product", "width": 2048, "out": 4096, "cols": 700},
-    {"kind": "experts", "width": 256, "out": 333, "experts": 5, "used": 2, "tokens": 3, "shared": False},
-    {"kind": "experts", "width": 512, "out": 1024, "experts": 8, "used": 3, "tokens": 500, "shared": True},
-]
-
-
-def close(a, b, case):
-    """rows equal; products: f32 sums of 2 K products on one side and K on the other, each as far from the true sum as mx_ref.check derives in the 2-norm (sqrt(2 K) + 1 roundings of 2^-24)"""
-    import torch
-
-    if case["kind"] in ("store", "convert", "read"):
-        return torch.equal(a, b)
-    return float((a.double() - b.double()).norm() / b.double().norm()) <= 2.0**-24 * 2 * ((2 * case["width"]) ** 0.5 + 1)
-
-
-def by_name(case):
-    return "-".join(str(v) for v in case.values())
-
-
-@pytest.mark.parametrize("case", CASES, ids=by_name)
-def test_result_is_read_by_torch_at_once(ops, case):
-    """a call's result, filled by torch just before it and read by torch just behind it"""
-    import torch
-
-    ops.own = False
-    want = ops.run(ops.prepare(case, 5)).clone()
-    ops.own = True
-    s = ops.prepare(case, 5)
-    out = ops.run(s)
-    torch.cuda.synchronize()
-    for _ in range(5):
-        out.fill_(float("nan"))
-        got = ops.run(s).clone()
-        assert got.data_ptr() != out.data_ptr()
-        assert close(got, want, case)
-
-
-def test_call_waits_for_torch(ops):
-    """torch still reads the last result, behind other work of its stream, when the next call comes"""
-    import torch
-
-    case = {"kind": "product", "width": 2048, "out": 4096, "cols": 40}
-    ops.own = True
-    a = ops.prepare(case, 7)
-    first = ops.run(a).clone()
-    torch.cuda.synchronize()
-    out = ops.run(a)
-    torch.cuda._sleep(20_000_000)  # (some 10 ms of the stream's time)
-    out.fill_(3.0)
-    kept = out.clone()
-    again = ops.run(a).clone()
-    torch.cuda.synchronize()
-    assert bool((kept == 3.0).all()) and torch.equal(again, first)
-
-
-@pytest.mark.parametrize("case", CASES, ids=by_name)
-def test_inputs_changed_between_two_calls(ops, case):
-    """a call takes what the state's tensors hold and which tensors they are when it comes: written anew in place behind other work of torch's stream, and exchanged for others"""
-    import torch
-
-    ops.own = False
-    plain = [ops.prepare(case, seed) for seed in (11, 12)]
-    names = [k for k, v in plain[0].items() if isinstance(v, torch.Tensor)]
-    given = [{k: p[k].clone() for k in names} for p in plain]
-    want = [ops.run(p).clone() for p in plain]
-    stored = [p.get("table") for p in plain]
-    ops.own = True
-    s = ops.prepare(case, 11)
-    got = [ops.run(s).clone()]
-    torch.cuda._sleep(5_000_000)
-    for k in names:
-        s[k].copy_(given[1][k])
-    got.append(ops.run(s).clone())
-    for k in names:
-        s[k] = given[0][k]
-    got.append(ops.run(s).clone())
-    for g, w in zip(got, (want[0], want[1], want[0])):
-        assert close(g, w, case)
-    if case["kind"] == "store":
-        assert torch.equal(s["table"], stored[0])  # (the rows are in the state's own table)
+@pytest.mark.gpu
+@pytest.mark.parametrize("check,kind", CHECKS)
+def test_calls_beside_torch(said, check, kind):
+    begun, done = (re.findall(rf"^{word} ({check}:{kind}-\S+)$", said, re.M) for word in ("CHECK", "OK"))
+    assert begun and begun == done, said[-6000:]
