@@ -829,9 +829,10 @@ template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, 2) k_
 // without both 2.7: 170 KB a stage and CU on the one path from L2 (its address unit works 64 % of the time).  What left the time as it was: rows in LDS 144 bytes apart, without a bank conflict (whole
 // rows: half of LDS's cycles), and a product of another tile between the two of a tile.  In a quarter that starts at a unit of 8 bytes (the odd ones: at its
 // second half) block i starts at byte i of a unit, and needs the two units behind it: one 16-byte read a block (the unit between two blocks is kept) and up to four byte shifts.
-__device__ __forceinline__ void mx_dma16(const uint8_t * base, const uint32_t off, const uint32_t lds) {  // lane i's 16 bytes at base + off to LDS[lds + 16 i]; base and lds of the wave
+// lane i's 16 bytes at base + off to LDS[lds + 16 i]; base and lds of the wave.  ("memory": the stage's one barrier waits for it by counting the requests behind it, none of which may move in front)
+__device__ __forceinline__ void mx_dma16(const uint8_t * base, const uint32_t off, const uint32_t lds) {
     uint32_t keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0" : "=&s"(keep) : "v"(off), "s"(base), "s"(lds));
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0" : "=&s"(keep) : "v"(off), "s"(base), "s"(lds) : "memory");
 }
 template <int RT> constexpr int mx_wide_pieces() { return (32 * RT * 17 + 511) / 512; }  // DMA instructions a wave and stage
 template <int RT> struct mx_wide_args {
@@ -927,7 +928,7 @@ template <int RT, int ODD> __device__ __forceinline__ void mx_wide_sum(const mx_
             const int i = g / SETS, t0 = (g % SETS) * SET;
             const mx_i8 hx = mx_op6(h4[i], h2[i]), lx = mx_op6(l4[i], l2[i]);
             const uint32_t sh = sx, sl = sh - 0x04040404u;
-            // (as many requests of digits lie behind the last DMA: those of block 1 and, with eight tiles, 2)
+            // (at least as many requests of digits lie behind the last DMA: those of block 1 and, with four tiles and eight, 2)
             if (g == GROUPS - 2) {
                 if (RT == 8) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 else asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
