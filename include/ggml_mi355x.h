@@ -57,6 +57,7 @@ ggml_backend_reg_t ggml_backend_mi355x_reg(void);
  *   "ggml_backend_mi355x_graph_key_probe" ggml_backend_mi355x_graph_key_probe_t   (tests: is graph b the graph a captured hipGraph of a stands for?)
  *   "ggml_backend_mi355x_scratch_probe"   ggml_backend_mi355x_scratch_probe_t   (tests: the scratch that a graph's partial products and records may take)
  *   "ggml_backend_mi355x_k_slices"        ggml_backend_mi355x_k_slices_t        (tests: K slices of a K-quant product)
+ *   "ggml_backend_mi355x_mx_tile_rows"    ggml_backend_mi355x_mx_tile_rows_t    (tests: rows of a tile of an MXFP4 product)
  *   "ggml_backend_mi355x_supports_probe"  ggml_backend_mi355x_supports_probe_t  (tests: what a device's supports_op answers)
  *   "ggml_backend_mi355x_prepare_columns" ggml_backend_mi355x_prepare_columns_t
  *   "ggml_backend_mi355x_result_to"       ggml_backend_mi355x_result_to_t
@@ -99,6 +100,9 @@ typedef int (*ggml_backend_mi355x_graph_key_probe_t)(const struct ggml_cgraph * 
  * n_cols columns.  Host arithmetic: both work without a device. */
 typedef int64_t (*ggml_backend_mi355x_scratch_probe_t)(const struct ggml_cgraph * g);
 typedef int (*ggml_backend_mi355x_k_slices_t)(int type, int64_t K, int64_t n_rows, int64_t n_cols);
+
+/* Rows of the tiles in which a product of cols columns by a dense MXFP4 matrix [K, N] runs (n_expert: by as many, MUL_MAT_ID; 0: MUL_MAT); 0 where it takes a form without tiles.  Host arithmetic. */
+typedef int (*ggml_backend_mi355x_mx_tile_rows_t)(int64_t K, int64_t N, int64_t n_expert, int64_t cols);
 
 /* 1 where a device of this registration would take operator `op`, else 0.  Host arithmetic: works without a device. */
 typedef int (*ggml_backend_mi355x_supports_probe_t)(const struct ggml_tensor * op);

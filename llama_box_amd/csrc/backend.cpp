@@ -1013,6 +1013,7 @@ static int api_graph_key_probe(const ggml_cgraph * a, const ggml_cgraph * b, int
 static int64_t api_scratch_probe(const ggml_cgraph * g) { return partials_reserved(g); }
 static int api_supports_probe(const ggml_tensor * op) { return supports_op(op) ? 1 : 0; }
 static int api_k_slices(int type, int64_t K, int64_t n_rows, int64_t M) { return mmq_pick_ksplit(K, n_rows, M, options().mmq_skinny, type); }
+static int api_mx_tile_rows(int64_t K, int64_t N, int64_t n_expert, int64_t cols) { return mx_tile_rows_of(K, N, n_expert, cols); }
 static int api_prepare_columns(ggml_backend_t be, const ggml_tensor * const * w, int n, int64_t from, int64_t to) {
     if (!be_is_ours(be) || w == nullptr || n < 1 || std::find(w, w + n, nullptr) != w + n) return -1;
     backend_ctx * c = (backend_ctx *) be->context;
@@ -1185,6 +1186,7 @@ static void * reg_get_proc_address(ggml_backend_reg_t, const char * name) {
     if (n == "ggml_backend_mi355x_graph_key_probe") return (void *) api_graph_key_probe;
     if (n == "ggml_backend_mi355x_scratch_probe") return (void *) api_scratch_probe;
     if (n == "ggml_backend_mi355x_supports_probe") return (void *) api_supports_probe;
+    if (n == "ggml_backend_mi355x_mx_tile_rows") return (void *) api_mx_tile_rows;
     if (n == "ggml_backend_mi355x_k_slices") return (void *) api_k_slices;
     return nullptr;
 }

@@ -543,6 +543,7 @@ void launch_mx_read(hipStream_t s, const tdesc & a, const tdesc * idx, const tde
 bool mx_vec_takes(int64_t K, int64_t N, int64_t cols);
 bool mx_id_vec_takes(int64_t K, int64_t N, int64_t cols);
 bool mx_product_ok(const tdesc & w, const tdesc & b);
+int mx_tile_rows_of(int64_t K, int64_t N, int64_t n_expert, int64_t cols);  // rows of a tile of dense matrices (n_expert 0: MUL_MAT); 0: a form without tiles
 size_t mx_act_bytes(int64_t K, int64_t cols);
 void launch_mx_act(hipStream_t s, const tdesc & b, void * act);
 void launch_mx_mul_mat(hipStream_t s, const tdesc & w, const tdesc & b, const tdesc & d, const void * act);

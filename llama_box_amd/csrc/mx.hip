@@ -1131,9 +1131,16 @@ template <bool ID> static void mx_launch_tile(hipStream_t s, const mx_mm & p, in
     else if (rt == 4) mx_launch_tile_of<ID, 4>(s, p, tiles);
     else mx_launch_tile_of<ID, 2>(s, p, tiles);
 }
-static int mx_tile_rows(int64_t N, int64_t tiles, int64_t groups, bool tail) {
+// Rows of a tile, in units of 32, among the heights that there is a kernel for: of rows in whole pieces 64, 128 and 256 where the matrix has as many (k_mx_wide, the costs above); of others 64 and 128
+// (k_mx_tile): 128 from 512 tiles of 64 on, two a CU, or 2200 of experts with few columns each (`each`).  us, tiles of 64 | 128 rows: 384 / 1024 / 2048 columns of 2080 x 14336 29.4 / 62.7 / 124 |
+// 27.4 / 53.6 / 98, 512 / 1024 / 2048 of 4064 x 4096 31.9 / 39.7 / 69 | 35.0 / 36.5 / 55, 1024 of 4224 x 2080 34.2 | 36.5; 2, 15 / 62 columns an expert, 32 experts of 2080 x 2080 25.5, 38.4 / 53.2 |
+// 27.5, 39.6 / 49.9, of 1056 x 4096 25.9, 34.8 / 46.2 | 29.2, 34.1 / 46.0, 15 of 128 experts of 2080 x 2080 123 | 113
+static int mx_tile_rows(const mx_mm & p, int64_t tiles, int64_t groups, int64_t each, bool tail) {
+    const int64_t N = p.n_rows;
+    if (!mx_pieces(p)) return N > 64 && (N + 63) / 64 * tiles >= (each >= 48 ? 512 : 2200) ? 4 : 2;
     int head, low;
-    const int64_t c2 = mx_tile_cost(2, N, tiles, groups), c4 = mx_tile_cost(4, N, tiles, groups), c8 = tail && groups >= 4 ? mx_tail(N, tiles, head, low) : mx_tile_cost(8, N, tiles, groups);
+    const int64_t never = INT64_MAX, c2 = mx_tile_cost(2, N, tiles, groups), c4 = N >= 128 ? mx_tile_cost(4, N, tiles, groups) : never;
+    const int64_t c8 = N < 256 ? never : tail && groups >= 4 ? mx_tail(N, tiles, head, low) : mx_tile_cost(8, N, tiles, groups);
     return c8 <= c4 && c8 <= c2 ? 8 : c4 <= c2 ? 4 : 2;
 }
 // Four waves where the rows and groups alone fill the GPU, eight where they do not (us for 8 / 32 columns, four waves | eight: 4096 rows of 14336 18.3 / 21.2 | 18.6 / 20.3, 14336 of 4096 15.4 / 17.1 |
@@ -1145,17 +1152,38 @@ template <bool ID> static void mx_launch_few(hipStream_t s, const mx_mm & p, int
     if (mx_dwords(p)) hipLaunchKernelGGL((k_mx_few<ID, true>), grid, block, lds, s, p);
     else hipLaunchKernelGGL((k_mx_few<ID, false>), grid, block, lds, s, p);
 }
+// the tiles' rows in units of 32, or 0: k_mx_few
+static int mx_form(const mx_mm & p) {
+    const int64_t groups = (p.cols + 31) / 32, tiles = (p.cols + 127) / 128;
+    return mx_few_cost(p.n_rows, groups) < mx_tile_cost(2, p.n_rows, tiles, groups) ? 0 : mx_tile_rows(p, tiles, groups, p.cols, mx_pieces(p));
+}
+// With fewer than 64 columns an expert the weights' way from memory counts for more than the products: of rows in whole pieces tiles of 256 rows where there are two rounds of them, of 64 (two workgroups a CU)
+// elsewhere.  us, 64 | 256 rows, 10 / 28 columns an expert: 32 experts of 2048 x 4096 44 / 68 | 46 / 56, of 1024 x 1024 15.7 / 19.6 | 20.6 / 23.4, 128 of 2048 x 768 40 / 51 | 48 / 55
+static int mx_id_form(const mx_mm & p) {
+    const int64_t g = mx_id_groups(p.n_expert, p.cols), tiles = mx_id_tiles(p.n_expert, p.cols), each = p.cols / p.n_expert;
+    if (mx_few_cost(p.n_rows, g) < mx_tile_cost(2, p.n_rows, tiles, each / 32 + 1)) return 0;
+    if (each >= 64 || !mx_pieces(p)) return mx_tile_rows(p, tiles, 4, each, false);
+    return each >= 16 && p.n_rows / 256 * tiles >= 512 ? 8 : 2;
+}
+int mx_tile_rows_of(int64_t K, int64_t N, int64_t n_expert, int64_t cols) {
+    mx_mm p{};
+    p.blocks = (int) (K / 32);
+    p.nb1 = K / 32 * MX_BLOCK;
+    p.nb2 = p.nb1 * N;
+    p.n_rows = (int) N;
+    p.n_expert = (int) n_expert;
+    p.cols = cols;
+    if (n_expert ? mx_id_vec_takes(K, N, cols) : mx_vec_takes(K, N, cols)) return 0;
+    return 32 * (n_expert ? mx_id_form(p) : mx_form(p));
+}
 // act: null where mx_vec_takes
 void launch_mx_mul_mat(hipStream_t s, const tdesc & w, const tdesc & b, const tdesc & d, const void * act) {
     mx_mm p = mx_args(w, d, b.ne[1] * b.ne[2] * b.ne[3]);
     p.act = (const uint8_t *) act;
     if (p.n_rows == 0 || p.cols == 0) return;
-    if (!act) mx_launch_vec(s, p, b, nullptr);
-    else {
-        const int64_t groups = (p.cols + 31) / 32, tiles = (p.cols + 127) / 128;
-        if (mx_few_cost(p.n_rows, groups) < mx_tile_cost(2, p.n_rows, tiles, groups)) mx_launch_few<false>(s, p, groups);
-        else mx_launch_tile<false>(s, p, tiles, mx_tile_rows(p.n_rows, tiles, groups, mx_pieces(p)));
-    }
+    if (!act) return mx_launch_vec(s, p, b, nullptr);
+    if (const int rt = mx_form(p)) mx_launch_tile<false>(s, p, (p.cols + 127) / 128, rt);
+    else mx_launch_few<false>(s, p, (p.cols + 31) / 32);
 }
 void launch_mx_mul_mat_id(hipStream_t s, const tdesc & w, const tdesc & b, const tdesc & ids, const tdesc & d, const void * ws, const float * bias, int64_t nb_bias) {
     const int64_t cols = ids.ne[0] * ids.ne[1], g = mx_id_groups(w.ne[2], cols);
@@ -1166,12 +1194,8 @@ void launch_mx_mul_mat_id(hipStream_t s, const tdesc & w, const tdesc & b, const
     if (!ws) return mx_launch_vec(s, p, b, &ids);
     p.act = (const uint8_t *) ws + mx_lists_bytes(g);
     p.l = mx_lists_at((void *) ws, g);
-    // With fewer than 64 columns an expert the weights' way from memory counts for more than the products: tiles of 256 rows where there are two rounds of them, of 64 (two workgroups a CU) elsewhere.  us, 64 |
-    // 256 rows, 10 / 28 columns an expert: 32 experts of 2048 x 4096 44 / 68 | 46 / 56, of 1024 x 1024 15.7 / 19.6 | 20.6 / 23.4, 128 of 2048 x 768 40 / 51 | 48 / 55
-    const int64_t tiles = mx_id_tiles(w.ne[2], cols), each = cols / w.ne[2];
-    if (mx_few_cost(p.n_rows, g) < mx_tile_cost(2, p.n_rows, tiles, each / 32 + 1)) mx_launch_few<true>(s, p, g);
-    else if (each >= 64) mx_launch_tile<true>(s, p, tiles, mx_tile_rows(p.n_rows, tiles, 4, false));
-    else mx_launch_tile<true>(s, p, tiles, each >= 16 && p.n_rows / 256 * tiles >= 512 ? 8 : 2);
+    if (const int rt = mx_id_form(p)) mx_launch_tile<true>(s, p, mx_id_tiles(w.ne[2], cols), rt);
+    else mx_launch_few<true>(s, p, g);
 }
 // Which operands the products take (type and shape; the rows of both are dense, whole blocks).  The kernels hold offsets inside a tile of 256 rows and inside a group's digits in 32 bits, and a launch less than
 // 2^32 threads in x
