@@ -46,17 +46,29 @@ def test_reading_of_a_listing():
     assert waits(ok[:3] + ["s_cbranch_scc1 12"] + ok[3:]) == [] and waits(ok[:-1] + ["v_mov_b32 v1, v2"]) == []
 
 
-def test_stage_waits_cover_the_dma(built, tmp_path):
-    """k_mx_wide waits for a stage's DMA with vmcnt(n), n digit requests behind the last DMA: requests complete in order, so at least n of them have to lie there in every build of it"""
+@pytest.fixture(scope="module")
+def listing(built, tmp_path_factory):
+    """{symbol: instructions} of the kernels of the file that holds the MXFP4 products"""
     if not os.path.exists(OBJDUMP):
         pytest.skip("no llvm-objdump")
     with open(L.BACKEND_SO, "rb") as f:
         elfs = [e for e in code_objects(f.read()) if b"k_mx_wide" in e]
     assert len(elfs) == 1
-    path = tmp_path / "mx.elf"
+    path = tmp_path_factory.mktemp("mx") / "mx.elf"
     path.write_bytes(elfs[0])
     text = subprocess.run([OBJDUMP, "-d", "--mcpu=gfx950", str(path)], capture_output=True, text=True, check=True).stdout
-    kernels = {m[1]: m[2].splitlines() for m in re.finditer(r"<(\w*k_mx_wide\w*)>:\n(.*?)(?=\n\n|\Z)", text, re.S)}
+    return {m[1]: m[2].splitlines() for m in re.finditer(r"<(\w+)>:\n(.*?)(?=\n\n|\Z)", text, re.S)}
+
+
+def test_results_stay_in_reach_of_their_reader(listing):
+    """no store of a product goes past the caches, from where the next node reads it"""
+    stores = [ln for name, lines in listing.items() if "k_mx_" in name for ln in lines if re.search(r"\b(global|buffer|flat)_store", ln)]
+    assert stores and not [ln for ln in stores if re.search(r"\b(nt|sc1)\b", ln)]
+
+
+def test_stage_waits_cover_the_dma(listing):
+    """k_mx_wide waits for a stage's DMA with vmcnt(n), n digit requests behind the last DMA: requests complete in order, so at least n of them have to lie there in every build of it"""
+    kernels = {name: lines for name, lines in listing.items() if "k_mx_wide" in name}
     assert len(kernels) == 6  # two, four and eight row tiles, of one matrix and of experts
     for name, lines in kernels.items():
         counted = [(n, behind) for n, behind in waits(lines) if n > 0]
