@@ -436,12 +436,13 @@ template <> struct mx_raw<false> {
     ACC = __builtin_amdgcn_mfma_scale_f32_##N##_f8f6f4(mx_op4(A), H, ACC, MX_FP4, MX_FP6, J, S, J, (int) (SH));              \
     ACC = __builtin_amdgcn_mfma_scale_f32_##N##_f8f6f4(mx_op4(A), L, ACC, MX_FP4, MX_FP6, J, S, J, (int) (SL));
 
-// ---- one to a few columns: 16 rows a workgroup, its waves take four steps of 128 values in turn.  The workgroup quantises its columns itself, while its first weights are on the way.  A lane of
+// ---- one to a few columns: 16 rows a workgroup, its waves take four steps of 128 values in turn.  The workgroup quantises its columns itself, behind the requests of its first weights (both are
+// there before the first product: requests complete in order).  A lane of
 // v_mfma_scale_f32_16x16x128: row (column) lane % 16, step lane / 16 of the four.  The weights' bytes bound it, behind the launch (us, with the 3.5 of a step's one launch: one column of 14336 x 4096,
 // 31 MB, 10.2; of 4096 x 4096 4.5; a token's 4 experts of 2048 x 4096, 18 MB, 6.6).  ONE: a wave has one turn, and no registers for the weights of a second (half as many, twice the waves: 8.7 us)
 // ID: blockIdx.y is a column (u + n_used t) of at most 64; the first column of an expert takes all of its expert, the others' workgroups end at once.
 static constexpr int MX_VEC_REC = 48;     // LDS bytes of a block of one column: 24 of h, 24 of l
-template <bool ID, bool DW, bool ONE> __global__ void __launch_bounds__(512, ONE ? 4 : DW ? 3 : 2) k_mx_vec(const mx_mm p, const tdesc b, const tdesc ids, const int chunk) {
+template <bool ID, bool DW, bool ONE> __global__ void __launch_bounds__(512, ONE ? 4 : 2) k_mx_vec(const mx_mm p, const tdesc b, const tdesc ids, const int chunk) {
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ int s_cols[64];
     __shared__ int64_t s_at[64];  // where the workgroup's columns start in b
@@ -518,7 +519,7 @@ template <bool ID, bool DW, bool ONE> __global__ void __launch_bounds__(512, ONE
                 if (j == 1) { MX_MFMA(16x16x128, acc, a, sw, 1, h, l, sx, sl) }
                 if (j == 2) { MX_MFMA(16x16x128, acc, a, sw, 2, h, l, sx, sl) }
                 if (j == 3) { MX_MFMA(16x16x128, acc, a, sw, 3, h, l, sx, sl) }
-                if (j & 1) __builtin_amdgcn_sched_barrier(0);  // (the digits of all four blocks at a time would cost a third of the waves)
+                if (j & 1) __builtin_amdgcn_sched_barrier(0);  // (two blocks' digits at a time: fewer registers)
             }
         };
         if (ONE && wave * 4 < p.steps) add(step, f0);

@@ -7,6 +7,7 @@ import subprocess
 import pytest
 
 import llama_box_amd as L
+from test_host_and_abi import built_kernels
 
 OBJDUMP = "/opt/rocm/llvm/bin/llvm-objdump"
 
@@ -58,6 +59,12 @@ def listing(built, tmp_path_factory):
     path.write_bytes(elfs[0])
     text = subprocess.run([OBJDUMP, "-d", "--mcpu=gfx950", str(path)], capture_output=True, text=True, check=True).stdout
     return {m[1]: m[2].splitlines() for m in re.finditer(r"<(\w+)>:\n(.*?)(?=\n\n|\Z)", text, re.S)}
+
+
+def test_no_scratch(built):
+    """no MXFP4 kernel spills: a launch with a scratch frame pays for it at every dispatch, and the frame is read back ahead of the first weights"""
+    kernels = {name: m for name, m in built_kernels().items() if re.search(r"k_mx_|k_add_id", name)}
+    assert len(kernels) > 20 and not {name: m[".private_segment_fixed_size"] for name, m in kernels.items() if m[".private_segment_fixed_size"]}
 
 
 def test_results_stay_in_reach_of_their_reader(listing):
