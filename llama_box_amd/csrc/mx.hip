@@ -438,8 +438,8 @@ template <> struct mx_raw<false> {
 
 // ---- one to a few columns: 16 rows a workgroup, its waves take four steps of 128 values in turn.  The workgroup quantises its columns itself, behind the requests of its first weights (both are
 // there before the first product: requests complete in order).  A lane of
-// v_mfma_scale_f32_16x16x128: row (column) lane % 16, step lane / 16 of the four.  The weights' bytes bound it, behind the launch (us, with the 3.5 of a step's one launch: one column of 14336 x 4096,
-// 31 MB, 10.2; of 4096 x 4096 4.5; a token's 4 experts of 2048 x 4096, 18 MB, 6.6).  ONE: a wave has one turn, and no registers for the weights of a second (half as many, twice the waves: 8.7 us)
+// v_mfma_scale_f32_16x16x128: row (column) lane % 16, step lane / 16 of the four.  The weights' bytes bound it, behind the launch (us, with the 4 that a graph of one small launch takes: one column of 14336 x 4096,
+// 31 MB, 9.9; of 4096 x 4096 4.8; a token's 4 experts of 2048 x 4096, 18 MB, 6.9).  ONE: a wave has one turn, and no registers for the weights of a second (half as many, twice the waves: 8.7 us)
 // ID: blockIdx.y is a column (u + n_used t) of at most 64; the first column of an expert takes all of its expert, the others' workgroups end at once.
 static constexpr int MX_VEC_REC = 48;     // LDS bytes of a block of one column: 24 of h, 24 of l
 template <bool ID, bool DW, bool ONE> __global__ void __launch_bounds__(512, ONE ? 4 : 2) k_mx_vec(const mx_mm p, const tdesc b, const tdesc ids, const int chunk) {
@@ -541,7 +541,7 @@ template <bool ID, bool DW, bool ONE> __global__ void __launch_bounds__(512, ONE
 }
 
 // ---- a few groups of columns: 32 rows by one group a workgroup, its waves take two steps in turn, everything straight from memory; the waves' sums are added in LDS in their order.  (Two groups a
-// workgroup would read the weights once for both; their digits do not fit in registers beside the weights of two turns: 64 columns of 4096 x 4096 22.4 us, 11.8 like this)
+// workgroup would read the weights once for both; their digits do not fit in registers beside the weights of two turns: 64 columns of 4096 x 4096 22.4 us, 12.2 like this)
 template <bool ID, bool DW> __global__ void __launch_bounds__(512) k_mx_few(const mx_mm p) {
     extern __shared__ __align__(16) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, r32 = lane & 31, half = lane >> 5;
@@ -628,7 +628,7 @@ __device__ __forceinline__ bool mx_tile_of(const mx_mm & p, const int block, con
     return rt < row_tiles;
 }
 // MUL_MAT_ID: a tile of columns and all of its row tiles to one die, whose L2 then serves its digits; the tiles go to the dies in turn (us, row tiles to the dies in turn | tiles: 2048 tokens of 128 experts,
-// 8 each, of 1536 x 2048 199 | 189, 600 of 32, 4 each, of 1024 x 1024 29.6 | 27.6, 1000 of 4096 x 2048 115 | 117)
+// 8 each, of 1536 x 2048 187 | 183, 600 of 32, 4 each, of 1024 x 1024 29.2 | 27.5, 1000 of 4096 x 2048 104 | 98, of 2048 x 4096 105 | 106)
 __device__ __forceinline__ void mx_id_tile_of(const int row_tiles, int & rt, int & tile) {
     const int at = (int) (blockIdx.x >> 3);
     rt = at % row_tiles;
@@ -826,7 +826,7 @@ template <bool ID, int RT, bool DW> __global__ void __launch_bounds__(256, 2) k_
 }
 // ---- many columns of rows that are whole 16-byte pieces (K a multiple of 512: 272 bytes): as k_mx_tile, but the weights go to LDS by DMA as they lie in memory, 512 values a stage and row by row, and a
 // lane moves its codes into place behind its LDS read.  Eight waves: a group of columns has two, which take the even and the odd quarters of a row's stage (68 bytes, four blocks each) and add up at the
-// end; the second wave of a SIMD issues while the first one's product runs (one wave alone, eight blocks a stage: 512 columns 46 us).  512 / 1900 columns of 4096 x 14336: 43 / 145 us, 2.8 / 3.1 10^15
+// end; the second wave of a SIMD issues while the first one's product runs (one wave alone, eight blocks a stage: 512 columns 46 us).  512 / 1900 columns of 4096 x 14336: 43 / 150 us, 2.8 / 3.0 10^15
 // operations a second of the 7.9 that the instruction reaches alone: 3.6 us a stage, of which the matrix pipe works 51 % (2.25 GHz).  Without the DMA a stage takes 2.9 us, without the digits' loads 3.4,
 // without both 2.7: 170 KB a stage and CU on the one path from L2 (its address unit works 64 % of the time).  What left the time as it was: rows in LDS 144 bytes apart, without a bank conflict (whole
 // rows: half of LDS's cycles), and a product of another tile between the two of a tile.  In a quarter that starts at a unit of 8 bytes (the odd ones: at its
@@ -1086,16 +1086,17 @@ static void mx_launch_vec(hipStream_t s, const mx_mm & p, const tdesc & b, const
     else one ? (dw ? go(k_mx_vec<false, true, true>) : go(k_mx_vec<false, false, true>)) : dw ? go(k_mx_vec<false, true, false>) : go(k_mx_vec<false, false, false>);
 }
 // Costs of a product by k_mx_few and in tiles of 32 rt rows, in quarters of a us at 4096 values a row: 256 workgroups at a time, a tile's by its groups of columns.  What they compare, us, k_mx_few | tiles of 64
-// rows: 32 columns of 4096 x 14336 18.8 | 14.4, of 4096 x 32000 30.4 | 18.6, of 14336 x 8192 23.3 | 29.0, 64 of 4096 x 4096 11.8 | 14.7, 128 17.9 | 19.5, 256 29.7 | 21.2; 4 / 18 columns an expert, 32 experts
-// of 2048 x 4096 49 / 87 | 36 / 58, 8 of 2080 x 512 16.0 | 18.7.  Tiles of 64 | 128 | 256 rows: 256 columns of 4096 x 14336 35.9 | 26.6 | 34.8, 384 51.5 | 47.6 | 37.5
+// rows: 32 columns of 4096 x 14336 18.9 | 14.4, of 4096 x 32000 30.5 | 19.0, of 14336 x 8192 23.5 | 28.3, 64 of 4096 x 4096 12.2 | 14.4, 128 18.0 | 19.8, 256 29.8 | 21.3; 4 / 18 columns an expert, 32 experts
+// of 2048 x 4096 49 / 87 | 35 / 59.  (k_mx_tile's tiles of 64 rows take longer, which these costs leave out: 256 columns of 4224 x 2080 24.3 | 29.6.)  Tiles of 64 | 128 | 256 rows: 256 columns of
+// 4096 x 14336 32.5 | 28.6 | 34.8, 384 46.1 | 48.5 | 38.7
 static int64_t mx_few_cost(int64_t N, int64_t groups) { return ((N + 31) / 32 * groups + 255) / 256 * 22; }
 static int64_t mx_tile_cost(int rt, int64_t N, int64_t tiles, int64_t groups) {
     const int64_t rounds = ((N + 32 * rt - 1) / (32 * rt) * tiles + 255) / 256, g = std::min<int64_t>(groups, 4);
     return rounds * (rt == 2 ? 20 + 9 * g : rt == 4 ? 47 + 11 * g : 70 + 17 * g);
 }
 // A product in tiles of 256 rows whose last round of 256 workgroups is far from full: that round's rows in lower tiles where it ends earlier by the costs above.  -> the cost; low: their height (0: none), head:
-// the row tiles in front of them.  us, without | with: 640 columns of 4096 x 14336 72.6 | 62.1, 768 73.0 | 67.1, 1900 (840 tiles, or 765 and 150 of
-// 128 rows) 154 | 145, 2048 of 4096 x 5632 75.9 | 70.3, 2200 of 14336 x 4096 217 | 191
+// the row tiles in front of them.  us, without | with: 640 columns of 4096 x 14336 75.6 | 61.5, 768 75.7 | 67.4, 1900 (840 tiles, or 765 and 150 of
+// 128 rows) 158 | 153, 2048 of 4096 x 5632 79.4 | 70.7, 2200 of 14336 x 4096 216 | 190
 static int64_t mx_tail(int64_t N, int64_t tiles, int & head, int & low) {
     const int64_t all = (N + 255) / 256, whole = all * tiles / 256, full = std::min(all, whole * 256 / tiles), idle = whole * 256 - full * tiles, c8 = mx_tile_cost(8, N, tiles, 4);
     head = (int) all;
@@ -1145,8 +1146,8 @@ static int mx_tile_rows(const mx_mm & p, int64_t tiles, int64_t groups, int64_t 
     const int64_t c8 = N < 256 ? never : tail && groups >= 4 ? mx_tail(N, tiles, head, low) : mx_tile_cost(8, N, tiles, groups);
     return c8 <= c4 && c8 <= c2 ? 8 : c4 <= c2 ? 4 : 2;
 }
-// Four waves where the rows and groups alone fill the GPU, eight where they do not (us for 8 / 32 columns, four waves | eight: 4096 rows of 14336 18.3 / 21.2 | 18.6 / 20.3, 14336 of 4096 15.4 / 17.1 |
-// 17.4 / 18.5; 10 / 125 tokens of 32 experts of 4096 x 2048 32.8 / 71.5 | 43.9 / 90.1)
+// Four waves where the rows and groups alone fill the GPU, eight where they do not (us for 8 / 32 columns, four waves | eight: 4096 rows of 14336 19.7 / 22.0 | 20.2 / 22.1, 14336 of 4096 17.5 / 18.9 |
+// 20.3 / 21.4; 10 / 125 tokens of 32 experts of 4096 x 2048 37.6 / 75.8 | 47.6 / 93.3)
 template <bool ID> static void mx_launch_few(hipStream_t s, const mx_mm & p, int64_t groups) {
     const int waves = (p.n_rows + 31) / 32 * groups < 256 ? 8 : 4;
     const dim3 grid((unsigned) ((p.n_rows + 31) / 32), (unsigned) groups), block((unsigned) (64 * waves));
@@ -1160,7 +1161,7 @@ static int mx_form(const mx_mm & p) {
     return mx_few_cost(p.n_rows, groups) < mx_tile_cost(2, p.n_rows, tiles, groups) ? 0 : mx_tile_rows(p, tiles, groups, p.cols, mx_pieces(p));
 }
 // With fewer than 64 columns an expert the weights' way from memory counts for more than the products: of rows in whole pieces tiles of 256 rows where there are two rounds of them, of 64 (two workgroups a CU)
-// elsewhere.  us, 64 | 256 rows, 10 / 28 columns an expert: 32 experts of 2048 x 4096 44 / 68 | 46 / 56, of 1024 x 1024 15.7 / 19.6 | 20.6 / 23.4, 128 of 2048 x 768 40 / 51 | 48 / 55
+// elsewhere.  us, 64 | 256 rows, 10 / 28 columns an expert: 32 experts of 2048 x 4096 48 / 71 | 46 / 57, of 1024 x 1024 16.8 / 20.4 | 21.1 / 23.8, 128 of 2048 x 768 40 / 53 | 48 / 57
 static int mx_id_form(const mx_mm & p) {
     const int64_t g = mx_id_groups(p.n_expert, p.cols), tiles = mx_id_tiles(p.n_expert, p.cols), each = p.cols / p.n_expert;
     if (mx_few_cost(p.n_rows, g) < mx_tile_cost(2, p.n_rows, tiles, each / 32 + 1)) return 0;
@@ -1215,7 +1216,7 @@ bool mx_id_ok(const tdesc & w, const tdesc & ids) {
 }
 
 // ------------------------------------------------------------------------------------------------ ADD_ID
-// a [N, n_used, T] + the row of b [N, n_expert] that ids [n_used, T] names (an id outside them: a's row alone)
+// a [N, n_used, T] + the row of b [N, n_expert] that ids [n_used, T] names (an id outside them: a's row alone).  Bytes bound it behind the launch: 1000 tokens of 4 rows of 4096 32 us, 4.1 TB/s
 __global__ void __launch_bounds__(256) k_add_id(const tdesc a, const tdesc b, const tdesc ids, const tdesc d) {
     const int64_t u = blockIdx.y, t = blockIdx.z, n = (int64_t) blockIdx.x * 256 + threadIdx.x;
     if (n >= a.ne[0]) return;
